@@ -282,6 +282,109 @@ int ltx_attention_fwd(ltx_ctx *ctx, const void *q_dev, int64_t ldq, const void *
                       const void *v_dev, int64_t ldv, int32_t v_dtype, int32_t batch, int32_t heads,
                       int32_t tq, int32_t tk, int32_t head_dim, float scale, void *out_dev, int64_t ldo);
 
+/* ── packed batches: requests of unequal length behind one another ─────────── */
+
+/* Four building blocks for a batch of requests ("documents": clips, chunks,
+ * text contexts) whose rows lie one behind another in one buffer, without
+ * padding: the projection with each row's own low-rank adapter, the rotary
+ * tables, the per-head norm with the rotation, and attention in which no
+ * document sees another's keys.  The reference has no counterpart: it runs
+ * one request at a time, merges its adapters into the weights, and passes
+ * mask = None (crates/ltx-dit/src/attention.rs:228-285).  All of them are
+ * inference operators, take caller-owned buffers on the context's device,
+ * set the context's device for the call and restore the caller's, and may be
+ * captured into a CUDA graph.  Index arrays on the device are read as they
+ * are: every access they lead to stays inside the buffers whatever they hold,
+ * and a bad value is reported by the next ltx_ctx_synchronize. */
+
+/* Which two values of a head's rotated part form a pair. */
+typedef enum {
+    LTX_ROPE_HALF = 0,          /* (j, j + rot_dim/2), as apply_split_rope (rope.rs:231-257) */
+    LTX_ROPE_INTERLEAVED = 1    /* (2j, 2j + 1)                                              */
+} ltx_rope_layout;
+
+/* cos/sin of 1-D positions, f32 [rows, rot_dim/2]:
+ *   f_i = theta^(-2i/rot_dim)
+ *   g_i = f_i / factor                                     original_len == 0
+ *   g_i = f_i w_i + f_i/factor (1 - w_i)                   original_len > 0,
+ *         w_i = clamp((original_len f_i/2pi - turns_low) / (turns_high - turns_low), 0, 1)
+ *   cos_dev[r][i] = amplitude cos(pos[r] g_i), sin_dev the same.
+ * factor 1 is the plain table; a larger one stretches every frequency, or
+ * with original_len only those that turn fewer than turns_high times over it.
+ * pos_dev int32 [rows], NULL = 0, 1, 2, ...  The angle is formed and reduced
+ * in f64, so far positions keep f32's accuracy.  rot_dim even, 2..512. */
+int ltx_rope_table(ltx_ctx *ctx, const int32_t *pos_dev, int32_t rows, int32_t rot_dim, double theta, double factor,
+                   int64_t original_len, double turns_low, double turns_high, double amplitude, float *cos_dev,
+                   float *sin_dev);
+
+/* Per head of every row of q (heads) and k (kv_heads):
+ *   y = x / sqrt(mean(x^2) + eps) * gamma   over the head's head_dim values (norm != 0; gamma NULL = 1)
+ *   the first rot_dim values are rotated: (a, b) -> (c a - s b, s a + c b), pairs by `layout`
+ * (the model's own q_norm/k_norm span all heads, attention.rs:154-155; this
+ * is the form with one norm per head).  dtype LTX_BF16, LTX_F16 or LTX_F32
+ * for q, k and the outputs; gamma, cos and sin f32.  Head h is columns
+ * [h*head_dim, (h+1)*head_dim); leading dimensions in elements, any
+ * alignment of whole elements.  cos_dev/sin_dev [table_rows, rot_dim/2]; row
+ * r takes table row pos_dev[r] (NULL: r % table_rows); a position outside
+ * the table takes its nearest row and is reported as LTX_ERR_INVALID_ARG by
+ * the next ltx_ctx_synchronize.  rot_dim 0 (cos/sin NULL) rotates nothing.  k
+ * may be NULL with kv_heads 0.  An output may be its input (same pointer and
+ * leading dimension); otherwise it may not overlap one.  head_dim 1..512. */
+int ltx_qk_norm_rope(ltx_ctx *ctx, int32_t dtype, const void *q_dev, int64_t ldq, const void *k_dev, int64_t ldk,
+                     void *q_out_dev, int64_t ldqo, void *k_out_dev, int64_t ldko, int32_t rows, int32_t heads,
+                     int32_t kv_heads, int32_t head_dim, int32_t norm, float eps, const float *gamma_q_dev,
+                     const float *gamma_k_dev, const float *cos_dev, const float *sin_dev, int32_t table_rows,
+                     int32_t rot_dim, int32_t layout, const int32_t *pos_dev);
+
+/* out = epilogue(x[m,k] . W[n,k]^T + low) with low[r] = coeff[a] (x[r] . A_a^T) . B_a^T,
+ * a = adapter_idx[r]: the projection of ltx_gemm_bf16 with every row's own
+ * adapter added unmerged, for batches whose rows belong to requests with
+ * different LoRAs (merging serves one: ltx_store_merge_lora).  A negative
+ * index means no adapter; one >= adapters counts as none and is reported as
+ * LTX_ERR_INVALID_ARG by the next ltx_ctx_synchronize.  Indices may come in
+ * any order; rows of one request side by side run fastest.
+ *   lora_a_dev bf16 [adapters, rank, k], lora_b_dev bf16 [adapters, n, rank],
+ *   coeff_dev f32 [adapters] (ltx_lora_coeff); an adapter of lower rank is
+ *   padded with zero rows of A (or zero columns of B).  rank a multiple of 8
+ *   up to LTX_MAX_ADAPTER_RANK, at most LTX_MAX_ADAPTERS adapters.
+ * x, W, epilogue, bias, gate and out as ltx_gemm_bf16 (x/W rows 16-byte
+ * aligned, k a multiple of 8; out and gate rows of any alignment).  The
+ * low-rank sums stay in f32; for the f32 epilogues the product with B is
+ * taken in two bf16 parts that together keep 16 bits of it.  Scratch comes
+ * from the context's pool in stream order. */
+#define LTX_MAX_ADAPTERS 4096
+#define LTX_MAX_ADAPTER_RANK 256
+int ltx_gemm_adapters(ltx_ctx *ctx, const void *x_dev, int64_t ldx, const void *w_dev, int64_t ldw, int32_t m,
+                      int32_t n, int32_t k, int32_t epilogue, const float *bias_dev, void *out_dev, int64_t ldo,
+                      const float *gate_dev, const int32_t *gate_idx_dev, int64_t ld_gate,
+                      const int32_t *adapter_idx_dev, const void *lora_a_dev, const void *lora_b_dev,
+                      const float *coeff_dev, int32_t adapters, int32_t rank);
+
+/* out = softmax(s) v per head over packed documents: document i is rows
+ * [q_offsets[i], q_offsets[i+1]) of q and out and [k_offsets[i],
+ * k_offsets[i+1]) of k and v (int32 [docs+1], ascending, within rows_q /
+ * rows_k; a bad entry is cut to the buffers and reported as
+ * LTX_ERR_INVALID_ARG by the next ltx_ctx_synchronize).  Query i of a
+ * document with lq queries and lk keys stands beside key i + lk - lq: the
+ * two end together, so new tokens over cached ones are the last.
+ *   s_ij = scale q_i.k_j;  softcap > 0: s_ij = softcap tanh(s_ij / softcap)
+ *   slopes (f32 [heads], NULL = none): s_ij -= slopes[h] |i + lk - lq - j|
+ *   keys seen: all of the document; with causal != 0 those with
+ *   j <= i + lk - lq, and with prefix_dev (int32 [docs]) also j < prefix[doc].
+ * A row that sees no key gives 0; rows of out outside every document stay as
+ * they were.  heads a multiple of kv_heads (at most 128 times as many); head
+ * h reads key head h / (heads / kv_heads).  q/k/out bf16, v bf16 or f16 (with
+ * f16 the probabilities are kept in f16 too), row-major with leading
+ * dimensions in elements (multiples of 8, 16-byte aligned bases); head_dim 64
+ * or 128; out overlaps no input.  What k and v hold outside the documents, or
+ * in other documents, never reaches a row, NaN and infinities included; a
+ * non-finite v row inside a document may reach every row of the document. */
+int ltx_attention_packed_fwd(ltx_ctx *ctx, const void *q_dev, int64_t ldq, const void *k_dev, int64_t ldk,
+                             const void *v_dev, int64_t ldv, int32_t v_dtype, const int32_t *q_offsets_dev,
+                             const int32_t *k_offsets_dev, int32_t docs, int32_t rows_q, int32_t rows_k, int32_t heads,
+                             int32_t kv_heads, int32_t head_dim, float scale, float softcap, const float *slopes_dev,
+                             int32_t causal, const int32_t *prefix_dev, void *out_dev, int64_t ldo);
+
 /* ── ltx-weights: the weight store ─────────────────────────────────────────── */
 
 typedef struct ltx_store ltx_store;

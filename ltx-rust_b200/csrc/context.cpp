@@ -22,6 +22,30 @@ int ensure_scratch(ltx_ctx *ctx, size_t bytes) {
     return LTX_OK;
 }
 
+int work_alloc(ltx_ctx *ctx, size_t bytes, void **out) {
+    *out = nullptr;
+    if (!ctx->pool) {
+        cudaMemPoolProps props{};
+        props.allocType = cudaMemAllocationTypePinned;
+        props.location.type = cudaMemLocationTypeDevice;
+        props.location.id = ctx->device;
+        LTX_CUDA_TRY(ctx, cudaMemPoolCreate(&ctx->pool, &props));
+        uint64_t keep = ~0ull;   // freed blocks stay in the pool for the next call
+        LTX_CUDA_TRY(ctx, cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &keep));
+    }
+    const cudaError_t e = cudaMallocFromPoolAsync(out, bytes, ctx->pool, ctx->stream);
+    if (e == cudaErrorMemoryAllocation) {
+        cudaGetLastError();   // reported here, not by the next launch check
+        return fail(ctx, LTX_ERR_OOM, "workspace of %zu bytes: %s", bytes, cudaGetErrorString(e));
+    }
+    return e == cudaSuccess ? LTX_OK : cuda_fail(ctx, e, "workspace");
+}
+
+int work_free(ltx_ctx *ctx, void *p) {
+    if (p) LTX_CUDA_TRY(ctx, cudaFreeAsync(p, ctx->stream));
+    return LTX_OK;
+}
+
 int upload(ltx_ctx *ctx, void *dst_dev, const void *src_host, size_t bytes) {
     if (bytes == 0) return LTX_OK;
     // The staging buffer is reused: the previous upload must have left it.
@@ -75,6 +99,7 @@ extern "C" void ltx_ctx_destroy(ltx_ctx *ctx) {
     cudaSetDevice(ctx->device);
     cudaStreamSynchronize(ctx->stream);
     ltx::comm_release(ctx, false);
+    if (ctx->pool) cudaMemPoolDestroy(ctx->pool);
     if (ctx->scratch) cudaFree(ctx->scratch);
     if (ctx->work) cudaFree(ctx->work);
     if (ctx->pinned) cudaFreeHost(ctx->pinned);
@@ -103,6 +128,13 @@ extern "C" int ltx_ctx_synchronize(ltx_ctx *ctx) {
             return ltx::fail(ctx, LTX_ERR_UNSUPPORTED,
                              "a forward had more than %d distinct timesteps on the device (pass them from the host: "
                              "ltx_denoise_step's mask_host)", ltx::kMaxDistinctTs);
+        if (flag == ltx::kErrBadPosition)
+            return ltx::fail(ctx, LTX_ERR_INVALID_ARG, "qk_norm_rope: a position lies outside the cos/sin tables");
+        if (flag == ltx::kErrBadAdapter)
+            return ltx::fail(ctx, LTX_ERR_INVALID_ARG, "gemm_adapters: an adapter index lies beyond the pool");
+        if (flag == ltx::kErrBadOffsets)
+            return ltx::fail(ctx, LTX_ERR_INVALID_ARG,
+                             "attention_packed: document offsets descend or lie outside the rows");
         return ltx::fail(ctx, LTX_ERR_TIMEOUT, "a device-side wait gave up (code %d)", flag);
     }
     return LTX_OK;

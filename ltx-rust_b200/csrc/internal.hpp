@@ -57,6 +57,8 @@ struct ltx_ctx {
     // Forward/step workspace (activations), grown on demand and reused.
     void *work = nullptr;
     size_t work_bytes = 0;
+    // Pool of the per-call workspaces (work_alloc), made by the first of them.
+    cudaMemPool_t pool = nullptr;
     // Pinned host staging for the small per-call uploads (timestep index),
     // so they do not serialise the host with the stream.
     void *pinned = nullptr;
@@ -100,8 +102,29 @@ inline int cuda_fail(ltx_ctx *ctx, cudaError_t e, const char *what) {
     return fail(ctx, LTX_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
+// Makes the context's device current for the scope and puts the caller's back
+// (a launch on the default stream goes to the current device).
+struct DeviceGuard {
+    int prev = -1;
+    explicit DeviceGuard(const ltx_ctx *ctx) {
+        if (cudaGetDevice(&prev) != cudaSuccess || prev == ctx->device) prev = -1;
+        if (prev >= 0) cudaSetDevice(ctx->device);
+    }
+    ~DeviceGuard() {
+        if (prev >= 0) cudaSetDevice(prev);
+    }
+    DeviceGuard(const DeviceGuard &) = delete;
+    DeviceGuard &operator=(const DeviceGuard &) = delete;
+};
+
 // Makes sure ctx->scratch holds at least `bytes`; returns a status.
 int ensure_scratch(ltx_ctx *ctx, size_t bytes);
+// A workspace for one call, allocated and freed in the order of the context's
+// stream.  Unlike the scratch buffer it belongs to that call alone: one captured
+// into a CUDA graph is the graph's own, so graphs do not share it and nothing
+// frees it under them.
+int work_alloc(ltx_ctx *ctx, size_t bytes, void **out);
+int work_free(ltx_ctx *ctx, void *p);
 // Copies host bytes to the device through the context's pinned staging
 // buffer (waits for the previous upload from that buffer to finish first).
 int upload(ltx_ctx *ctx, void *dst_dev, const void *src_host, size_t bytes);

@@ -105,6 +105,11 @@ size_t cfg_scratch_bytes();
 // table; more than umax distinct values set *flag = code.
 constexpr int kMaxDistinctTs = 8;
 constexpr int kErrTooManyTimesteps = 1001;   // device error code: more distinct timesteps than kMaxDistinctTs
+// Device error codes of bad index values (packed batches): reported as
+// LTX_ERR_INVALID_ARG by ltx_ctx_synchronize.
+constexpr int kErrBadPosition = 1002;   // a rotary position outside its table
+constexpr int kErrBadAdapter = 1003;    // an adapter index beyond the pool
+constexpr int kErrBadOffsets = 1004;    // document offsets that descend or leave the buffer
 cudaError_t timestep_set(cudaStream_t st, const float *ts, int64_t rows, int umax, float *ts_u, int *idx, int *flag,
                          int code);
 // ts[h*T + t] = mask[t] * sigma for h < halves.

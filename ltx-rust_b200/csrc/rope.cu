@@ -1,0 +1,211 @@
+// Rotary positions for packed batches: the cos/sin tables of 1-D positions
+// (stretched for long contexts) and the per-head RMSNorm of queries and keys
+// with the rotation in the same pass.
+//
+// Both are bound by the bytes they move.  The table writes rot_dim * 4 bytes
+// per position; the norm reads and writes every query and key value once and
+// adds one table row per token.
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "device_common.cuh"
+#include "internal.hpp"
+#include "kernels.hpp"
+
+namespace ltx {
+
+namespace {
+
+constexpr int kMaxRot = 512, kMaxHeadDim = 512;
+
+// ── tables ───────────────────────────────────────────────────────────────────
+
+struct TableParams {
+    const int *pos;
+    int rows, half;
+    double log2_theta, inv_factor, orig_turns;   // orig_turns = original_len / 2pi, 0 = stretch every frequency
+    double turns_low, inv_span;
+    float amplitude;
+    float *cos_out, *sin_out;
+};
+
+// The angle in turns, pos * g_i / 2pi, is reduced to [-1/2, 1/2] in f64 (a
+// position of 2^24 has 2.7 million turns) and only the fraction goes to f32:
+// its rounding is at most 2^-26 turns, 1e-7 of the unit circle.
+__global__ void rope_table_1d_kernel(TableParams p) {
+    __shared__ double turns[kMaxRot / 2];
+    for (int i = threadIdx.x; i < p.half; i += blockDim.x) {
+        const double f = exp2(-p.log2_theta * i / p.half);   // theta^(-2i/rot)
+        const double w = p.orig_turns > 0 ? fmin(fmax((p.orig_turns * f - p.turns_low) * p.inv_span, 0.0), 1.0) : 0.0;
+        turns[i] = f * (w + (1.0 - w) * p.inv_factor) * 0.15915494309189533577;   // 1/2pi
+    }
+    __syncthreads();
+    const int64_t n = (int64_t)p.rows * p.half;
+    for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = e / p.half;
+        double t = (double)(p.pos ? p.pos[r] : (int)r) * turns[e - r * p.half];
+        t -= rint(t);
+        float s, c;
+        sincospif((float)(2.0 * t), &s, &c);
+        p.cos_out[e] = c * p.amplitude;
+        p.sin_out[e] = s * p.amplitude;
+    }
+}
+
+// ── per-head norm + rotation ─────────────────────────────────────────────────
+
+struct NormRopeParams {
+    const void *q, *k;
+    void *qo, *ko;
+    int64_t ldq, ldk, ldqo, ldko;
+    int rows, heads, kv_heads, d, norm;
+    float eps;
+    const float *gq, *gk, *cos_t, *sin_t;
+    int table_rows, half, interleaved;
+    const int *pos;
+    int *flag;
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) {
+    if constexpr (sizeof(T) == 4) return v;
+    else if constexpr (std::is_same_v<T, __half>) return __half2float(v);
+    else return __bfloat162float(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_f32(float v) {
+    if constexpr (sizeof(T) == 4) return v;
+    else if constexpr (std::is_same_v<T, __half>) return __float2half_rn(v);
+    else return __float2bfloat16_rn(v);
+}
+
+// The table row of token `row`: its position, or the row itself modulo the
+// table.  A position outside the table takes the nearest row and raises the flag.
+__device__ __forceinline__ int64_t table_row(const NormRopeParams &p, int row) {
+    if (!p.pos) return row % p.table_rows;
+    const int r = p.pos[row];
+    if ((unsigned)r >= (unsigned)p.table_rows) {
+        atomicExch(p.flag, kErrBadPosition);
+        return r < 0 ? 0 : p.table_rows - 1;
+    }
+    return r;
+}
+
+// Any head_dim, rot_dim, layout and alignment: one warp per (row, head), the
+// head in shared memory as f32 between the norm and the rotation.
+template <typename T>
+__global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(NormRopeParams p) {
+    __shared__ float xs[8][kMaxHeadDim];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int all = p.heads + p.kv_heads;
+    const int64_t item = (int64_t)blockIdx.x * 8 + warp;
+    if (item >= (int64_t)p.rows * all) return;
+    const int row = (int)(item / all), h = (int)(item % all);
+    const bool is_q = h < p.heads;
+    const int hh = is_q ? h : h - p.heads;
+    const T *x = static_cast<const T *>(is_q ? p.q : p.k) + (int64_t)row * (is_q ? p.ldq : p.ldk) + (int64_t)hh * p.d;
+    T *y = static_cast<T *>(is_q ? p.qo : p.ko) + (int64_t)row * (is_q ? p.ldqo : p.ldko) + (int64_t)hh * p.d;
+    const float *g = is_q ? p.gq : p.gk;
+    float *s = xs[warp];
+    float ss = 0.f;
+    for (int e = lane; e < p.d; e += 32) {
+        const float v = to_f32(x[e]);
+        s[e] = v;
+        ss += v * v;
+    }
+    float inv = 1.f;
+    if (p.norm) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        inv = 1.f / sqrtf(ss / (float)p.d + p.eps);
+        for (int e = lane; e < p.d; e += 32) s[e] *= g ? inv * g[e] : inv;
+    }
+    __syncwarp();
+    if (p.half) {
+        const int64_t tr = table_row(p, row) * p.half;
+        for (int j = lane; j < p.half; j += 32) {
+            const int a = p.interleaved ? 2 * j : j, b = p.interleaved ? 2 * j + 1 : j + p.half;
+            const float c = p.cos_t[tr + j], sn = p.sin_t[tr + j], u = s[a], v = s[b];
+            y[a] = from_f32<T>(c * u - sn * v);
+            y[b] = from_f32<T>(sn * u + c * v);
+        }
+    }
+    for (int e = 2 * p.half + lane; e < p.d; e += 32) y[e] = from_f32<T>(s[e]);
+}
+
+template <typename T>
+void launch_norm_rope(const NormRopeParams &p, cudaStream_t st) {
+    const int64_t items = (int64_t)p.rows * (p.heads + p.kv_heads);
+    qk_norm_rope_any_kernel<T><<<(unsigned)((items + 7) / 8), 256, 0, st>>>(p);
+}
+
+}  // namespace
+
+}  // namespace ltx
+
+extern "C" int ltx_rope_table(ltx_ctx *ctx, const int32_t *pos_dev, int32_t rows, int32_t rot_dim, double theta,
+                              double factor, int64_t original_len, double turns_low, double turns_high,
+                              double amplitude, float *cos_dev, float *sin_dev) {
+    using namespace ltx;
+    if (!ctx) return LTX_ERR_INVALID_ARG;
+    if (rows < 0 || rot_dim < 2 || rot_dim > kMaxRot || rot_dim % 2)
+        return fail(ctx, LTX_ERR_SHAPE, "rope_table: %d rows, rot_dim %d (even, 2..%d)", rows, rot_dim, kMaxRot);
+    if (!(theta > 0) || !std::isfinite(theta) || !(factor > 0) || !std::isfinite(factor) || !std::isfinite(amplitude) ||
+        original_len < 0)
+        return fail(ctx, LTX_ERR_INVALID_ARG, "rope_table: theta and factor must be finite and > 0, original_len >= 0");
+    if (original_len > 0 && !(turns_high > turns_low && std::isfinite(turns_high) && std::isfinite(turns_low)))
+        return fail(ctx, LTX_ERR_INVALID_ARG, "rope_table: turns_high must exceed turns_low");
+    if (rows == 0) return LTX_OK;
+    if (!cos_dev || !sin_dev) return fail(ctx, LTX_ERR_INVALID_ARG, "rope_table: null output");
+    DeviceGuard guard(ctx);
+    TableParams p{pos_dev, rows, rot_dim / 2, std::log2(theta), 1.0 / factor,
+                  (double)original_len * 0.15915494309189533577, turns_low,
+                  original_len > 0 ? 1.0 / (turns_high - turns_low) : 0.0, (float)amplitude, cos_dev, sin_dev};
+    const int64_t n = (int64_t)rows * p.half;
+    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((n + 255) / 256, (int64_t)ctx->sm_count * 8));
+    rope_table_1d_kernel<<<grid, 256, 0, ctx->stream>>>(p);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? LTX_OK : cuda_fail(ctx, e, "rope_table launch");
+}
+
+extern "C" int ltx_qk_norm_rope(ltx_ctx *ctx, int32_t dtype, const void *q_dev, int64_t ldq, const void *k_dev,
+                                int64_t ldk, void *q_out_dev, int64_t ldqo, void *k_out_dev, int64_t ldko, int32_t rows,
+                                int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t norm, float eps,
+                                const float *gamma_q_dev, const float *gamma_k_dev, const float *cos_dev,
+                                const float *sin_dev, int32_t table_rows, int32_t rot_dim, int32_t layout,
+                                const int32_t *pos_dev) {
+    using namespace ltx;
+    if (!ctx) return LTX_ERR_INVALID_ARG;
+    if (dtype != LTX_BF16 && dtype != LTX_F16 && dtype != LTX_F32)
+        return fail(ctx, LTX_ERR_DTYPE, "qk_norm_rope: dtype %d (BF16, F16 or F32)", dtype);
+    if (rows < 0 || heads < 0 || kv_heads < 0 || head_dim < 1 || head_dim > kMaxHeadDim)
+        return fail(ctx, LTX_ERR_SHAPE, "qk_norm_rope: %d rows, %d + %d heads of %d (1..%d)", rows, heads, kv_heads,
+                    head_dim, kMaxHeadDim);
+    if (rot_dim < 0 || rot_dim > head_dim || rot_dim % 2)
+        return fail(ctx, LTX_ERR_SHAPE, "qk_norm_rope: rot_dim %d must be even and at most head_dim %d", rot_dim, head_dim);
+    if (layout != LTX_ROPE_HALF && layout != LTX_ROPE_INTERLEAVED)
+        return fail(ctx, LTX_ERR_INVALID_ARG, "qk_norm_rope: bad layout %d", layout);
+    if (norm && !(eps >= 0.f && std::isfinite(eps)))
+        return fail(ctx, LTX_ERR_INVALID_ARG, "qk_norm_rope: eps must be finite and >= 0");
+    if (rot_dim > 0 && (!cos_dev || !sin_dev || table_rows < 1))
+        return fail(ctx, LTX_ERR_INVALID_ARG, "qk_norm_rope: a rotation needs cos/sin tables with at least one row");
+    const int64_t qc = (int64_t)heads * head_dim, kc = (int64_t)kv_heads * head_dim;
+    if (rows == 0 || qc + kc == 0) return LTX_OK;
+    if ((heads && (!q_dev || !q_out_dev)) || (kv_heads && (!k_dev || !k_out_dev)))
+        return fail(ctx, LTX_ERR_INVALID_ARG, "qk_norm_rope: null q or k");
+    if ((heads && (ldq < qc || ldqo < qc)) || (kv_heads && (ldk < kc || ldko < kc)))
+        return fail(ctx, LTX_ERR_SHAPE, "qk_norm_rope: leading dimensions shorter than the heads");
+    if ((int64_t)rows * (heads + (int64_t)kv_heads) > (int64_t)1 << 33)
+        return fail(ctx, LTX_ERR_UNSUPPORTED, "qk_norm_rope: more than 2^33 heads in one call");
+    DeviceGuard guard(ctx);
+    NormRopeParams p{q_dev, k_dev, q_out_dev, k_out_dev, ldq, ldk, ldqo, ldko, rows, heads, kv_heads, head_dim, norm,
+                     eps, gamma_q_dev, gamma_k_dev, cos_dev, sin_dev, table_rows, rot_dim / 2,
+                     layout == LTX_ROPE_INTERLEAVED, pos_dev, ctx->timeout_flag};
+    if (dtype == LTX_F32) launch_norm_rope<float>(p, ctx->stream);
+    else if (dtype == LTX_F16) launch_norm_rope<__half>(p, ctx->stream);
+    else launch_norm_rope<__nv_bfloat16>(p, ctx->stream);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? LTX_OK : cuda_fail(ctx, e, "qk_norm_rope launch");
+}

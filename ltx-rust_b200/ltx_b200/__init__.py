@@ -75,6 +75,14 @@ def lib() -> ctypes.CDLL:
         "ltx_quantize_rows_e4m3": (I, [V, P, I64, ctypes.c_int32, ctypes.c_int32, P, I64, P]),
         "ltx_attention_fwd": (I, [V, P, I64, P, I64, P, I64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
                                   ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, F, P, I64]),
+        "ltx_rope_table": (I, [V, P, ctypes.c_int32, ctypes.c_int32, ctypes.c_double, ctypes.c_double, I64,
+                               ctypes.c_double, ctypes.c_double, ctypes.c_double, P, P]),
+        "ltx_qk_norm_rope": (I, [V, ctypes.c_int32, P, I64, P, I64, P, I64, P, I64] + [ctypes.c_int32] * 5 +
+                             [F, P, P, P, P, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, P]),
+        "ltx_gemm_adapters": (I, [V, P, I64, P, I64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, P,
+                                  P, I64, P, P, I64, P, P, P, P, ctypes.c_int32, ctypes.c_int32]),
+        "ltx_attention_packed_fwd": (I, [V, P, I64, P, I64, P, I64, ctypes.c_int32, P, P] + [ctypes.c_int32] * 6 +
+                                     [F, F, P, ctypes.c_int32, P, P, I64]),
         "ltx_store_open": (I, [V, ctypes.POINTER(ctypes.c_char_p), ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(V)]),
         "ltx_store_destroy": (None, [V]),
         "ltx_store_merge_lora": (I, [V, ctypes.c_char_p, F, ctypes.POINTER(ctypes.c_int32),
@@ -141,6 +149,7 @@ class Context:
             import torch
             stream = torch.cuda.current_stream(device).cuda_stream
         self.h = ctypes.c_void_p()
+        self.device = device
         # stores and models made on this context: closed before it (their
         # destructors synchronise on the context's stream)
         self._owned = weakref.WeakSet()
@@ -252,6 +261,132 @@ def attention(ctx: "Context", q, k, v, out, batch, heads, tq, tk, scale, head_di
     ctx.check(lib().ltx_attention_fwd(ctx.h, _ptr(q), q.stride(0), _ptr(k), k.stride(0), _ptr(v), v.stride(0), vdt,
                                       batch, heads, tq, tk, head_dim, scale, _ptr(out), out.stride(0)),
               "ltx_attention_fwd")
+
+
+# ── packed batches ─────────────────────────────────────────────────────────────
+
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+
+
+def _want(ctx: "Context", what, t, name, dtypes, ndim, rows=None, cols=None, dense=False):
+    """Raises LtxError unless t is a CUDA tensor of the context's device with one of `dtypes`, `ndim` dimensions, the
+    given first / last sizes and a contiguous last dimension (dense: contiguous altogether)."""
+    if not t.is_cuda or t.device.index != ctx.device:
+        raise LtxError(1, f"{what}: {name} must be on cuda:{ctx.device}, not {t.device}")
+    if t.dtype not in dtypes:
+        raise LtxError(3, f"{what}: {name} is {t.dtype}, not {' or '.join(str(d) for d in dtypes)}")
+    if t.dim() != ndim or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[-1] != cols):
+        raise LtxError(2, f"{what}: {name} has shape {tuple(t.shape)}")
+    if dense and not t.is_contiguous():
+        raise LtxError(2, f"{what}: {name} must be contiguous")
+    if t.numel() and ((t.shape[-1] > 1 and t.stride(-1) != 1) or (ndim == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+        raise LtxError(2, f"{what}: {name} needs contiguous, non-overlapping rows")
+
+
+def _ld(t):
+    """Leading dimension of a 2-D tensor; a single row's stride says nothing, so its length stands for it."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+
+
+def rope_table(ctx: "Context", pos, cos, sin, theta=10000.0, factor=1.0, original_len=0, turns_low=1.0, turns_high=32.0,
+               amplitude=1.0):
+    """cos/sin f32 [rows, rot_dim/2] of int32 positions [rows] (None: 0, 1, 2, ...), stretched by `factor`
+    (ltx_rope_table)."""
+    import torch
+    rows, half = cos.shape
+    _want(ctx, "rope_table", cos, "cos", (torch.float32,), 2, dense=True)
+    _want(ctx, "rope_table", sin, "sin", (torch.float32,), 2, rows, half, dense=True)
+    if pos is not None:
+        _want(ctx, "rope_table", pos, "pos", (torch.int32,), 1, rows, dense=True)
+    ctx.check(lib().ltx_rope_table(ctx.h, _ptr(pos), rows, 2 * half, theta, factor, original_len, turns_low, turns_high,
+                                   amplitude, _ptr(cos), _ptr(sin)), "ltx_rope_table")
+
+
+def qk_norm_rope(ctx: "Context", q, k, q_out, k_out, heads, kv_heads, cos, sin, pos=None, gamma_q=None, gamma_k=None,
+                 norm=True, eps=1e-6, layout=ROPE_HALF):
+    """Per-head RMSNorm of q [rows, heads*d] and k [rows, kv_heads*d] (k None with kv_heads 0) and the rotation of
+    each head's first values by cos/sin [table_rows, rot_dim/2] (None: no rotation), row r at table row pos[r]
+    (ltx_qk_norm_rope).  q_out / k_out may be q / k."""
+    import torch
+    what, rows = "qk_norm_rope", q.shape[0]
+    d = q.shape[-1] // max(heads, 1)
+    types = {torch.bfloat16: LTX_BF16, torch.float16: LTX_F16, torch.float32: LTX_F32}
+    _want(ctx, what, q, "q", tuple(types), 2, cols=heads * d)
+    _want(ctx, what, q_out, "q_out", (q.dtype,), 2, rows, heads * d)
+    if kv_heads:
+        _want(ctx, what, k, "k", (q.dtype,), 2, rows, kv_heads * d)
+        _want(ctx, what, k_out, "k_out", (q.dtype,), 2, rows, kv_heads * d)
+    for g, name in ((gamma_q, "gamma_q"), (gamma_k, "gamma_k")):
+        if g is not None:
+            _want(ctx, what, g, name, (torch.float32,), 1, d, dense=True)
+    half = table = 0
+    if cos is not None:
+        table, half = cos.shape
+        _want(ctx, what, cos, "cos", (torch.float32,), 2, dense=True)
+        _want(ctx, what, sin, "sin", (torch.float32,), 2, table, half, dense=True)
+    if pos is not None:
+        _want(ctx, what, pos, "pos", (torch.int32,), 1, rows, dense=True)
+    kp, kl, kop, kol = (_ptr(k), _ld(k), _ptr(k_out), _ld(k_out)) if kv_heads else (None, 0, None, 0)
+    ctx.check(lib().ltx_qk_norm_rope(ctx.h, types[q.dtype], _ptr(q), _ld(q), kp, kl, _ptr(q_out), _ld(q_out), kop, kol,
+                                     rows, heads, kv_heads, d, int(norm), eps, _ptr(gamma_q), _ptr(gamma_k), _ptr(cos),
+                                     _ptr(sin), table, 2 * half, layout, _ptr(pos)), "ltx_qk_norm_rope")
+
+
+def gemm_adapters(ctx: "Context", x, w, out, adapter_idx, lora_a, lora_b, coeff, epilogue=EPI_BF16, bias=None,
+                  gate=None, gate_idx=None):
+    """out = epilogue(x @ w.T + coeff[a] (x @ lora_a[a].T) @ lora_b[a].T) with a = adapter_idx[row], -1 for none
+    (ltx_gemm_adapters): x [M,K], w [N,K], lora_a [adapters,rank,K], lora_b [adapters,N,rank] bf16, coeff f32,
+    adapter_idx int32 [M], out bf16 or (EPI_F32, EPI_RESID) f32 [M,N]."""
+    import torch
+    what, (M, K), N = "gemm_adapters", x.shape, w.shape[0]
+    bf, f32, i32 = (torch.bfloat16,), (torch.float32,), (torch.int32,)
+    _want(ctx, what, x, "x", bf, 2)
+    _want(ctx, what, w, "w", bf, 2, cols=K)
+    _want(ctx, what, out, "out", f32 if epilogue in (EPI_F32, EPI_RESID) else bf, 2, M, N)
+    _want(ctx, what, adapter_idx, "adapter_idx", i32, 1, M, dense=True)
+    _want(ctx, what, lora_a, "lora_a", bf, 3, cols=K, dense=True)
+    n, rank = lora_a.shape[:2]
+    _want(ctx, what, lora_b, "lora_b", bf, 3, n, rank, dense=True)
+    if lora_b.shape[1] != N:
+        raise LtxError(2, f"{what}: lora_b has shape {tuple(lora_b.shape)}")
+    _want(ctx, what, coeff, "coeff", f32, 1, n, dense=True)
+    if bias is not None:
+        _want(ctx, what, bias, "bias", f32, 1, N, dense=True)
+    if gate is not None:
+        _want(ctx, what, gate, "gate", f32, 2, cols=N)
+    if gate_idx is not None:
+        _want(ctx, what, gate_idx, "gate_idx", i32, 1, M, dense=True)
+    ctx.check(lib().ltx_gemm_adapters(ctx.h, _ptr(x), _ld(x), _ptr(w), _ld(w), M, N, K, epilogue, _ptr(bias), _ptr(out),
+                                      _ld(out), _ptr(gate), _ptr(gate_idx), _ld(gate) if gate is not None else 0,
+                                      _ptr(adapter_idx), _ptr(lora_a), _ptr(lora_b), _ptr(coeff), n, rank),
+              "ltx_gemm_adapters")
+
+
+def attention_packed(ctx: "Context", q, k, v, out, q_offsets, k_offsets, heads, kv_heads, scale, head_dim=128,
+                     softcap=0.0, slopes=None, causal=False, prefix=None):
+    """out = softmax over the row's own document's keys (ltx_attention_packed_fwd): q/out [rows_q, heads*head_dim] and
+    k/v [rows_k, kv_heads*head_dim] bf16 (v bf16 or f16), document i at rows q_offsets[i]:q_offsets[i+1] and
+    k_offsets[i]:k_offsets[i+1] (int32 CUDA [docs+1]); slopes f32 [heads], prefix int32 [docs] (with causal)."""
+    import torch
+    what, docs = "attention_packed", q_offsets.shape[0] - 1
+    if docs < 0:
+        raise LtxError(2, f"{what}: q_offsets needs docs + 1 entries")
+    bf, i32 = (torch.bfloat16,), (torch.int32,)
+    _want(ctx, what, q, "q", bf, 2, cols=heads * head_dim)
+    _want(ctx, what, out, "out", bf, 2, q.shape[0], heads * head_dim)
+    _want(ctx, what, k, "k", bf, 2, cols=kv_heads * head_dim)
+    _want(ctx, what, v, "v", (torch.bfloat16, torch.float16), 2, k.shape[0], kv_heads * head_dim)
+    _want(ctx, what, q_offsets, "q_offsets", i32, 1, dense=True)
+    _want(ctx, what, k_offsets, "k_offsets", i32, 1, docs + 1, dense=True)
+    if slopes is not None:
+        _want(ctx, what, slopes, "slopes", (torch.float32,), 1, heads, dense=True)
+    if prefix is not None:
+        _want(ctx, what, prefix, "prefix", i32, 1, docs, dense=True)
+    ctx.check(lib().ltx_attention_packed_fwd(ctx.h, _ptr(q), _ld(q), _ptr(k), _ld(k), _ptr(v), _ld(v),
+                                             LTX_F16 if v.dtype == torch.float16 else LTX_BF16, _ptr(q_offsets),
+                                             _ptr(k_offsets), docs, q.shape[0], k.shape[0], heads, kv_heads, head_dim,
+                                             scale, softcap, _ptr(slopes), int(causal), _ptr(prefix), _ptr(out),
+                                             _ld(out)), "ltx_attention_packed_fwd")
 
 
 KEYMAP_IDENTITY, KEYMAP_TRANSFORMER = 0, 1
