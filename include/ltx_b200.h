@@ -352,7 +352,7 @@ int ltx_qk_norm_rope(ltx_ctx *ctx, int32_t dtype, const void *q_dev, int64_t ldq
  * low-rank sums stay in f32; for the f32 epilogues the product with B is
  * taken in two bf16 parts that together keep 16 bits of it.  Scratch comes
  * from the context's pool in stream order. */
-#define LTX_MAX_ADAPTERS 4096
+#define LTX_MAX_ADAPTERS 2048
 #define LTX_MAX_ADAPTER_RANK 256
 int ltx_gemm_adapters(ltx_ctx *ctx, const void *x_dev, int64_t ldx, const void *w_dev, int64_t ldw, int32_t m,
                       int32_t n, int32_t k, int32_t epilogue, const float *bias_dev, void *out_dev, int64_t ldo,

@@ -1,8 +1,20 @@
 // Projection with one low-rank adapter per row:
 //   out[m] = epilogue(x[m] W^T + c_a (x[m] A_a^T) B_a^T),  a = idx[m].
 //
-// The simplest form: one kernel for the low-rank products low[m] = c_a x[m]
-// A_a^T in f32 (a warp per value), one tiled f32 kernel for everything else.
+// Two kernels.  low_kernel forms low[m] = c_a x[m] A_a^T, a tenth of a percent
+// to a few percent of the work, and keeps it as bf16 (f32 epilogues: two bf16
+// parts).  project_kernel is the shared projection with low as more of its K
+// loop: for every adapter a in a tile of tokens, one more block multiplies
+// B_a's rows by low with the rows of other adapters set to 0, into the same
+// f32 accumulator.  So an adapter costs rank / 64 blocks beside the K / 64
+// that every tile has, whatever the order of the rows.
+//
+// Both work on D[128 weight rows, TN tokens]: weight rows are the MMA's M, so
+// few tokens (TN 16) cost no wasted rows and the weights stream at HBM's rate,
+// and many (TN 256) give the widest tile.
+#include <cuda.h>
+
+#include <algorithm>
 #include <cmath>
 
 #include "device_common.cuh"
@@ -13,82 +25,692 @@ namespace ltx {
 
 namespace {
 
+constexpr int BM = 128;             // weight rows of a tile
+constexpr int kMaxWords = LTX_MAX_ADAPTERS / 32;
+
 struct AdapterParams {
-    const __nv_bfloat16 *x, *w, *a, *b;
-    int64_t ldx, ldw, ldo, ld_gate;
-    int m, n, k, rank, adapters, epilogue;
+    int m, n, k, rank, adapters, rank_blocks, parts, splits, m_tiles, n_tiles, group_m, tok_lanes;
     const int *idx, *gate_idx;
     const float *coeff, *bias, *gate;
-    float *low;   // [m, rank]
+    int64_t ldo, ld_gate;
+    __nv_bfloat16 *low;   // [parts][m][rank_blocks * 64]
     void *out;
     int *flag;
 };
 
-// The adapter of row m, -1 for none; an index beyond the pool counts as none
-// and raises the flag.
-__device__ __forceinline__ int adapter_of(const AdapterParams &p, int m) {
-    const int a = p.idx[m];
-    if (a >= p.adapters) {
-        atomicExch(p.flag, kErrBadAdapter);
-        return -1;
-    }
-    return a < 0 ? -1 : a;
+// The threads of a list builder: one warp, or four on named barrier 1.
+template <int NT>
+__device__ __forceinline__ void builder_sync() {
+    if constexpr (NT == 32) __syncwarp();
+    else asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
 }
+__device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_peer(const float *smem, uint32_t rank) {
+    uint32_t a;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(smem)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+// Programmatic dependent launch: project_kernel starts beside low_kernel and
+// waits for it only where it reads low.
+__device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-__global__ void low_kernel(AdapterParams p) {
-    const int lane = threadIdx.x & 31;
-    const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    if (item >= (int64_t)p.m * p.rank) return;
-    const int m = (int)(item / p.rank), r = (int)(item % p.rank), a = adapter_of(p, m);
-    float s = 0.f;
-    if (a >= 0) {
-        const __nv_bfloat16 *ar = p.a + ((int64_t)a * p.rank + r) * p.k, *xr = p.x + m * p.ldx;
-        for (int e = lane; e < p.k; e += 32) s += __bfloat162float(ar[e]) * __bfloat162float(xr[e]);
+// The adapters of a tile of tokens.
+template <int TN>
+struct TileList {
+    int count;
+    uint16_t ids[TN];   // ascending
+};
+template <int TN>
+struct ListScratch {
+    uint32_t bits[kMaxWords];
+    int sums[4];
+    int16_t tok[TN];    // each token's adapter, -1 for none
+};
+
+// Fills `l` and `s.tok` for tokens [m0, m0 + TN), by NT threads (tid of them).  An index beyond the pool counts as none and raises the
+// flag.
+template <int TN, int NT>
+__device__ __forceinline__ void build_list(const AdapterParams &p, int m0, int tid, TileList<TN> &l,
+                                           ListScratch<TN> &s) {
+    constexpr int W = (kMaxWords + NT - 1) / NT;   // words of the bit set for each thread
+    for (int i = tid; i < kMaxWords; i += NT) s.bits[i] = 0;
+    builder_sync<NT>();
+    for (int i = tid; i < TN; i += NT) {
+        int a = m0 + i < p.m ? p.idx[m0 + i] : -1;
+        if (a >= p.adapters) {
+            atomicExch(p.flag, kErrBadAdapter);
+            a = -1;
+        }
+        s.tok[i] = (int16_t)max(a, -1);
+        if (a >= 0) atomicOr(&s.bits[a >> 5], 1u << (a & 31));
+    }
+    builder_sync<NT>();
+    uint32_t w[W];
+    int n = 0;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        s *= p.coeff[a];
+    for (int i = 0; i < W; ++i) n += __popc(w[i] = tid * W + i < kMaxWords ? s.bits[tid * W + i] : 0u);
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if ((tid & 31) >= o) incl += v;
     }
-    if (lane == 0) p.low[item] = s;
+    if ((tid & 31) == 31) s.sums[tid >> 5] = incl;
+    builder_sync<NT>();
+    int at = incl - n;
+    for (int i = 0; i < (tid >> 5); ++i) at += s.sums[i];
+    if (tid == NT - 1) l.count = at + n;
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+        for (uint32_t b = w[i]; b; b &= b - 1) l.ids[at++] = (uint16_t)((tid * W + i) * 32 + __ffs(b) - 1);
+    builder_sync<NT>();
 }
 
-__global__ void __launch_bounds__(256) adapter_tile_kernel(AdapterParams p) {
-    __shared__ float xs[64][33], ws[64][33];
-    const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < p.k; k0 += 32) {
-        __syncthreads();
-        for (int e = threadIdx.x; e < 64 * 32; e += 256) {
-            const int r = e >> 5, c = e & 31;
-            xs[r][c] = m0 + r < p.m && k0 + c < p.k ? __bfloat162float(p.x[(int64_t)(m0 + r) * p.ldx + k0 + c]) : 0.f;
-            ws[r][c] = n0 + r < p.n && k0 + c < p.k ? __bfloat162float(p.w[(int64_t)(n0 + r) * p.ldw + k0 + c]) : 0.f;
+// Splits v into bf16 parts hi + lo: together 16 significant bits.
+__device__ __forceinline__ void split_bf16(float v, __nv_bfloat16 &hi, __nv_bfloat16 &lo) {
+    hi = __float2bfloat16_rn(v);
+    lo = __float2bfloat16_rn(v - __bfloat162float(hi));
+}
+
+// ── low[m] = c_a x[m] A_a^T ──────────────────────────────────────────────────
+//
+// One cluster of `splits` CTAs per (tile of TN tokens, lane of its adapters):
+// D[rank, TN] = A_a . x^T over the cluster's shares of K, joined in the order
+// of the ranks.  tok_lanes CTAs share a tile's adapters when tiles are few.
+
+template <int TN>
+struct LowCfg {
+    static constexpr int A_BYTES = BM * 128, STAGE = A_BYTES + TN * 128;
+    static constexpr int STAGES = TN >= 128 ? 3 : 4;   // two CTAs per SM
+    static constexpr int RING = STAGES * STAGE;
+    static constexpr int LIST = RING + 256;
+    static constexpr int BYTES = 1024 + LIST + (int)sizeof(TileList<TN>) + (int)sizeof(ListScratch<TN>);
+    static constexpr int COLS = TN < 32 ? 32 : TN;
+    static_assert(TN * BM * 4 <= RING, "the f32 partials fit the ring");
+};
+constexpr int kLowThreads = 192;
+
+template <int TN>
+__global__ void __launch_bounds__(kLowThreads)
+    low_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmX, AdapterParams p) {
+    using C = LowCfg<TN>;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::RING), *empty = full + C::STAGES, *done = empty + C::STAGES;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
+    TileList<TN> &list = *reinterpret_cast<TileList<TN> *>(smem + C::LIST);
+    ListScratch<TN> &scratch = *reinterpret_cast<ListScratch<TN> *>(smem + C::LIST + sizeof(TileList<TN>));
+    float *part = reinterpret_cast<float *>(smem);   // [TN][128], in the ring's place
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = blockIdx.x % p.splits, job = blockIdx.x / p.splits;
+    const int m0 = job / p.tok_lanes * TN, tok_lane = job % p.tok_lanes;
+    grid_dep_launch();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
         }
-        __syncthreads();
-        for (int c = 0; c < 32; ++c)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) acc[i][j] += xs[ty * 4 + i][c] * ws[tx + 16 * j][c];
+        mbar_init(done, 1);
+        fence_barrier_init();
     }
-    for (int i = 0; i < 4; ++i) {
-        const int m = m0 + ty * 4 + i;
-        if (m >= p.m) continue;
-        const int a = adapter_of(p, m);
-        for (int j = 0; j < 4; ++j) {
-            const int n = n0 + tx + 16 * j;
-            if (n >= p.n) continue;
-            float y = acc[i][j];
-            if (a >= 0)
-                for (int r = 0; r < p.rank; ++r)
-                    y += p.low[(int64_t)m * p.rank + r] * __bfloat162float(p.b[((int64_t)a * p.n + n) * p.rank + r]);
-            if (p.bias) y += p.bias[n];
-            if (p.epilogue == LTX_EPI_GELU_BF16)
-                y = 0.5f * y * (1.f + tanhf(0.7978845608028654f * (y + 0.044715f * y * y * y)));
-            const int64_t at = (int64_t)m * p.ldo + n;
-            if (p.epilogue == LTX_EPI_F32) static_cast<float *>(p.out)[at] = y;
-            else if (p.epilogue == LTX_EPI_RESID)
-                static_cast<float *>(p.out)[at] +=
-                    p.gate ? y * p.gate[(int64_t)(p.gate_idx ? p.gate_idx[m] : 0) * p.ld_gate + n] : y;
-            else static_cast<__nv_bfloat16 *>(p.out)[at] = __float2bfloat16_rn(y);
+    if (warp == 0) {
+        tmem_alloc(tmem_slot, C::COLS);
+        tmem_relinquish();
+    }
+    if (warp >= 2) build_list<TN, 128>(p, m0, threadIdx.x - 64, list, scratch);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    bool aborted = false;
+
+    const int kb = (p.k + 63) / 64;
+    const int k0 = (int)((int64_t)kb * split / p.splits), k1 = (int)((int64_t)kb * (split + 1) / p.splits);
+    const int m_blocks = (p.rank + BM - 1) / BM, units = list.count * m_blocks;   // (adapter, 128 of its ranks)
+    const int box = min(p.rank, BM);
+    uint32_t it = 0, turn = 0;
+    for (int u = tok_lane; u < units; u += p.tok_lanes, ++turn) {
+        const int a = list.ids[u / m_blocks], r0 = u % m_blocks * BM;
+        if (warp == 0) {
+            if (elect_one())
+                for (int kk = k0; kk < k1; ++kk, ++it) {
+                    const int s = it % C::STAGES;
+                    if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, p.flag, 401, &aborted)) break;
+                    mbar_arrive_expect_tx(&full[s], box * 128 + TN * 128);
+                    tma_load_2d(smem + s * C::STAGE, &tmA, &full[s], kk * 64, a * p.rank + r0);
+                    tma_load_2d(smem + s * C::STAGE + C::A_BYTES, &tmX, &full[s], kk * 64, m0);
+                }
+        } else if (warp == 1) {
+            if (elect_one()) {
+                constexpr uint32_t idesc = idesc_f16(BM, TN, true);
+                for (int kk = k0; kk < k1; ++kk, ++it) {
+                    const int s = it % C::STAGES;
+                    if (!mbar_wait(&full[s], (it / C::STAGES) & 1, p.flag, 402, &aborted)) break;
+                    tc_fence_after();
+                    const uint32_t ad = smem_u32(smem + s * C::STAGE), bd = ad + C::A_BYTES;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        umma_f16_ss(tmem, sdesc_sw128(ad + q * 32, 16, 1024), sdesc_sw128(bd + q * 32, 16, 1024), idesc,
+                                    kk > k0 || q ? 1u : 0u);
+                    umma_commit(&empty[s]);
+                }
+                if (!aborted) umma_commit(done);
+            }
+        } else if (warp_wait(done, turn & 1, p.flag, 403, &aborted)) {
+            // every load has been read: the partials take the ring's place
+            tc_fence_after();
+            const int r = (warp & 3) * 32 + lane;
+#pragma unroll
+            for (int c = 0; c < C::COLS; c += 32) {
+                uint32_t v[32];
+                tmem_ld_32x32b_x32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + c, v);
+                tmem_ld_wait_regs(v);
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (c + j < TN) part[(c + j) * BM + r] = __uint_as_float(v[j]);
+            }
+            tc_fence_before();
+        }
+        if (p.splits > 1) cluster_sync();
+        else __syncthreads();
+        // rank `split` writes tokens [split TN/S, ...): lanes run along the rank
+        if (warp >= 2 && !aborted) {
+            const int r = threadIdx.x - 64, per = TN / p.splits, ld = p.rank_blocks * 64;
+            const float c = p.coeff[a];
+            for (int j = split * per; j < (split + 1) * per; ++j) {
+                if (scratch.tok[j] != a || r0 + r >= ld) continue;
+                float v = 0.f;
+                if (r0 + r < p.rank) {
+                    for (int s = 0; s < p.splits; ++s) v += p.splits > 1 ? ld_peer(&part[j * BM + r], s) : part[j * BM + r];
+                    v *= c;
+                }
+                __nv_bfloat16 hi, lo;
+                split_bf16(v, hi, lo);
+                const int64_t at = (int64_t)(m0 + j) * ld + r0 + r;
+                p.low[at] = hi;
+                if (p.parts == 2) p.low[(int64_t)p.m * ld + at] = lo;
+            }
+        }
+        // the ring may be filled again, by TMA, once every rank has read it
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (p.splits > 1) cluster_sync();
+        else __syncthreads();
+        tc_fence_after();
+    }
+    if (aborted && warp == 0) {   // let the copies already issued land before the CTA exits
+        bool a2 = false;
+        for (uint32_t j = it > (uint32_t)C::STAGES ? it - C::STAGES : 0; j < it; ++j)
+            mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, nullptr, 0, &a2);
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem, C::COLS);
+    }
+}
+
+// ── the projection ───────────────────────────────────────────────────────────
+//
+// 7 warps: 0 TMA, 1 MMA, 2-5 epilogue (two accumulators: the epilogue of one
+// tile runs under the next one's products), 6 the builder: it lists each tile's
+// adapters and copies its rows of low, zeros for other adapters' tokens, into
+// buffers beside the ring while the main blocks are multiplied.
+// Few tiles: a cluster of `splits` CTAs shares a tile's blocks and joins its
+// f32 sums through distributed shared memory in the order of the ranks.
+
+template <int TN>
+struct ProjCfg {
+    static constexpr int A_BYTES = BM * 128, B_BYTES = TN * 128, STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = TN == 256 ? 4 : TN == 128 ? 6 : TN == 64 ? 8 : 10;
+    static constexpr int BUFS = TN == 256 ? 1 : TN == 128 ? 2 : 4;   // rows of low
+    static constexpr int RING = STAGES * STAGE, BUF = RING, BAR = BUF + BUFS * B_BYTES;
+    static constexpr int LIST = BAR + ((2 * STAGES + 8 + 2 * BUFS) * 8 + 8 + 15) / 16 * 16;
+    static constexpr int BYTES = 1024 + LIST + 2 * (int)sizeof(TileList<TN>) + (int)sizeof(ListScratch<TN>);
+    static constexpr int ACC = TN < 32 ? 32 : TN, COLS = 2 * ACC;
+    static_assert(TN * BM * 4 <= RING, "the f32 partials fit the ring");
+    static_assert(BYTES <= 232448, "shared memory exceeds the per-CTA limit");
+};
+constexpr int kProjThreads = 224;
+
+// Tile -> (token tile, weight tile): groups of group_m token tiles, token tiles
+// fastest inside a group.
+__device__ __forceinline__ void tile_at(const AdapterParams &p, int t, int &mt, int &nt) {
+    const int per = p.group_m * p.n_tiles, g = t / per, first = g * p.group_m, gm = min(p.group_m, p.m_tiles - first);
+    const int r = t - g * per;
+    mt = first + r % gm;
+    nt = r / gm;
+}
+
+// One tile's blocks in order: `nk` of the main product, `na` of the adapters'
+// spread evenly among them (so that a builder has time for each) or, where
+// low_kernel still runs while the weights stream, behind them.
+template <typename F, typename G>
+__device__ __forceinline__ void blocks_in_order(int nk, int na, bool behind, F main_block, G adapter_block) {
+    int i = 0;
+    for (int k = 0; k <= nk; ++k) {
+        for (; i < na && (behind ? nk : (int)((int64_t)(i + 1) * nk / (na + 1))) <= k; ++i)
+            if (!adapter_block(i)) return;
+        if (k < nk && !main_block(k)) return;
+    }
+}
+
+template <int EPI>
+__device__ __forceinline__ void finish16(const AdapterParams &p, int m, int count, int n, float bias, const float (&v)[16]) {
+    // 16 tokens from m on (count of them inside), weight row n of this thread;
+    // a warp's threads hold 32 weight rows side by side
+    if constexpr (EPI == LTX_EPI_BF16 || EPI == LTX_EPI_GELU_BF16) {
+        __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(p.out) + (int64_t)m * p.ldo + n;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            float y = v[j] + bias;
+            // gelu_tanh(y) = y / (1 + e^(-2u)), u = sqrt(2/pi) (y + 0.044715 y^3)
+            if constexpr (EPI == LTX_EPI_GELU_BF16)
+                y = __fdividef(y, 1.f + ex2(-2.302208198f * y * (1.f + 0.044715f * y * y)));
+            if (j < count) o[j * p.ldo] = __float2bfloat16_rn(y);
+        }
+    } else if constexpr (EPI == LTX_EPI_F32) {
+        float *o = static_cast<float *>(p.out) + (int64_t)m * p.ldo + n;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (j < count) o[j * p.ldo] = v[j] + bias;
+    } else {
+        float *o = static_cast<float *>(p.out) + (int64_t)m * p.ldo + n;
+        float x[16], g[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            x[j] = j < count ? o[j * p.ldo] : 0.f;
+            g[j] = 1.f;
+            if (p.gate && j < count) g[j] = __ldg(p.gate + (p.gate_idx ? p.gate_idx[m + j] : 0) * p.ld_gate + n);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (j < count) o[j * p.ldo] = x[j] + (v[j] + bias) * g[j];
+    }
+}
+
+template <int TN, int EPI>
+__global__ void __launch_bounds__(kProjThreads, 1)
+    project_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                   const __grid_constant__ CUtensorMap tmB, AdapterParams p) {
+    using C = ProjCfg<TN>;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::BAR), *empty = full + C::STAGES, *tfull = empty + C::STAGES;
+    uint64_t *tempty = tfull + 2, *lfull = tempty + 2, *lempty = lfull + 2, *bfull = lempty + 2, *bempty = bfull + C::BUFS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bempty + C::BUFS);
+    TileList<TN> *lists = reinterpret_cast<TileList<TN> *>(smem + C::LIST);
+    ListScratch<TN> &scratch = *reinterpret_cast<ListScratch<TN> *>(smem + C::LIST + 2 * sizeof(TileList<TN>));
+    float *part = reinterpret_cast<float *>(smem);   // [TN][128], in the ring's place (splits > 1)
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = blockIdx.x % p.splits;
+    const int first = blockIdx.x / p.splits, stride = gridDim.x / p.splits, tiles = p.m_tiles * p.n_tiles;
+    const int kb = (p.k + 63) / 64;
+    const int k0 = (int)((int64_t)kb * split / p.splits), nk = (int)((int64_t)kb * (split + 1) / p.splits) - k0;
+    const int per_adapter = p.rank_blocks * p.parts;
+    // this rank's share of a tile's adapter blocks
+    auto share = [&](int count, int &a0, int &na) {
+        const int64_t all = (int64_t)count * per_adapter;
+        a0 = (int)(all * split / p.splits);
+        na = (int)(all * (split + 1) / p.splits) - a0;
+    };
+    const bool behind = p.splits > 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&tfull[i], 1);
+            mbar_init(&tempty[i], 4);
+            mbar_init(&lfull[i], 32);
+            mbar_init(&lempty[i], 2);
+        }
+        for (int i = 0; i < C::BUFS; ++i) {
+            mbar_init(&bfull[i], 32);
+            mbar_init(&bempty[i], 1);
+        }
+        fence_barrier_init();
+    }
+    if (warp == 0) {
+        tmem_alloc(tmem_slot, C::COLS);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    bool aborted = false;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            tma_prefetch_desc(&tmW);
+            tma_prefetch_desc(&tmX);
+            if (p.adapters) tma_prefetch_desc(&tmB);
+            uint32_t it = 0, i = 0;
+            for (int t = first; t < tiles && !aborted; t += stride, ++i) {
+                int mt, nt;
+                tile_at(p, t, mt, nt);
+                const TileList<TN> &list = lists[i & 1];
+                if (!mbar_wait(&lfull[i & 1], (i >> 1) & 1, p.flag, 411, &aborted)) break;
+                int a0, na;
+                share(list.count, a0, na);
+                auto take = [&](uint32_t bytes) {
+                    const int s = it % C::STAGES;
+                    if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, p.flag, 412, &aborted)) return -1;
+                    mbar_arrive_expect_tx(&full[s], bytes);
+                    ++it;
+                    return s;
+                };
+                blocks_in_order(
+                    nk, na, behind,
+                    [&](int k) {
+                        const int s = take(C::STAGE);
+                        if (s < 0) return false;
+                        tma_load_2d(smem + s * C::STAGE, &tmW, &full[s], (k0 + k) * 64, nt * BM);
+                        tma_load_2d(smem + s * C::STAGE + C::A_BYTES, &tmX, &full[s], (k0 + k) * 64, mt * TN);
+                        return true;
+                    },
+                    [&](int b) {
+                        const int s = take(C::A_BYTES);
+                        if (s < 0) return false;
+                        const int e = a0 + b, rb = e % per_adapter / p.parts;
+                        tma_load_2d(smem + s * C::STAGE, &tmB, &full[s], rb * 64, list.ids[e / per_adapter] * p.n + nt * BM);
+                        return true;
+                    });
+                mbar_arrive(&lempty[i & 1]);
+            }
+            if (aborted) {   // let the copies already issued land before the CTA exits
+                bool a2 = false;
+                for (uint32_t j = it > (uint32_t)C::STAGES ? it - C::STAGES : 0; j < it; ++j)
+                    mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, nullptr, 0, &a2);
+            }
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+            constexpr uint32_t idesc = idesc_f16(BM, TN, true);
+            uint32_t it = 0, i = 0, built = 0;
+            for (int t = first; t < tiles && !aborted; t += stride, ++i) {
+                const uint32_t acc = i & 1;
+                if (!mbar_wait(&lfull[acc], (i >> 1) & 1, p.flag, 413, &aborted)) break;
+                int a0, na;
+                share(lists[acc].count, a0, na);
+                if (!mbar_wait(&tempty[acc], ((i >> 1) & 1) ^ 1, p.flag, 414, &aborted)) break;
+                tc_fence_after();
+                const uint32_t d = tmem + acc * C::ACC;
+                uint32_t more = 0;
+                auto multiply = [&](uint32_t b_addr) {
+                    const int s = it % C::STAGES;
+                    const uint32_t a_addr = smem_u32(smem + s * C::STAGE);
+                    if (!b_addr) b_addr = a_addr + C::A_BYTES;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        umma_f16_ss(d, sdesc_sw128(a_addr + q * 32, 16, 1024), sdesc_sw128(b_addr + q * 32, 16, 1024), idesc,
+                                    more);
+                        more = 1;
+                    }
+                    umma_commit(&empty[s]);
+                    ++it;
+                };
+                blocks_in_order(
+                    nk, na, behind,
+                    [&](int) {
+                        if (!mbar_wait(&full[it % C::STAGES], (it / C::STAGES) & 1, p.flag, 415, &aborted)) return false;
+                        tc_fence_after();
+                        multiply(0);
+                        return true;
+                    },
+                    [&](int) {
+                        const int b = built % C::BUFS;
+                        if (!mbar_wait(&full[it % C::STAGES], (it / C::STAGES) & 1, p.flag, 416, &aborted) ||
+                            !mbar_wait(&bfull[b], (built / C::BUFS) & 1, p.flag, 417, &aborted))
+                            return false;
+                        tc_fence_after();
+                        multiply(smem_u32(smem + C::BUF + b * C::B_BYTES));
+                        umma_commit(&bempty[b]);
+                        ++built;
+                        return true;
+                    });
+                if (aborted) break;
+                mbar_arrive(&lempty[acc]);
+                umma_commit(&tfull[acc]);
+            }
+        }
+    } else if (warp == 6) {
+        const int ld = p.rank_blocks * 64;
+        bool waited = false;
+        uint32_t i = 0, built = 0;
+        for (int t = first; t < tiles && !aborted; t += stride, ++i) {
+            int mt, nt;
+            tile_at(p, t, mt, nt);
+            const int m0 = mt * TN;
+            TileList<TN> &list = lists[i & 1];
+            if (!warp_wait(&lempty[i & 1], ((i >> 1) & 1) ^ 1, p.flag, 418, &aborted)) break;
+            if (p.adapters) {
+                build_list<TN, 32>(p, m0, lane, list, scratch);
+            } else if (lane == 0) {
+                list.count = 0;
+            }
+            mbar_arrive(&lfull[i & 1]);
+            __syncwarp();
+            int a0, na;
+            share(list.count, a0, na);
+            if (na > 0 && !waited) {
+                grid_dep_wait();
+                waited = true;
+            }
+            auto hand_over = [&](uint32_t which) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&bfull[which % C::BUFS]);
+            };
+            for (int b = 0; b < na; ++b, ++built) {
+                const int buf = built % C::BUFS;
+                if (!warp_wait(&bempty[buf], ((built / C::BUFS) & 1) ^ 1, p.flag, 419, &aborted)) break;
+                const int e = a0 + b, a = list.ids[e / per_adapter], rest = e % per_adapter, rb = rest / p.parts;
+                const __nv_bfloat16 *src = p.low + (rest % p.parts ? (int64_t)p.m * ld : 0) + rb * 64;
+                const uint32_t dst = smem_u32(smem + C::BUF + buf * C::B_BYTES);
+#pragma unroll 8
+                for (int x = lane; x < TN * 8; x += 32) {   // 16-byte piece c of token j sits at c ^ (j % 8)
+                    const int j = x >> 3, c = x & 7;
+                    const bool mine = scratch.tok[j] == a;
+                    const __nv_bfloat16 *from = mine ? src + (int64_t)(m0 + j) * ld + c * 8 : p.low;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + j * 128 + ((c ^ (j & 7)) << 4)),
+                                 "l"(from), "r"(mine ? 16 : 0)
+                                 : "memory");
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if constexpr (C::BUFS == 1) {
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    hand_over(built);
+                } else if (b > 0) {   // the one before, while this one is on its way
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    hand_over(built - 1);
+                }
+            }
+            if (C::BUFS > 1 && na > 0 && !aborted) {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                hand_over(built - 1);
+            }
+        }
+        grid_dep_wait();   // low_kernel has ended before this kernel does: the workspace is free behind it
+    } else {
+        const int quad = warp & 3;
+        uint32_t i = 0;
+        for (int t = first; t < tiles && !aborted; t += stride, ++i) {
+            int mt, nt;
+            tile_at(p, t, mt, nt);
+            const uint32_t acc = i & 1;
+            if (!warp_wait(&tfull[acc], (i >> 1) & 1, p.flag, 420, &aborted)) break;
+            tc_fence_after();
+            const int row = quad * 32 + lane, n = nt * BM + row, m0 = mt * TN;
+            const float bias = p.bias && n < p.n ? p.bias[n] : 0.f;
+#pragma unroll 1
+            for (int c = 0; c < C::ACC && (p.splits > 1 || m0 + c < p.m); c += 32) {
+                uint32_t r[32];
+                tmem_ld_32x32b_x32(tmem + ((uint32_t)(quad * 32) << 16) + acc * C::ACC + c, r);
+                tmem_ld_wait_regs(r);
+                if (p.splits > 1) {   // every load has been read: the partials take the ring's place
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (c + j < TN) part[(c + j) * BM + row] = __uint_as_float(r[j]);
+                    continue;
+                }
+#pragma unroll
+                for (int h = 0; h < 32; h += 16) {
+                    float v[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[h + j]);
+                    const int count = min(TN - c - h, p.m - m0 - c - h);
+                    if (n < p.n && count > 0) finish16<EPI>(p, m0 + c + h, count, n, bias, v);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tempty[acc]);
         }
     }
+
+    if (p.splits > 1) {   // one tile per cluster
+        cluster_sync();
+        int mt, nt;
+        tile_at(p, first, mt, nt);
+        if (warp >= 2 && warp < 6 && !aborted) {
+            const int row = threadIdx.x - 64, n = nt * BM + row, per = TN / p.splits;
+            const float bias = p.bias && n < p.n ? p.bias[n] : 0.f;
+            for (int j0 = split * per; j0 < (split + 1) * per; j0 += 16) {
+                float v[16];
+                const int left = min(per, (split + 1) * per - j0);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = 0.f;
+                for (int s = 0; s < p.splits; ++s)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (j < left) v[j] += ld_peer(&part[(j0 + j) * BM + row], s);
+                const int count = min(left, p.m - mt * TN - j0);
+                if (n < p.n && count > 0) finish16<EPI>(p, mt * TN + j0, count, n, bias, v);
+            }
+        }
+        cluster_sync();   // the peers have read this CTA's shared memory
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_dealloc(tmem, C::COLS);
+    }
+}
+
+// ── host side ────────────────────────────────────────────────────────────────
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(f);
+    });
+    return fn;
+}
+
+// bf16 [rows, cols] with row stride ld (elements), boxes of 64 x box_rows.
+bool make_map(CUtensorMap *m, const void *ptr, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(ptr), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename K, typename... Args>
+cudaError_t launch(K kern, int grid, int threads, int smem, int cluster, bool dependent, cudaStream_t st, const Args &...args) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = dependent ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// Shares of K over a cluster: doubled while the CTAs stay within `room` and
+// each keeps at least four blocks of K.
+int splits_for(int64_t jobs, int room, int kb) {
+    int s = 1;
+    while (s < 8 && jobs * s * 2 <= room && kb >= s * 2 * 4) s *= 2;
+    return s;
+}
+
+template <int TN>
+cudaError_t run_low(AdapterParams p, const CUtensorMap &ta, const CUtensorMap &tx, int sms, cudaStream_t st) {
+    const int tiles = (p.m + TN - 1) / TN, room = 2 * sms;
+    p.splits = splits_for(tiles, room, (p.k + 63) / 64);
+    // the SMs left over share the adapters of a tile
+    p.tok_lanes = std::max(1, std::min({room / (tiles * p.splits), p.adapters * ((p.rank + BM - 1) / BM), std::min(TN, p.m)}));
+    return launch(low_kernel<TN>, tiles * p.tok_lanes * p.splits, kLowThreads, LowCfg<TN>::BYTES, p.splits, false, st, ta, tx, p);
+}
+
+template <int TN>
+cudaError_t run_project(AdapterParams p, int epilogue, const CUtensorMap &tw, const CUtensorMap &tx, const CUtensorMap &tb,
+                        int sms, cudaStream_t st) {
+    p.m_tiles = (p.m + TN - 1) / TN;
+    p.n_tiles = (p.n + BM - 1) / BM;
+    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+    p.splits = splits_for(tiles, sms, (p.k + 63) / 64);
+    // A weight within 48 MB stays in L2: then the weight tiles of one token
+    // tile run back to back.  Otherwise as many token tiles go together as keep
+    // their rows of x within 48 MB, and the weights stream once per group.
+    constexpr int64_t kPanel = 48 << 20;
+    p.group_m = (int64_t)p.n * p.k * 2 <= kPanel
+                    ? 1
+                    : (int)std::max<int64_t>(1, std::min<int64_t>(p.m_tiles, kPanel / ((int64_t)TN * p.k * 2)));
+    const int grid = p.splits > 1 ? (int)tiles * p.splits : (int)std::min<int64_t>(tiles, sms);
+    auto go = [&](auto kern) {
+        return launch(kern, grid, kProjThreads, ProjCfg<TN>::BYTES, p.splits, p.adapters > 0, st, tw, tx, tb, p);
+    };
+    switch (epilogue) {
+    case LTX_EPI_BF16: return go(project_kernel<TN, LTX_EPI_BF16>);
+    case LTX_EPI_GELU_BF16: return go(project_kernel<TN, LTX_EPI_GELU_BF16>);
+    case LTX_EPI_F32: return go(project_kernel<TN, LTX_EPI_F32>);
+    default: return go(project_kernel<TN, LTX_EPI_RESID>);
+    }
+}
+
+// Tokens of a tile: the least that holds them all up to 256; above, 256 (the
+// fewest bytes per product), but three tiles of 128 where two of 256 would be
+// a third empty.
+int tokens_for(int m) {
+    for (int t = 16; t < 256; t *= 2)
+        if (m <= t) return t;
+    return m > 256 && m <= 384 ? 128 : 256;
 }
 
 }  // namespace
@@ -119,16 +741,51 @@ extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const void *x_dev, int64_t ldx, c
     if (epilogue == LTX_EPI_RESID && gate_dev && ld_gate < n)
         return fail(ctx, LTX_ERR_SHAPE, "%s: gate rows shorter than n", w);
     DeviceGuard guard(ctx);
+    if ((int64_t)adapters * n > 0x7fffffff || (int64_t)((m + 15) / 16) * ((n + BM - 1) / BM) > 0x7fffffff / 8)
+        return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: %d x %d with %d adapters is too large", w, m, n, adapters);
+    AdapterParams p{};
+    p.m = m;
+    p.n = n;
+    p.k = k;
+    p.rank = rank;
+    p.adapters = adapters;
+    p.rank_blocks = (rank + 63) / 64;
+    p.parts = epilogue == LTX_EPI_F32 || epilogue == LTX_EPI_RESID ? 2 : 1;
+    p.idx = adapter_idx_dev;
+    p.gate_idx = gate_idx_dev;
+    p.coeff = coeff_dev;
+    p.bias = bias_dev;
+    p.gate = gate_dev;
+    p.ldo = ldo;
+    p.ld_gate = ld_gate;
+    p.out = out_dev;
+    p.flag = ctx->timeout_flag;
+    const int tn = tokens_for(m), tl = std::min(tn, 128);
+    CUtensorMap tw, tx, txl, ta, tb;
+    bool ok = make_map(&tw, w_dev, n, k, ldw, BM) && make_map(&tx, x_dev, m, k, ldx, tn);
+    ta = tb = txl = tx;
+    if (adapters)
+        ok = ok && make_map(&txl, x_dev, m, k, ldx, tl) &&
+             make_map(&ta, lora_a_dev, (int64_t)adapters * rank, k, k, std::min(rank, BM)) &&
+             make_map(&tb, lora_b_dev, (int64_t)adapters * n, rank, rank, BM);
+    if (!ok) return fail(ctx, LTX_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", w);
     void *low = nullptr;
-    int rc = work_alloc(ctx, (size_t)m * rank * sizeof(float), &low);
-    if (rc != LTX_OK) return rc;
-    AdapterParams p{static_cast<const __nv_bfloat16 *>(x_dev), static_cast<const __nv_bfloat16 *>(w_dev),
-                    static_cast<const __nv_bfloat16 *>(lora_a_dev), static_cast<const __nv_bfloat16 *>(lora_b_dev), ldx,
-                    ldw, ldo, ld_gate, m, n, k, rank, adapters, epilogue, adapter_idx_dev, gate_idx_dev, coeff_dev,
-                    bias_dev, gate_dev, static_cast<float *>(low), out_dev, ctx->timeout_flag};
-    low_kernel<<<(unsigned)(((int64_t)m * rank + 7) / 8), 256, 0, ctx->stream>>>(p);
-    adapter_tile_kernel<<<dim3((n + 63) / 64, (m + 63) / 64), 256, 0, ctx->stream>>>(p);
-    const cudaError_t e = cudaGetLastError();
-    rc = work_free(ctx, low);
+    cudaError_t e = cudaSuccess;
+    if (adapters) {
+        const int rc = work_alloc(ctx, (size_t)p.parts * m * p.rank_blocks * 128, &low);
+        if (rc != LTX_OK) return rc;
+        p.low = static_cast<__nv_bfloat16 *>(low);
+        e = tl == 16   ? run_low<16>(p, ta, txl, ctx->sm_count, ctx->stream)
+            : tl == 32 ? run_low<32>(p, ta, txl, ctx->sm_count, ctx->stream)
+            : tl == 64 ? run_low<64>(p, ta, txl, ctx->sm_count, ctx->stream)
+                       : run_low<128>(p, ta, txl, ctx->sm_count, ctx->stream);
+    }
+    if (e == cudaSuccess)
+        e = tn == 16    ? run_project<16>(p, epilogue, tw, tx, tb, ctx->sm_count, ctx->stream)
+            : tn == 32  ? run_project<32>(p, epilogue, tw, tx, tb, ctx->sm_count, ctx->stream)
+            : tn == 64  ? run_project<64>(p, epilogue, tw, tx, tb, ctx->sm_count, ctx->stream)
+            : tn == 128 ? run_project<128>(p, epilogue, tw, tx, tb, ctx->sm_count, ctx->stream)
+                        : run_project<256>(p, epilogue, tw, tx, tb, ctx->sm_count, ctx->stream);
+    const int rc = work_free(ctx, low);
     return e == cudaSuccess ? rc : cuda_fail(ctx, e, w);
 }
