@@ -29,7 +29,8 @@ constexpr int BM = 128;             // weight rows of a tile
 constexpr int kMaxWords = LTX_MAX_ADAPTERS / 32;
 
 struct AdapterParams {
-    int m, n, k, rank, adapters, rank_blocks, parts, splits, m_tiles, n_tiles, group_m, tok_lanes;
+    int m, n, k, rank, adapters, rank_blocks, parts, splits, m_tiles, n_tiles, group_m;
+    int tile_lanes, unit;   // low_kernel: CTAs (clusters) per tile, adapters in one of their products
     const int *idx, *gate_idx;
     const float *coeff, *bias, *gate;
     int64_t ldo, ld_gate;
@@ -48,13 +49,51 @@ __device__ __forceinline__ void cluster_sync() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_peer(const float *smem, uint32_t rank) {
+// The address of this CTA's shared memory word `smem` in the CTA `rank` of the
+// cluster, and a store there.
+__device__ __forceinline__ uint32_t peer_addr(const void *smem, uint32_t rank) {
     uint32_t a;
-    float v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(smem)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-    return v;
+    return a;
 }
+__device__ __forceinline__ void st_peer(uint32_t addr, uint32_t v) {
+    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+
+// Joins the partial sums of a cluster's `splits` CTAs: rank d receives tokens
+// [d per, (d + 1) per), per = TN / splits, as part[source][per][128].  Each of
+// four warps sends the 32 rows of TMEM that are its own, straight to the owners'
+// shared memory (stores: nothing waits for a peer's answer); the first `count`
+// tokens are wanted.
+template <int TN>
+__device__ __forceinline__ void send_partials(uint32_t acc, int row, const float *part, int splits, int rank, int count) {
+    const int per = TN / splits, shift = __ffs(per) - 1;   // both powers of two
+    uint32_t to = 0;
+#pragma unroll 1
+    for (int c = 0; c < count; c += 16) {
+        uint32_t r[16];
+        tmem_ld_32x32b_x16(acc + c, r);
+        tmem_ld_wait_regs(r);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            if (j == 0 || ((c + j) & (per - 1)) == 0)   // the next owner
+                to = peer_addr(part + (rank * per + ((c + j) & (per - 1))) * BM + row, min(c + j, TN - 1) >> shift);
+            if (c + j < TN) st_peer(to, r[j]);
+            to += BM * 4;
+        }
+    }
+}
+// 8 tokens from j0 of this rank's share, summed over the sources in their order.
+__device__ __forceinline__ void sum_partials(const float *part, int per, int splits, int j0, int row, float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    const float *at = part + j0 * BM + row;
+    for (int s = 0; s < splits; ++s, at += per * BM)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j0 + j < per) v[j] += at[j * BM];
+}
+
 // Programmatic dependent launch: project_kernel starts beside low_kernel and
 // waits for it only where it reads low.
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -62,7 +101,7 @@ __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol
 
 // The adapters of a tile of tokens.
 template <int TN>
-struct TileList {
+struct alignas(8) TileList {
     int count;
     uint16_t ids[TN];   // ascending
 };
@@ -70,7 +109,7 @@ template <int TN>
 struct ListScratch {
     uint32_t bits[kMaxWords];
     int sums[4];
-    int16_t tok[TN];    // each token's adapter, -1 for none
+    alignas(8) int16_t tok[TN + 8];   // each token's adapter, -1 for none (8 more: read in eights)
 };
 
 // Fills `l` and `s.tok` for tokens [m0, m0 + TN), by NT threads (tid of them).  An index beyond the pool counts as none and raises the
@@ -121,18 +160,21 @@ __device__ __forceinline__ void split_bf16(float v, __nv_bfloat16 &hi, __nv_bflo
 // ── low[m] = c_a x[m] A_a^T ──────────────────────────────────────────────────
 //
 // One cluster of `splits` CTAs per (tile of TN tokens, lane of its adapters):
-// D[rank, TN] = A_a . x^T over the cluster's shares of K, joined in the order
-// of the ranks.  tok_lanes CTAs share a tile's adapters when tiles are few.
+// D[ranks, TN] = A . x^T over the cluster's shares of K, joined in the order of
+// the ranks of the cluster.  One product takes `unit` adapters at once, their
+// ranks behind one another in its 128 rows, so a mixed tile reads x once; with
+// few tiles, lanes of CTAs share a tile's adapters instead.
 
 template <int TN>
 struct LowCfg {
     static constexpr int A_BYTES = BM * 128, STAGE = A_BYTES + TN * 128;
-    static constexpr int STAGES = TN >= 128 ? 3 : 4;   // two CTAs per SM
+    static constexpr int STAGES = TN == 64 ? 4 : 5;   // two CTAs per SM
     static constexpr int RING = STAGES * STAGE;
     static constexpr int LIST = RING + 256;
     static constexpr int BYTES = 1024 + LIST + (int)sizeof(TileList<TN>) + (int)sizeof(ListScratch<TN>);
     static constexpr int COLS = TN < 32 ? 32 : TN;
     static_assert(TN * BM * 4 <= RING, "the f32 partials fit the ring");
+    static_assert(2 * (BYTES + 1024) <= 228 * 1024, "two CTAs share an SM");
 };
 constexpr int kLowThreads = 192;
 
@@ -146,13 +188,15 @@ __global__ void __launch_bounds__(kLowThreads)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
     TileList<TN> &list = *reinterpret_cast<TileList<TN> *>(smem + C::LIST);
     ListScratch<TN> &scratch = *reinterpret_cast<ListScratch<TN> *>(smem + C::LIST + sizeof(TileList<TN>));
-    float *part = reinterpret_cast<float *>(smem);   // [TN][128], in the ring's place
+    float *part = reinterpret_cast<float *>(smem);   // partial sums in the ring's place
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = blockIdx.x % p.splits, job = blockIdx.x / p.splits;
-    const int m0 = job / p.tok_lanes * TN, tok_lane = job % p.tok_lanes;
+    const int m0 = job / p.tile_lanes * TN;
     grid_dep_launch();
     if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmX);
         for (int s = 0; s < C::STAGES; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
@@ -172,19 +216,25 @@ __global__ void __launch_bounds__(kLowThreads)
     bool aborted = false;
 
     const int kb = (p.k + 63) / 64;
-    const int k0 = (int)((int64_t)kb * split / p.splits), k1 = (int)((int64_t)kb * (split + 1) / p.splits);
-    const int m_blocks = (p.rank + BM - 1) / BM, units = list.count * m_blocks;   // (adapter, 128 of its ranks)
-    const int box = min(p.rank, BM);
+    const int k0 = kb * split / p.splits, k1 = kb * (split + 1) / p.splits;
+    const int m_blocks = (p.rank + BM - 1) / BM, box = min(p.rank, BM);   // unit is 1 where m_blocks is not
+    const int units = (list.count + p.unit - 1) / p.unit * m_blocks;
     uint32_t it = 0, turn = 0;
-    for (int u = tok_lane; u < units; u += p.tok_lanes, ++turn) {
-        const int a = list.ids[u / m_blocks], r0 = u % m_blocks * BM;
+    for (int u = job % p.tile_lanes; u < units; u += p.tile_lanes, ++turn) {
+        const int first = u / m_blocks * p.unit, n_here = min(p.unit, list.count - first), r0 = u % m_blocks * BM;
+        // an epilogue thread's row: rank r0 + row % box of adapter `mine`
+        const int row = (warp & 3) * 32 + lane, slot = row / box, mine = slot < n_here ? list.ids[first + slot] : -2;
+        const float c = warp >= 2 && mine >= 0 ? __ldg(p.coeff + mine) : 0.f;
+        const uint32_t acc = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         if (warp == 0) {
             if (elect_one())
                 for (int kk = k0; kk < k1; ++kk, ++it) {
                     const int s = it % C::STAGES;
                     if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, p.flag, 401, &aborted)) break;
-                    mbar_arrive_expect_tx(&full[s], box * 128 + TN * 128);
-                    tma_load_2d(smem + s * C::STAGE, &tmA, &full[s], kk * 64, a * p.rank + r0);
+                    mbar_arrive_expect_tx(&full[s], n_here * box * 128 + TN * 128);
+                    for (int i = 0; i < n_here; ++i)
+                        tma_load_2d(smem + s * C::STAGE + i * box * 128, &tmA, &full[s], kk * 64,
+                                    list.ids[first + i] * p.rank + r0);
                     tma_load_2d(smem + s * C::STAGE + C::A_BYTES, &tmX, &full[s], kk * 64, m0);
                 }
         } else if (warp == 1) {
@@ -203,45 +253,53 @@ __global__ void __launch_bounds__(kLowThreads)
                 }
                 if (!aborted) umma_commit(done);
             }
-        } else if (warp_wait(done, turn & 1, p.flag, 403, &aborted)) {
-            // every load has been read: the partials take the ring's place
+        } else {
+            warp_wait(done, turn & 1, p.flag, 403, &aborted);   // every load has been read
             tc_fence_after();
-            const int r = (warp & 3) * 32 + lane;
+        }
+        if (p.splits > 1) {   // the partials take the ring's place, in every CTA of the cluster
+            cluster_sync();
+            if (warp >= 2 && !aborted && (warp & 3) * 32 < n_here * box)
+                send_partials<TN>(acc, row, part, p.splits, split, min(TN, p.m - m0));
+            tc_fence_before();
+            cluster_sync();
+        }
+        if (warp >= 2 && !aborted) {   // lanes run along the ranks
+            const int ld = p.rank_blocks * 64, r = r0 + row - slot * box, tokens = TN / p.splits;
+            const bool used = r < p.rank;
+            __nv_bfloat16 *low = p.low + (int64_t)(m0 + split * tokens) * ld + r;
+#pragma unroll 1
+            for (int j0 = 0; j0 < tokens; j0 += 8) {
+                float v[8];
+                if (p.splits > 1) {
+                    sum_partials(part, tokens, p.splits, j0, row, v);
+                } else {
+                    uint32_t u[8];
+                    tmem_ld_32x32b_x8(acc + j0, u);
+                    tmem_ld_wait_regs(u);
 #pragma unroll
-            for (int c = 0; c < C::COLS; c += 32) {
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(tmem + ((uint32_t)((warp & 3) * 32) << 16) + c, v);
-                tmem_ld_wait_regs(v);
+                    for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(u[j]);
+                }
+                // adapters of the 8 tokens: 16 bits each
+                int16_t of[8];
+                *reinterpret_cast<uint2 *>(of) = reinterpret_cast<const uint2 *>(scratch.tok)[(split * tokens + j0) / 4];
+                *reinterpret_cast<uint2 *>(of + 4) = reinterpret_cast<const uint2 *>(scratch.tok)[(split * tokens + j0) / 4 + 1];
+                if (tokens < 4) of[0] = scratch.tok[split * tokens], of[1] = scratch.tok[split * tokens + 1];
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (c + j < TN) part[(c + j) * BM + r] = __uint_as_float(v[j]);
+                for (int j = 0; j < 8; ++j) {
+                    if (!used || j0 + j >= tokens || of[j] != mine) continue;
+                    __nv_bfloat16 hi, lo;
+                    split_bf16(v[j] * c, hi, lo);
+                    low[(j0 + j) * ld] = hi;
+                    if (p.parts == 2) low[(int64_t)p.m * ld + (j0 + j) * ld] = lo;
+                }
             }
             tc_fence_before();
         }
-        if (p.splits > 1) cluster_sync();
-        else __syncthreads();
-        // rank `split` writes tokens [split TN/S, ...): lanes run along the rank
-        if (warp >= 2 && !aborted) {
-            const int r = threadIdx.x - 64, per = TN / p.splits, ld = p.rank_blocks * 64;
-            const float c = p.coeff[a];
-            for (int j = split * per; j < (split + 1) * per; ++j) {
-                if (scratch.tok[j] != a || r0 + r >= ld) continue;
-                float v = 0.f;
-                if (r0 + r < p.rank) {
-                    for (int s = 0; s < p.splits; ++s) v += p.splits > 1 ? ld_peer(&part[j * BM + r], s) : part[j * BM + r];
-                    v *= c;
-                }
-                __nv_bfloat16 hi, lo;
-                split_bf16(v, hi, lo);
-                const int64_t at = (int64_t)(m0 + j) * ld + r0 + r;
-                p.low[at] = hi;
-                if (p.parts == 2) p.low[(int64_t)p.m * ld + at] = lo;
-            }
-        }
-        // the ring may be filled again, by TMA, once every rank has read it
+        // the ring may be filled again, by TMA, once this CTA has read it; the
+        // peers send into it only after the next unit's first cluster_sync
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        if (p.splits > 1) cluster_sync();
-        else __syncthreads();
+        __syncthreads();
         tc_fence_after();
     }
     if (aborted && warp == 0) {   // let the copies already issued land before the CTA exits
@@ -259,8 +317,8 @@ __global__ void __launch_bounds__(kLowThreads)
 
 // ── the projection ───────────────────────────────────────────────────────────
 //
-// 7 warps: 0 TMA, 1 MMA, 2-5 epilogue (two accumulators: the epilogue of one
-// tile runs under the next one's products), 6 the builder: it lists each tile's
+// 11 warps: 0 TMA, 1 MMA, 2-9 epilogue (two accumulators: the epilogue of one
+// tile runs under the next one's products), 10 the builder: it lists each tile's
 // adapters and copies its rows of low, zeros for other adapters' tokens, into
 // buffers beside the ring while the main blocks are multiplied.
 // Few tiles: a cluster of `splits` CTAs shares a tile's blocks and joins its
@@ -278,7 +336,7 @@ struct ProjCfg {
     static_assert(TN * BM * 4 <= RING, "the f32 partials fit the ring");
     static_assert(BYTES <= 232448, "shared memory exceeds the per-CTA limit");
 };
-constexpr int kProjThreads = 224;
+constexpr int kProjThreads = 352;
 
 // Tile -> (token tile, weight tile): groups of group_m token tiles, token tiles
 // fastest inside a group.
@@ -294,18 +352,46 @@ __device__ __forceinline__ void tile_at(const AdapterParams &p, int t, int &mt, 
 // low_kernel still runs while the weights stream, behind them.
 template <typename F, typename G>
 __device__ __forceinline__ void blocks_in_order(int nk, int na, bool behind, F main_block, G adapter_block) {
-    int i = 0;
+    auto place = [&](int i) { return behind ? nk : (i + 1) * nk / (na + 1); };   // block i comes before main block place(i)
+    int i = 0, next = na > 0 ? place(0) : nk + 1;
     for (int k = 0; k <= nk; ++k) {
-        for (; i < na && (behind ? nk : (int)((int64_t)(i + 1) * nk / (na + 1))) <= k; ++i)
+        while (next == k) {
             if (!adapter_block(i)) return;
+            next = ++i < na ? place(i) : nk + 1;
+        }
         if (k < nk && !main_block(k)) return;
     }
 }
 
+// What the residual epilogue reads for 16 tokens from m on (count of them
+// inside), weight row n: fetched ahead of its use.
+struct Ahead {
+    float x[16], g[16];
+    // Called by whole warps; gidx: in lanes `at` to `at` + 15 the tokens' gate rows.
+    __device__ __forceinline__ void fetch(const AdapterParams &p, int m, int count, int n, int gidx, int at) {
+        const int64_t o = (int64_t)m * p.ldo + n;
+        const bool in = n < p.n;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = in && j < count ? static_cast<const float *>(p.out)[o + j * p.ldo] : 0.f;
+        if (!p.gate) return;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int64_t row = __shfl_sync(0xffffffffu, gidx, at + j) * p.ld_gate;
+            g[j] = in && j < count ? __ldg(p.gate + row + n) : 0.f;
+        }
+    }
+};
+// The gate rows of tokens m + lane.
+__device__ __forceinline__ int gate_rows(const AdapterParams &p, int m, int lane) {
+    return p.gate && p.gate_idx && m + lane < p.m ? __ldg(p.gate_idx + m + lane) : 0;
+}
+
+// 16 tokens from m on (count of them inside), weight row n of this thread; a
+// warp's threads hold 32 weight rows side by side.
 template <int EPI>
-__device__ __forceinline__ void finish16(const AdapterParams &p, int m, int count, int n, float bias, const float (&v)[16]) {
-    // 16 tokens from m on (count of them inside), weight row n of this thread;
-    // a warp's threads hold 32 weight rows side by side
+__device__ __forceinline__ void finish16(const AdapterParams &p, int m, int count, int n, float bias, const float (&v)[16],
+                                         const Ahead &h) {
+    if (n >= p.n) return;
     if constexpr (EPI == LTX_EPI_BF16 || EPI == LTX_EPI_GELU_BF16) {
         __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(p.out) + (int64_t)m * p.ldo + n;
 #pragma unroll
@@ -316,23 +402,11 @@ __device__ __forceinline__ void finish16(const AdapterParams &p, int m, int coun
                 y = __fdividef(y, 1.f + ex2(-2.302208198f * y * (1.f + 0.044715f * y * y)));
             if (j < count) o[j * p.ldo] = __float2bfloat16_rn(y);
         }
-    } else if constexpr (EPI == LTX_EPI_F32) {
-        float *o = static_cast<float *>(p.out) + (int64_t)m * p.ldo + n;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (j < count) o[j * p.ldo] = v[j] + bias;
     } else {
         float *o = static_cast<float *>(p.out) + (int64_t)m * p.ldo + n;
-        float x[16], g[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            x[j] = j < count ? o[j * p.ldo] : 0.f;
-            g[j] = 1.f;
-            if (p.gate && j < count) g[j] = __ldg(p.gate + (p.gate_idx ? p.gate_idx[m + j] : 0) * p.ld_gate + n);
-        }
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-            if (j < count) o[j * p.ldo] = x[j] + (v[j] + bias) * g[j];
+            if (j < count) o[j * p.ldo] = EPI == LTX_EPI_RESID ? h.x[j] + (v[j] + bias) * (p.gate ? h.g[j] : 1.f) : v[j] + bias;
     }
 }
 
@@ -348,19 +422,19 @@ __global__ void __launch_bounds__(kProjThreads, 1)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bempty + C::BUFS);
     TileList<TN> *lists = reinterpret_cast<TileList<TN> *>(smem + C::LIST);
     ListScratch<TN> &scratch = *reinterpret_cast<ListScratch<TN> *>(smem + C::LIST + 2 * sizeof(TileList<TN>));
-    float *part = reinterpret_cast<float *>(smem);   // [TN][128], in the ring's place (splits > 1)
+    float *part = reinterpret_cast<float *>(smem);   // partial sums in the ring's place (splits > 1)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int split = blockIdx.x % p.splits;
     const int first = blockIdx.x / p.splits, stride = gridDim.x / p.splits, tiles = p.m_tiles * p.n_tiles;
     const int kb = (p.k + 63) / 64;
-    const int k0 = (int)((int64_t)kb * split / p.splits), nk = (int)((int64_t)kb * (split + 1) / p.splits) - k0;
+    const int k0 = kb * split / p.splits, nk = kb * (split + 1) / p.splits - k0;
     const int per_adapter = p.rank_blocks * p.parts;
     // this rank's share of a tile's adapter blocks
     auto share = [&](int count, int &a0, int &na) {
-        const int64_t all = (int64_t)count * per_adapter;
-        a0 = (int)(all * split / p.splits);
-        na = (int)(all * (split + 1) / p.splits) - a0;
+        const int all = count * per_adapter;
+        a0 = all * split / p.splits;
+        na = all * (split + 1) / p.splits - a0;
     };
     const bool behind = p.splits > 1;
 
@@ -371,7 +445,7 @@ __global__ void __launch_bounds__(kProjThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&tfull[i], 1);
-            mbar_init(&tempty[i], 4);
+            mbar_init(&tempty[i], 8);
             mbar_init(&lfull[i], 32);
             mbar_init(&lempty[i], 2);
         }
@@ -485,7 +559,7 @@ __global__ void __launch_bounds__(kProjThreads, 1)
                 umma_commit(&tfull[acc]);
             }
         }
-    } else if (warp == 6) {
+    } else if (warp == 10) {
         const int ld = p.rank_blocks * 64;
         bool waited = false;
         uint32_t i = 0, built = 0;
@@ -521,7 +595,7 @@ __global__ void __launch_bounds__(kProjThreads, 1)
 #pragma unroll 8
                 for (int x = lane; x < TN * 8; x += 32) {   // 16-byte piece c of token j sits at c ^ (j % 8)
                     const int j = x >> 3, c = x & 7;
-                    const bool mine = scratch.tok[j] == a;
+                    const bool mine = scratch.tok[j] == a && rb * 64 + c * 8 < p.rank;   // ranks behind the last: 0
                     const __nv_bfloat16 *from = mine ? src + (int64_t)(m0 + j) * ld + c * 8 : p.low;
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + j * 128 + ((c ^ (j & 7)) << 4)),
                                  "l"(from), "r"(mine ? 16 : 0)
@@ -543,34 +617,47 @@ __global__ void __launch_bounds__(kProjThreads, 1)
         }
         grid_dep_wait();   // low_kernel has ended before this kernel does: the workspace is free behind it
     } else {
-        const int quad = warp & 3;
+        // warps 2-5 and 6-9 take every other 32 tokens of a tile
+        const int quad = warp & 3, side = warp >= 6 ? 32 : 0;
         uint32_t i = 0;
         for (int t = first; t < tiles && !aborted; t += stride, ++i) {
             int mt, nt;
             tile_at(p, t, mt, nt);
             const uint32_t acc = i & 1;
+            const int n = nt * BM + quad * 32 + lane, m0 = mt * TN;
+            const float bias = p.bias && n < p.n ? p.bias[n] : 0.f;
+            const int tokens = min(TN, p.m - m0);
+            Ahead cur, next;
+            int gidx = 0;
+            if (EPI == LTX_EPI_RESID && p.splits == 1 && side < tokens) {   // under the products
+                gidx = gate_rows(p, m0 + side, lane);
+                next.fetch(p, m0 + side, tokens - side, n, gidx, 0);
+            }
             if (!warp_wait(&tfull[acc], (i >> 1) & 1, p.flag, 420, &aborted)) break;
             tc_fence_after();
-            const int row = quad * 32 + lane, n = nt * BM + row, m0 = mt * TN;
-            const float bias = p.bias && n < p.n ? p.bias[n] : 0.f;
+            if (p.splits == 1) {
+                const uint32_t d = tmem + ((uint32_t)(quad * 32) << 16) + acc * C::ACC;
 #pragma unroll 1
-            for (int c = 0; c < C::ACC && (p.splits > 1 || m0 + c < p.m); c += 32) {
-                uint32_t r[32];
-                tmem_ld_32x32b_x32(tmem + ((uint32_t)(quad * 32) << 16) + acc * C::ACC + c, r);
-                tmem_ld_wait_regs(r);
-                if (p.splits > 1) {   // every load has been read: the partials take the ring's place
+                for (int c = side; c < tokens; c += 64) {
+                    uint32_t r[32];
+                    tmem_ld_32x32b_x32(d + c, r);
+                    int gnext = 0;
+                    if (EPI == LTX_EPI_RESID && c + 64 < tokens) gnext = gate_rows(p, m0 + c + 64, lane);
+                    tmem_ld_wait_regs(r);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (c + j < TN) part[(c + j) * BM + row] = __uint_as_float(r[j]);
-                    continue;
-                }
+                    for (int h = 0; h < 32; h += 16) {
+                        if (c + h >= tokens) break;
+                        if constexpr (EPI == LTX_EPI_RESID) {
+                            cur = next;
+                            const int to = h ? c + 64 : c + 16;
+                            if (to < tokens) next.fetch(p, m0 + to, tokens - to, n, h ? gnext : gidx, h ? 0 : 16);
+                        }
+                        float v[16];
 #pragma unroll
-                for (int h = 0; h < 32; h += 16) {
-                    float v[16];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[h + j]);
-                    const int count = min(TN - c - h, p.m - m0 - c - h);
-                    if (n < p.n && count > 0) finish16<EPI>(p, m0 + c + h, count, n, bias, v);
+                        for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[h + j]);
+                        finish16<EPI>(p, m0 + c + h, tokens - c - h, n, bias, v, cur);
+                    }
+                    gidx = gnext;
                 }
             }
             tc_fence_before();
@@ -579,27 +666,33 @@ __global__ void __launch_bounds__(kProjThreads, 1)
         }
     }
 
-    if (p.splits > 1) {   // one tile per cluster
-        cluster_sync();
+    if (p.splits > 1) {   // one tile per cluster; all its loads have been read
+        const int row = (warp & 3) * 32 + lane, per = TN / p.splits;
         int mt, nt;
         tile_at(p, first, mt, nt);
+        cluster_sync();   // the partials take the ring's place in every CTA
+        if (warp >= 2 && warp < 6 && !aborted)
+            send_partials<TN>(tmem + ((uint32_t)((warp & 3) * 32) << 16), row, part, p.splits, split,
+                              min(TN, p.m - mt * TN));
+        cluster_sync();
         if (warp >= 2 && warp < 6 && !aborted) {
-            const int row = threadIdx.x - 64, n = nt * BM + row, per = TN / p.splits;
+            const int n = nt * BM + row;
             const float bias = p.bias && n < p.n ? p.bias[n] : 0.f;
-            for (int j0 = split * per; j0 < (split + 1) * per; j0 += 16) {
-                float v[16];
-                const int left = min(per, (split + 1) * per - j0);
+            for (int j0 = 0; j0 < per; j0 += 16) {
+                const int m = mt * TN + split * per + j0, count = min(per - j0, p.m - m);
+                if (count <= 0) break;
+                Ahead h;
+                if (EPI == LTX_EPI_RESID) h.fetch(p, m, count, n, gate_rows(p, m, lane), 0);
+                float v[16], half[8];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = 0.f;
-                for (int s = 0; s < p.splits; ++s)
+                for (int q = 0; q < 16; q += 8) {
+                    sum_partials(part, per, p.splits, j0 + q, row, half);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (j < left) v[j] += ld_peer(&part[(j0 + j) * BM + row], s);
-                const int count = min(left, p.m - mt * TN - j0);
-                if (n < p.n && count > 0) finish16<EPI>(p, mt * TN + j0, count, n, bias, v);
+                    for (int j = 0; j < 8; ++j) v[q + j] = half[j];
+                }
+                finish16<EPI>(p, m, count, n, bias, v, h);
             }
         }
-        cluster_sync();   // the peers have read this CTA's shared memory
     }
     tc_fence_before();
     __syncthreads();
@@ -673,9 +766,11 @@ template <int TN>
 cudaError_t run_low(AdapterParams p, const CUtensorMap &ta, const CUtensorMap &tx, int sms, cudaStream_t st) {
     const int tiles = (p.m + TN - 1) / TN, room = 2 * sms;
     p.splits = splits_for(tiles, room, (p.k + 63) / 64);
-    // the SMs left over share the adapters of a tile
-    p.tok_lanes = std::max(1, std::min({room / (tiles * p.splits), p.adapters * ((p.rank + BM - 1) / BM), std::min(TN, p.m)}));
-    return launch(low_kernel<TN>, tiles * p.tok_lanes * p.splits, kLowThreads, LowCfg<TN>::BYTES, p.splits, false, st, ta, tx, p);
+    // the SMs left over share the adapters of a tile; what one takes goes together
+    const int blocks = (p.rank + BM - 1) / BM, most = std::min({p.adapters, TN, p.m});
+    p.tile_lanes = std::max(1, std::min(room / (tiles * p.splits), most * blocks));
+    p.unit = blocks > 1 ? 1 : std::min(BM / p.rank, (most + p.tile_lanes - 1) / p.tile_lanes);
+    return launch(low_kernel<TN>, tiles * p.tile_lanes * p.splits, kLowThreads, LowCfg<TN>::BYTES, p.splits, false, st, ta, tx, p);
 }
 
 template <int TN>
@@ -727,7 +822,7 @@ extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const void *x_dev, int64_t ldx, c
     const char *w = "gemm_adapters";
     if (epilogue < LTX_EPI_BF16 || epilogue > LTX_EPI_RESID)
         return fail(ctx, LTX_ERR_INVALID_ARG, "%s: bad epilogue %d", w, epilogue);
-    if (m < 0 || n < 1 || k < 1) return fail(ctx, LTX_ERR_SHAPE, "%s: %d x %d x %d", w, m, n, k);
+    if (m < 0 || n < 1 || k < 1 || k > 1 << 24) return fail(ctx, LTX_ERR_SHAPE, "%s: %d x %d x %d", w, m, n, k);
     if (adapters < 0 || adapters > LTX_MAX_ADAPTERS || rank < 8 || rank > LTX_MAX_ADAPTER_RANK || rank % 8)
         return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: %d adapters of rank %d (at most %d, rank a multiple of 8 up to %d)", w,
                     adapters, rank, LTX_MAX_ADAPTERS, LTX_MAX_ADAPTER_RANK);
@@ -760,7 +855,7 @@ extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const void *x_dev, int64_t ldx, c
     p.ld_gate = ld_gate;
     p.out = out_dev;
     p.flag = ctx->timeout_flag;
-    const int tn = tokens_for(m), tl = std::min(tn, 128);
+    const int tn = tokens_for(m), tl = std::min(tn, 64);
     CUtensorMap tw, tx, txl, ta, tb;
     bool ok = make_map(&tw, w_dev, n, k, ldw, BM) && make_map(&tx, x_dev, m, k, ldx, tn);
     ta = tb = txl = tx;
@@ -777,8 +872,7 @@ extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const void *x_dev, int64_t ldx, c
         p.low = static_cast<__nv_bfloat16 *>(low);
         e = tl == 16   ? run_low<16>(p, ta, txl, ctx->sm_count, ctx->stream)
             : tl == 32 ? run_low<32>(p, ta, txl, ctx->sm_count, ctx->stream)
-            : tl == 64 ? run_low<64>(p, ta, txl, ctx->sm_count, ctx->stream)
-                       : run_low<128>(p, ta, txl, ctx->sm_count, ctx->stream);
+                       : run_low<64>(p, ta, txl, ctx->sm_count, ctx->stream);
     }
     if (e == cudaSuccess)
         e = tn == 16    ? run_project<16>(p, epilogue, tw, tx, tb, ctx->sm_count, ctx->stream)

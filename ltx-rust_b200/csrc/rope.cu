@@ -34,23 +34,45 @@ struct TableParams {
 // The angle in turns, pos * g_i / 2pi, is reduced to [-1/2, 1/2] in f64 (a
 // position of 2^24 has 2.7 million turns) and only the fraction goes to f32:
 // its rounding is at most 2^-26 turns, 1e-7 of the unit circle.
-__global__ void rope_table_1d_kernel(TableParams p) {
-    __shared__ double turns[kMaxRot / 2];
+//
+// A thread keeps VEC neighbouring frequencies of its own and walks down the
+// rows: no division per value, 16-byte stores (VEC 4; 1 where rot_dim / 2 is
+// no multiple of 4).
+template <int VEC>
+__global__ void __launch_bounds__(256) rope_table_1d_kernel(TableParams p) {
+    __shared__ double s_turns[kMaxRot / 2];
     for (int i = threadIdx.x; i < p.half; i += blockDim.x) {
         const double f = exp2(-p.log2_theta * i / p.half);   // theta^(-2i/rot)
         const double w = p.orig_turns > 0 ? fmin(fmax((p.orig_turns * f - p.turns_low) * p.inv_span, 0.0), 1.0) : 0.0;
-        turns[i] = f * (w + (1.0 - w) * p.inv_factor) * 0.15915494309189533577;   // 1/2pi
+        s_turns[i] = f * (w + (1.0 - w) * p.inv_factor) * 0.15915494309189533577;   // 1/2pi
     }
     __syncthreads();
-    const int64_t n = (int64_t)p.rows * p.half;
-    for (int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; e < n; e += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t r = e / p.half;
-        double t = (double)(p.pos ? p.pos[r] : (int)r) * turns[e - r * p.half];
-        t -= rint(t);
-        float s, c;
-        sincospif((float)(2.0 * t), &s, &c);
-        p.cos_out[e] = c * p.amplitude;
-        p.sin_out[e] = s * p.amplitude;
+    const int per_row = p.half / VEC, rows_at_once = 256 / per_row;   // per_row <= 256: rot_dim <= 512
+    const int i = threadIdx.x % per_row * VEC;
+    if (threadIdx.x / per_row >= rows_at_once) return;
+    double turns[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) turns[v] = s_turns[i + v];
+    for (int64_t r = (int64_t)blockIdx.x * rows_at_once + threadIdx.x / per_row; r < p.rows;
+         r += (int64_t)gridDim.x * rows_at_once) {
+        const double pos = p.pos ? p.pos[r] : (int)r;
+        float c[VEC], s[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            double t = pos * turns[v];
+            t -= rint(t);
+            sincospif(2.f * (float)t, &s[v], &c[v]);
+            c[v] *= p.amplitude;
+            s[v] *= p.amplitude;
+        }
+        const int64_t at = r * p.half + i;
+        if constexpr (VEC == 4) {
+            *reinterpret_cast<float4 *>(p.cos_out + at) = make_float4(c[0], c[1], c[2], c[3]);
+            *reinterpret_cast<float4 *>(p.sin_out + at) = make_float4(s[0], s[1], s[2], s[3]);
+        } else {
+            p.cos_out[at] = c[0];
+            p.sin_out[at] = s[0];
+        }
     }
 }
 
@@ -93,7 +115,8 @@ __device__ __forceinline__ int64_t table_row(const NormRopeParams &p, int row) {
     return r;
 }
 
-// Any head_dim, rot_dim, layout and alignment: one warp per (row, head), the
+// Any head_dim, rot_dim, layout and alignment (what the kernel below does not
+// take): one warp per (row, head), the
 // head in shared memory as f32 between the norm and the rotation.
 template <typename T>
 __global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(NormRopeParams p) {
@@ -135,8 +158,152 @@ __global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(NormRopeParams p)
     for (int e = 2 * p.half + lane; e < p.d; e += 32) y[e] = from_f32<T>(s[e]);
 }
 
+// The same with 16-byte accesses: a lane holds 8 neighbouring values, LANES
+// lanes a head (the power of two that covers head_dim / 8), and a warp works on
+// 32 / LANES heads of one row at a time, kHeadsDeep times, with all of its
+// loads issued before the first sum.  A pair of the half layout lies rot_dim/16
+// lanes apart (a shuffle), one of the interleaved layout in one lane.
+constexpr int kHeadsDeep = 4;
+
+template <typename T>
+struct Vec8 {
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4 *>(p)[i];
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const T *e = reinterpret_cast<const T *>(w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+    }
+    __device__ __forceinline__ void put(const float (&v)[8], T *p) {
+        T *e = reinterpret_cast<T *>(w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(p)[i] = w[i];
+    }
+};
+
+__device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
+template <typename T, int LANES>
+__global__ void __launch_bounds__(256) qk_norm_rope_vec_kernel(NormRopeParams p) {
+    constexpr int kSide = 32 / LANES;   // heads side by side in a warp
+    const int lane = threadIdx.x & 31, sub = lane / LANES, e0 = lane % LANES * 8;
+    const int all = p.heads + p.kv_heads, per_row = (all + kSide * kHeadsDeep - 1) / (kSide * kHeadsDeep);
+    const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int64_t row64 = item / per_row;
+    if (row64 >= p.rows) return;
+    const int row = (int)row64, h0 = (int)(item % per_row) * kSide * kHeadsDeep + sub;
+    const bool in_head = e0 < p.d;
+
+    Vec8<T> x[kHeadsDeep];
+#pragma unroll
+    for (int u = 0; u < kHeadsDeep; ++u) {
+        const int h = h0 + u * kSide;
+        if (in_head && h < all)
+            x[u].load(h < p.heads ? static_cast<const T *>(p.q) + (int64_t)row * p.ldq + h * p.d + e0
+                                  : static_cast<const T *>(p.k) + (int64_t)row * p.ldk + (h - p.heads) * p.d + e0);
+        else x[u] = Vec8<T>{};
+    }
+    // rotation of this lane's 8 values: out = x * c + partner * s
+    const int rot = 2 * p.half;
+    const bool turns = e0 < rot;
+    const int apart = p.half / 8;                                 // half layout: lanes between a pair
+    const bool second = !p.interleaved && turns && e0 >= p.half;
+    float c[8], s[8];
+    if (turns) {
+        const int64_t at = table_row(p, row) * p.half;
+        if (!p.interleaved) {
+            const int j = second ? e0 - p.half : e0;
+            load8(p.cos_t + at + j, c);
+            load8(p.sin_t + at + j, s);
+        } else {
+            const float4 c4 = __ldg(reinterpret_cast<const float4 *>(p.cos_t + at + e0 / 2));
+            const float4 s4 = __ldg(reinterpret_cast<const float4 *>(p.sin_t + at + e0 / 2));
+            const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, sv[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                c[i] = cc[i / 2];
+                s[i] = sv[i / 2];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (p.interleaved ? !(i & 1) : !second) s[i] = -s[i];
+    }
+#pragma unroll
+    for (int u = 0; u < kHeadsDeep; ++u) {
+        const int h = h0 + u * kSide;
+        const bool is_q = h < p.heads;
+        float v[8];
+        x[u].get(v);
+        if (p.norm) {
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss += v[i] * v[i];
+#pragma unroll
+            for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float inv = 1.f / sqrtf(ss / (float)p.d + p.eps);
+            const float *g = is_q ? p.gq : p.gk;
+            if (g && in_head) {
+                float gv[8];
+                load8(g + e0, gv);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= inv * gv[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= inv;
+            }
+        }
+        if (rot) {
+            float w[8];
+            if (!p.interleaved) {
+                const int from = second ? lane - apart : lane + apart;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = __shfl_sync(0xffffffffu, v[i], from & 31);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = v[i ^ 1];
+            }
+            if (turns)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = v[i] * c[i] + w[i] * s[i];
+        }
+        if (in_head && h < all)
+            x[u].put(v, is_q ? static_cast<T *>(p.qo) + (int64_t)row * p.ldqo + h * p.d + e0
+                             : static_cast<T *>(p.ko) + (int64_t)row * p.ldko + (h - p.heads) * p.d + e0);
+    }
+}
+
+template <typename T, int LANES>
+void launch_vec(const NormRopeParams &p, cudaStream_t st) {
+    const int heads = 32 / LANES * kHeadsDeep;
+    const int64_t items = (int64_t)p.rows * ((p.heads + p.kv_heads + heads - 1) / heads);
+    qk_norm_rope_vec_kernel<T, LANES><<<(unsigned)((items + 7) / 8), 256, 0, st>>>(p);
+}
+
 template <typename T>
 void launch_norm_rope(const NormRopeParams &p, cudaStream_t st) {
+    // 16-byte accesses need whole groups of 8 values everywhere: the head, each
+    // half of the rotated part (interleaved: the part), rows and bases.
+    constexpr int kAlign = 16 / sizeof(T);
+    const uintptr_t bases = (uintptr_t)p.q | (uintptr_t)p.qo | (uintptr_t)p.k | (uintptr_t)p.ko | (uintptr_t)p.gq |
+                            (uintptr_t)p.gk | (uintptr_t)p.cos_t | (uintptr_t)p.sin_t;
+    const int64_t lds = p.ldq | p.ldqo | p.ldk | p.ldko;
+    if (p.d % 8 == 0 && p.d <= 256 && p.half % (p.interleaved ? 4 : 8) == 0 && !(bases & 15) && lds % kAlign == 0) {
+        if (p.d <= 32) launch_vec<T, 4>(p, st);
+        else if (p.d <= 64) launch_vec<T, 8>(p, st);
+        else if (p.d <= 128) launch_vec<T, 16>(p, st);
+        else launch_vec<T, 32>(p, st);
+        return;
+    }
     const int64_t items = (int64_t)p.rows * (p.heads + p.kv_heads);
     qk_norm_rope_any_kernel<T><<<(unsigned)((items + 7) / 8), 256, 0, st>>>(p);
 }
@@ -163,9 +330,11 @@ extern "C" int ltx_rope_table(ltx_ctx *ctx, const int32_t *pos_dev, int32_t rows
     TableParams p{pos_dev, rows, rot_dim / 2, std::log2(theta), 1.0 / factor,
                   (double)original_len * 0.15915494309189533577, turns_low,
                   original_len > 0 ? 1.0 / (turns_high - turns_low) : 0.0, (float)amplitude, cos_dev, sin_dev};
-    const int64_t n = (int64_t)rows * p.half;
-    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((n + 255) / 256, (int64_t)ctx->sm_count * 8));
-    rope_table_1d_kernel<<<grid, 256, 0, ctx->stream>>>(p);
+    const bool vec = p.half % 4 == 0 && !(((uintptr_t)cos_dev | (uintptr_t)sin_dev) & 15);
+    const int at_once = 256 / (vec ? p.half / 4 : p.half);
+    const int grid = std::min((rows + at_once - 1) / at_once, ctx->sm_count * 8);
+    if (vec) rope_table_1d_kernel<4><<<grid, 256, 0, ctx->stream>>>(p);
+    else rope_table_1d_kernel<1><<<grid, 256, 0, ctx->stream>>>(p);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? LTX_OK : cuda_fail(ctx, e, "rope_table launch");
 }

@@ -268,24 +268,42 @@ def attention(ctx: "Context", q, k, v, out, batch, heads, tq, tk, scale, head_di
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 
 
-def _want(ctx: "Context", what, t, name, dtypes, ndim, rows=None, cols=None, dense=False):
-    """Raises LtxError unless t is a CUDA tensor of the context's device with one of `dtypes`, `ndim` dimensions, the
-    given first / last sizes and a contiguous last dimension (dense: contiguous altogether)."""
+def _refuse(ctx, what, name, t, dtypes, shape):
+    """The reason why `t` is not a tensor of the context's device, one of `dtypes` and `shape`, its rows contiguous."""
     if not t.is_cuda or t.device.index != ctx.device:
         raise LtxError(1, f"{what}: {name} must be on cuda:{ctx.device}, not {t.device}")
     if t.dtype not in dtypes:
         raise LtxError(3, f"{what}: {name} is {t.dtype}, not {' or '.join(str(d) for d in dtypes)}")
-    if t.dim() != ndim or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[-1] != cols):
+    if tuple(t.shape) != tuple(shape):
+        raise LtxError(2, f"{what}: {name} has shape {tuple(t.shape)}, not {tuple(shape)}")
+    raise LtxError(2, f"{what}: {name} needs contiguous, non-overlapping rows")
+
+
+def _dense(ctx, what, name, t, dtype, shape):
+    """Address of a contiguous CUDA tensor of the context's device; LtxError for any other."""
+    if t.get_device() != ctx.device or t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        _refuse(ctx, what, name, t, (dtype,), shape)
+    return t.data_ptr()
+
+
+def _rows(ctx, what, name, t, dtypes, rows, cols):
+    """(address, leading dimension) of a CUDA matrix [rows, cols] of the context's device with contiguous rows that do
+    not overlap; LtxError for any other.  A single row's stride says nothing, so its length stands for it."""
+    if t.get_device() != ctx.device or t.dtype not in dtypes or t.shape != (rows, cols):
+        _refuse(ctx, what, name, t, dtypes, (rows, cols))
+    ld, step = t.stride()
+    if (step != 1 and cols > 1) or (ld < cols and rows > 1):
+        if rows and cols:
+            _refuse(ctx, what, name, t, dtypes, (rows, cols))
+        ld = cols
+    return t.data_ptr(), (ld if rows > 1 and ld > cols else cols)
+
+
+def _matrix(what, name, t):
+    """Shape of a two-dimensional tensor."""
+    if t.dim() != 2:
         raise LtxError(2, f"{what}: {name} has shape {tuple(t.shape)}")
-    if dense and not t.is_contiguous():
-        raise LtxError(2, f"{what}: {name} must be contiguous")
-    if t.numel() and ((t.shape[-1] > 1 and t.stride(-1) != 1) or (ndim == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1])):
-        raise LtxError(2, f"{what}: {name} needs contiguous, non-overlapping rows")
-
-
-def _ld(t):
-    """Leading dimension of a 2-D tensor; a single row's stride says nothing, so its length stands for it."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+    return t.shape
 
 
 def rope_table(ctx: "Context", pos, cos, sin, theta=10000.0, factor=1.0, original_len=0, turns_low=1.0, turns_high=32.0,
@@ -293,13 +311,13 @@ def rope_table(ctx: "Context", pos, cos, sin, theta=10000.0, factor=1.0, origina
     """cos/sin f32 [rows, rot_dim/2] of int32 positions [rows] (None: 0, 1, 2, ...), stretched by `factor`
     (ltx_rope_table)."""
     import torch
-    rows, half = cos.shape
-    _want(ctx, "rope_table", cos, "cos", (torch.float32,), 2, dense=True)
-    _want(ctx, "rope_table", sin, "sin", (torch.float32,), 2, rows, half, dense=True)
-    if pos is not None:
-        _want(ctx, "rope_table", pos, "pos", (torch.int32,), 1, rows, dense=True)
-    ctx.check(lib().ltx_rope_table(ctx.h, _ptr(pos), rows, 2 * half, theta, factor, original_len, turns_low, turns_high,
-                                   amplitude, _ptr(cos), _ptr(sin)), "ltx_rope_table")
+    what, f32 = "rope_table", torch.float32
+    shape = rows, half = _matrix(what, "cos", cos)
+    c, s = _dense(ctx, what, "cos", cos, f32, shape), _dense(ctx, what, "sin", sin, f32, shape)
+    p = None if pos is None else _dense(ctx, what, "pos", pos, torch.int32, (rows,))
+    rc = lib().ltx_rope_table(ctx.h, p, rows, 2 * half, theta, factor, original_len, turns_low, turns_high, amplitude, c, s)
+    if rc:
+        ctx.check(rc, "ltx_rope_table")
 
 
 def qk_norm_rope(ctx: "Context", q, k, q_out, k_out, heads, kv_heads, cos, sin, pos=None, gamma_q=None, gamma_k=None,
@@ -308,28 +326,30 @@ def qk_norm_rope(ctx: "Context", q, k, q_out, k_out, heads, kv_heads, cos, sin, 
     each head's first values by cos/sin [table_rows, rot_dim/2] (None: no rotation), row r at table row pos[r]
     (ltx_qk_norm_rope).  q_out / k_out may be q / k."""
     import torch
-    what, rows = "qk_norm_rope", q.shape[0]
-    d = q.shape[-1] // max(heads, 1)
-    types = {torch.bfloat16: LTX_BF16, torch.float16: LTX_F16, torch.float32: LTX_F32}
-    _want(ctx, what, q, "q", tuple(types), 2, cols=heads * d)
-    _want(ctx, what, q_out, "q_out", (q.dtype,), 2, rows, heads * d)
+    what, f32, dt = "qk_norm_rope", torch.float32, q.dtype
+    rows, cols = _matrix(what, "q", q)
+    d = cols // max(heads, 1)
+    types = {torch.bfloat16: LTX_BF16, torch.float16: LTX_F16, f32: LTX_F32}
+    qp, ldq = _rows(ctx, what, "q", q, types, rows, heads * d)
+    qop, ldqo = _rows(ctx, what, "q_out", q_out, (dt,), rows, heads * d)
+    kp = kop = gq = gk = cp = sp = pp = None
+    ldk = ldko = table = half = 0
     if kv_heads:
-        _want(ctx, what, k, "k", (q.dtype,), 2, rows, kv_heads * d)
-        _want(ctx, what, k_out, "k_out", (q.dtype,), 2, rows, kv_heads * d)
-    for g, name in ((gamma_q, "gamma_q"), (gamma_k, "gamma_k")):
-        if g is not None:
-            _want(ctx, what, g, name, (torch.float32,), 1, d, dense=True)
-    half = table = 0
+        kp, ldk = _rows(ctx, what, "k", k, (dt,), rows, kv_heads * d)
+        kop, ldko = _rows(ctx, what, "k_out", k_out, (dt,), rows, kv_heads * d)
+    if gamma_q is not None:
+        gq = _dense(ctx, what, "gamma_q", gamma_q, f32, (d,))
+    if gamma_k is not None:
+        gk = _dense(ctx, what, "gamma_k", gamma_k, f32, (d,))
     if cos is not None:
-        table, half = cos.shape
-        _want(ctx, what, cos, "cos", (torch.float32,), 2, dense=True)
-        _want(ctx, what, sin, "sin", (torch.float32,), 2, table, half, dense=True)
+        shape = table, half = _matrix(what, "cos", cos)
+        cp, sp = _dense(ctx, what, "cos", cos, f32, shape), _dense(ctx, what, "sin", sin, f32, shape)
     if pos is not None:
-        _want(ctx, what, pos, "pos", (torch.int32,), 1, rows, dense=True)
-    kp, kl, kop, kol = (_ptr(k), _ld(k), _ptr(k_out), _ld(k_out)) if kv_heads else (None, 0, None, 0)
-    ctx.check(lib().ltx_qk_norm_rope(ctx.h, types[q.dtype], _ptr(q), _ld(q), kp, kl, _ptr(q_out), _ld(q_out), kop, kol,
-                                     rows, heads, kv_heads, d, int(norm), eps, _ptr(gamma_q), _ptr(gamma_k), _ptr(cos),
-                                     _ptr(sin), table, 2 * half, layout, _ptr(pos)), "ltx_qk_norm_rope")
+        pp = _dense(ctx, what, "pos", pos, torch.int32, (rows,))
+    rc = lib().ltx_qk_norm_rope(ctx.h, types[dt], qp, ldq, kp, ldk, qop, ldqo, kop, ldko, rows, heads, kv_heads, d,
+                                1 if norm else 0, eps, gq, gk, cp, sp, table, 2 * half, layout, pp)
+    if rc:
+        ctx.check(rc, "ltx_qk_norm_rope")
 
 
 def gemm_adapters(ctx: "Context", x, w, out, adapter_idx, lora_a, lora_b, coeff, epilogue=EPI_BF16, bias=None,
@@ -338,28 +358,28 @@ def gemm_adapters(ctx: "Context", x, w, out, adapter_idx, lora_a, lora_b, coeff,
     (ltx_gemm_adapters): x [M,K], w [N,K], lora_a [adapters,rank,K], lora_b [adapters,N,rank] bf16, coeff f32,
     adapter_idx int32 [M], out bf16 or (EPI_F32, EPI_RESID) f32 [M,N]."""
     import torch
-    what, (M, K), N = "gemm_adapters", x.shape, w.shape[0]
-    bf, f32, i32 = (torch.bfloat16,), (torch.float32,), (torch.int32,)
-    _want(ctx, what, x, "x", bf, 2)
-    _want(ctx, what, w, "w", bf, 2, cols=K)
-    _want(ctx, what, out, "out", f32 if epilogue in (EPI_F32, EPI_RESID) else bf, 2, M, N)
-    _want(ctx, what, adapter_idx, "adapter_idx", i32, 1, M, dense=True)
-    _want(ctx, what, lora_a, "lora_a", bf, 3, cols=K, dense=True)
+    what, bf, f32, i32 = "gemm_adapters", torch.bfloat16, torch.float32, torch.int32
+    M, K = _matrix(what, "x", x)
+    N = _matrix(what, "w", w)[0]
+    xp, ldx = _rows(ctx, what, "x", x, (bf,), M, K)
+    wp, ldw = _rows(ctx, what, "w", w, (bf,), N, K)
+    op, ldo = _rows(ctx, what, "out", out, (f32,) if epilogue in (EPI_F32, EPI_RESID) else (bf,), M, N)
+    if lora_a.dim() != 3:
+        raise LtxError(2, f"{what}: lora_a has shape {tuple(lora_a.shape)}")
     n, rank = lora_a.shape[:2]
-    _want(ctx, what, lora_b, "lora_b", bf, 3, n, rank, dense=True)
-    if lora_b.shape[1] != N:
-        raise LtxError(2, f"{what}: lora_b has shape {tuple(lora_b.shape)}")
-    _want(ctx, what, coeff, "coeff", f32, 1, n, dense=True)
-    if bias is not None:
-        _want(ctx, what, bias, "bias", f32, 1, N, dense=True)
-    if gate is not None:
-        _want(ctx, what, gate, "gate", f32, 2, cols=N)
-    if gate_idx is not None:
-        _want(ctx, what, gate_idx, "gate_idx", i32, 1, M, dense=True)
-    ctx.check(lib().ltx_gemm_adapters(ctx.h, _ptr(x), _ld(x), _ptr(w), _ld(w), M, N, K, epilogue, _ptr(bias), _ptr(out),
-                                      _ld(out), _ptr(gate), _ptr(gate_idx), _ld(gate) if gate is not None else 0,
-                                      _ptr(adapter_idx), _ptr(lora_a), _ptr(lora_b), _ptr(coeff), n, rank),
-              "ltx_gemm_adapters")
+    ip = _dense(ctx, what, "adapter_idx", adapter_idx, i32, (M,))
+    ap = _dense(ctx, what, "lora_a", lora_a, bf, (n, rank, K))
+    bp = _dense(ctx, what, "lora_b", lora_b, bf, (n, N, rank))
+    cp = _dense(ctx, what, "coeff", coeff, f32, (n,))
+    bias = None if bias is None else _dense(ctx, what, "bias", bias, f32, (N,))
+    gp, ldg = (None, 0) if gate is None else _rows(ctx, what, "gate", gate, (f32,), _matrix(what, "gate", gate)[0], N)
+    if gate is not None and gate.shape[0] == 0:
+        raise LtxError(2, f"{what}: gate has no rows")
+    gate_idx = None if gate_idx is None else _dense(ctx, what, "gate_idx", gate_idx, i32, (M,))
+    rc = lib().ltx_gemm_adapters(ctx.h, xp, ldx, wp, ldw, M, N, K, epilogue, bias, op, ldo, gp, gate_idx, ldg, ip, ap, bp,
+                                 cp, n, rank)
+    if rc:
+        ctx.check(rc, "ltx_gemm_adapters")
 
 
 def attention_packed(ctx: "Context", q, k, v, out, q_offsets, k_offsets, heads, kv_heads, scale, head_dim=128,
@@ -368,25 +388,24 @@ def attention_packed(ctx: "Context", q, k, v, out, q_offsets, k_offsets, heads, 
     k/v [rows_k, kv_heads*head_dim] bf16 (v bf16 or f16), document i at rows q_offsets[i]:q_offsets[i+1] and
     k_offsets[i]:k_offsets[i+1] (int32 CUDA [docs+1]); slopes f32 [heads], prefix int32 [docs] (with causal)."""
     import torch
-    what, docs = "attention_packed", q_offsets.shape[0] - 1
+    what, bf, i32, qc, kc = "attention_packed", torch.bfloat16, torch.int32, heads * head_dim, kv_heads * head_dim
+    docs = q_offsets.shape[0] - 1 if q_offsets.dim() == 1 else -1
     if docs < 0:
         raise LtxError(2, f"{what}: q_offsets needs docs + 1 entries")
-    bf, i32 = (torch.bfloat16,), (torch.int32,)
-    _want(ctx, what, q, "q", bf, 2, cols=heads * head_dim)
-    _want(ctx, what, out, "out", bf, 2, q.shape[0], heads * head_dim)
-    _want(ctx, what, k, "k", bf, 2, cols=kv_heads * head_dim)
-    _want(ctx, what, v, "v", (torch.bfloat16, torch.float16), 2, k.shape[0], kv_heads * head_dim)
-    _want(ctx, what, q_offsets, "q_offsets", i32, 1, dense=True)
-    _want(ctx, what, k_offsets, "k_offsets", i32, 1, docs + 1, dense=True)
-    if slopes is not None:
-        _want(ctx, what, slopes, "slopes", (torch.float32,), 1, heads, dense=True)
-    if prefix is not None:
-        _want(ctx, what, prefix, "prefix", i32, 1, docs, dense=True)
-    ctx.check(lib().ltx_attention_packed_fwd(ctx.h, _ptr(q), _ld(q), _ptr(k), _ld(k), _ptr(v), _ld(v),
-                                             LTX_F16 if v.dtype == torch.float16 else LTX_BF16, _ptr(q_offsets),
-                                             _ptr(k_offsets), docs, q.shape[0], k.shape[0], heads, kv_heads, head_dim,
-                                             scale, softcap, _ptr(slopes), int(causal), _ptr(prefix), _ptr(out),
-                                             _ld(out)), "ltx_attention_packed_fwd")
+    rows_q, rows_k = _matrix(what, "q", q)[0], _matrix(what, "k", k)[0]
+    qp, ldq = _rows(ctx, what, "q", q, (bf,), rows_q, qc)
+    op, ldo = _rows(ctx, what, "out", out, (bf,), rows_q, qc)
+    kp, ldk = _rows(ctx, what, "k", k, (bf,), rows_k, kc)
+    vp, ldv = _rows(ctx, what, "v", v, (bf, torch.float16), rows_k, kc)
+    qo = _dense(ctx, what, "q_offsets", q_offsets, i32, (docs + 1,))
+    ko = _dense(ctx, what, "k_offsets", k_offsets, i32, (docs + 1,))
+    slopes = None if slopes is None else _dense(ctx, what, "slopes", slopes, torch.float32, (heads,))
+    prefix = None if prefix is None else _dense(ctx, what, "prefix", prefix, i32, (docs,))
+    rc = lib().ltx_attention_packed_fwd(ctx.h, qp, ldq, kp, ldk, vp, ldv, LTX_BF16 if v.dtype is bf else LTX_F16, qo, ko,
+                                        docs, rows_q, rows_k, heads, kv_heads, head_dim, scale, softcap, slopes,
+                                        1 if causal else 0, prefix, op, ldo)
+    if rc:
+        ctx.check(rc, "ltx_attention_packed_fwd")
 
 
 KEYMAP_IDENTITY, KEYMAP_TRANSFORMER = 0, 1
