@@ -94,11 +94,6 @@ __device__ __forceinline__ void sum_partials(const float *part, int per, int spl
             if (j0 + j < per) v[j] += at[j * BM];
 }
 
-// Programmatic dependent launch: project_kernel starts beside low_kernel and
-// waits for it only where it reads low.
-__device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // The adapters of a tile of tokens.
 template <int TN>
 struct alignas(8) TileList {

@@ -33,6 +33,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "attention_packed.cuh"
 #include "device_common.cuh"
 #include "internal.hpp"
 #include "kernels.hpp"
@@ -41,20 +42,7 @@ namespace ltx {
 
 namespace {
 
-constexpr int BQ = 128, BKV = 128;
 constexpr int kThreads = 320;
-constexpr float kRescaleLog2 = 8.0f;
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct PackedParams {
-    __nv_bfloat16 *out;
-    int64_t ldo;
-    const int *qo, *ko, *prefix;
-    const float *slopes;
-    int docs, rows_q, rows_k, kv_heads, group, tile_tokens, causal, pairs, splits;
-    float scale, softcap;
-    int *flag;
-};
 
 // D 128: 16-bit K and V tiles of 32 KB (two 64-column swizzle blocks), D 64: 16 KB.
 template <int D>
@@ -69,20 +57,6 @@ struct Smem {
     static_assert(2 * 128 * D * 4 <= RING_SLOTS * TILE, "the f32 partials of both tiles fit the ring");
     static_assert(BYTES <= 232448, "shared memory exceeds the per-CTA limit");
 };
-
-// What a CTA works on: the document's rows and the first of its query tiles.
-struct Item {
-    int qs, lq, ks, lk, tile0, doc;
-};
-
-// Document i's rows [s, e) of an offsets array, kept inside [0, rows] whatever
-// the array holds; an entry that descends or lies outside raises the flag.
-__device__ __forceinline__ void doc_span(const int *off, int i, int rows, int *flag, int &s, int &e) {
-    const int a = off[i], b = off[i + 1];
-    if (a < 0 || b < a || b > rows) atomicExch(flag, kErrBadOffsets);
-    s = min(max(a, 0), rows);
-    e = min(max(b, s), rows);
-}
 
 // The pair-th pair of query tiles over all documents, found by one warp; false
 // when there are fewer.  A causal document's last tiles have the most keys and
@@ -119,13 +93,6 @@ __device__ __forceinline__ bool find_item(const PackedParams &p, int pair, int l
     return false;
 }
 
-// Keys that token `t` of the document sees: the first of them.
-__device__ __forceinline__ int limit_of(const PackedParams &p, const Item &it, int t, int prefix) {
-    if (!p.causal) return it.lk;
-    const int64_t upto = (int64_t)t + it.lk - it.lq + 1;
-    return max(prefix, (int)min((int64_t)it.lk, max((int64_t)0, upto)));
-}
-
 __device__ __forceinline__ void cluster_sync() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -148,18 +115,6 @@ __device__ __forceinline__ float2 ld_peer2(uint32_t addr) {
     asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
     return v;
 }
-
-// How a raw score becomes one in the log2 domain when it is capped or biased.
-struct ScoreMod {
-    float scale, twice_over_cap, cap2;   // scale; 2 log2e / cap (0 = no cap); cap log2e
-    float slope2, place;                 // slope log2e (0 = no bias), the row's key less the tile's first
-    __device__ __forceinline__ float operator()(float s, int e) const {
-        s *= scale;
-        // tanh(u) = 1 - 2 / (2^(2u log2e) + 1): absolute error of some 1e-7, right at both ends
-        s = twice_over_cap > 0.f ? cap2 * (1.f - __fdividef(2.f, ex2(s * twice_over_cap) + 1.f)) : s * kLog2e;
-        return s - slope2 * fabsf(place - (float)e);
-    }
-};
 
 // VF16: V (and so P) are f16, otherwise bf16; Q and K are bf16.  MOD: scores
 // are capped or biased.
@@ -602,37 +557,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void *f = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(f);
-    });
-    return fn;
-}
-
-// [rows, heads, D] of 16-bit values with row stride ld (elements), box {64, box_heads, box_rows}.
-bool make_map(CUtensorMap *m, const void *ptr, int64_t rows, int heads, int d, int64_t ld, bool f16, int box_heads,
-              int box_rows) {
-    EncodeTiledFn fn = encode_tiled();
-    if (!fn) return false;
-    cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)rows};
-    cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)ld * 2};
-    cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
-    cuuint32_t estr[3] = {1, 1, 1};
-    return fn(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(ptr),
-              dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int D>
 cudaError_t launch_packed(bool f16, bool mod, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
                           const PackedParams &p, cudaStream_t st) {
@@ -654,7 +578,37 @@ cudaError_t launch_packed(bool f16, bool mod, const CUtensorMap &tq, const CUten
     return cudaLaunchKernelEx(&cfg, kern, tq, tk, tv, p);
 }
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(f);
+    });
+    return fn;
+}
+
 }  // namespace
+
+bool packed_map(CUtensorMap *m, const void *ptr, int64_t rows, int heads, int d, int64_t ld, bool f16, int box_heads,
+              int box_rows) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)rows};
+    cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)ld * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return fn(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(ptr),
+              dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 }  // namespace ltx
 
@@ -688,23 +642,30 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const void *q_dev, int64_t
     DeviceGuard guard(ctx);
     const int group = heads / kv_heads, tokens = 128 / group;
     CUtensorMap tq, tk, tv;
-    bool ok = make_map(&tq, q_dev, rows_q, heads, head_dim, ldq, false, group, tokens);
+    bool ok = packed_map(&tq, q_dev, rows_q, heads, head_dim, ldq, false, group, tokens);
     tk = tv = tq;   // never read without keys
     if (rows_k)
-        ok = ok && make_map(&tk, k_dev, rows_k, kv_heads, head_dim, ldk, false, 1, BKV) &&
-             make_map(&tv, v_dev, rows_k, kv_heads, head_dim, ldv, v_dtype == LTX_F16, 1, BKV);
+        ok = ok && packed_map(&tk, k_dev, rows_k, kv_heads, head_dim, ldk, false, 1, BKV) &&
+             packed_map(&tv, v_dev, rows_k, kv_heads, head_dim, ldv, v_dtype == LTX_F16, 1, BKV);
     if (!ok) return fail(ctx, LTX_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", w);
+    PackedParams p{static_cast<__nv_bfloat16 *>(out_dev), ldo, q_offsets_dev, k_offsets_dev, prefix_dev, slopes_dev,
+                   docs, rows_q, rows_k, kv_heads, group, tokens, causal, 0, 1, scale, softcap, ctx->timeout_flag};
+    // Few rows per document over many keys, by their averages (the host does
+    // not see the offsets): the kernel whose tiles have keys as rows and whose
+    // CTAs share every document.  Under some 512 keys its join and its start
+    // cost more than it saves.
+    const int some = std::min(docs, rows_q);
+    const int64_t rows_per_doc = (int64_t)((rows_q + some - 1) / some) * group;
+    if (rows_per_doc <= kMaxFewRows && rows_k / docs >= 512)
+        return attention_packed_few(ctx, tk, tv, q_dev, ldq, p, heads, head_dim, v_dtype == LTX_F16, (int)rows_per_doc);
     // Pairs of query tiles over all documents: sum ceil(lq / per) <= (rows + docs (per - 1)) / per.
     const int64_t per = 2 * tokens;
-    const int64_t pairs = (rows_q + std::min<int64_t>(docs, rows_q) * (per - 1)) / per, items = pairs * kv_heads;
+    const int64_t pairs = (rows_q + (int64_t)some * (per - 1)) / per, items = pairs * kv_heads;
     if (items > 0x7fffffff / 8) return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: more than 2^28 tiles", w);
     // Too few CTAs for the SMs: split the keys over a cluster, at least two K/V
     // tiles each if one document had them all.
-    int splits = 1;
-    while (splits < 8 && items * splits * 2 <= ctx->sm_count && (int64_t)splits * 4 * BKV <= rows_k) splits *= 2;
-    PackedParams p{static_cast<__nv_bfloat16 *>(out_dev), ldo, q_offsets_dev, k_offsets_dev, prefix_dev, slopes_dev,
-                   docs, rows_q, rows_k, kv_heads, group, tokens, causal, (int)pairs, splits, scale, softcap,
-                   ctx->timeout_flag};
+    while (p.splits < 8 && items * p.splits * 2 <= ctx->sm_count && (int64_t)p.splits * 4 * BKV <= rows_k) p.splits *= 2;
+    p.pairs = (int)pairs;
     const bool mod = softcap > 0.f || slopes_dev;
     const cudaError_t e = head_dim == 64 ? launch_packed<64>(v_dtype == LTX_F16, mod, tq, tk, tv, p, ctx->stream)
                                          : launch_packed<128>(v_dtype == LTX_F16, mod, tq, tk, tv, p, ctx->stream);

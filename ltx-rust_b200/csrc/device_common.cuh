@@ -143,6 +143,12 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, int *f
     return false;
 }
 
+// Programmatic dependent launch: a kernel launched as a dependent may start when
+// every CTA of the one before has called grid_dep_launch, and waits in
+// grid_dep_wait for that kernel's end and its writes.
+__device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ── TMA ─────────────────────────────────────────────────────────────────────
 
 __device__ __forceinline__ void tma_load_2d(void *smem_dst, const void *tmap, uint64_t *bar, int x, int y) {
