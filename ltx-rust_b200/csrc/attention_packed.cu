@@ -7,31 +7,38 @@
 // least that many), so a row needs one number and a tile of keys is either
 // whole for all rows of a warp or compared against it.
 //
-// One CTA per (document, key head, up to 256 query rows).  A query row is a
-// (token, head of the key head's group): a 128-row tile holds 128 / group
-// tokens times the group's heads, so the heads that share a key head read
-// each K/V tile once, and a single new token still brings `group` rows.
-// Both 128-row tiles A and B of the CTA share every K/V tile.
+// Items are (key head, document, up to 256 query rows), one per CTA of the grid; a
+// CTA that has told its roles about one takes over the next CTA not yet launched
+// (cluster launch control), so its loads and products run on under the epilogue
+// and unequal items still spread evenly.  A query row is a (token, head of the key head's group): a
+// 128-row tile holds 128 / group tokens times the group's heads, so the heads
+// that share a key head read each K/V tile once.  Both 128-row tiles A and B of
+// an item share every K/V tile, and tiles go from the last keys to the first
+// (with a bias by distance the largest scores come first, and the running
+// maximum hardly moves).
 // TMEM (512 columns): S_A, S_B (128 f32 columns each), O_A, O_B; P goes back
 // into the upper half of its S as packed 16-bit pairs and is the A operand of
 // P.V from there.
 // 10 warps:
-//   warp 0     TMA: the Q tiles, then K_j, V_j through a ring.  Afterwards it
-//              zeroes the V rows behind the document's end in the last tile:
-//              P is 0 there, but 0 times another document's NaN is not.
-//   warp 1     one thread issues QK_A QK_B | PV_A(j) QK_A(j+1) PV_B(j) QK_B(j+1).
+//   warp 0     finds the items and tells the others; TMA: the Q tiles, then K_j,
+//              V_j through a ring that runs on into the next item.
+//   warp 1     one thread issues QK_A QK_B | PV_A(j) QK_A(j+1) PV_B(j) QK_B(j+1);
+//              the next item's QK follows under this one's epilogue.
 //   warps 2-5  softmax of tile A, 6-9 of tile B, one row per thread: running
 //              maximum and sum in f32, O rescaled in TMEM only when a row's
 //              maximum grew by more than 2^kRescaleLog2.
-// With few CTAs (few rows over long keys) a cluster of S CTAs shares the
-// keys of one item and joins its partial O, maximum and sum through
-// distributed shared memory, in the order of the ranks.
+// V rows behind a document's end are zeroed by a softmax warp's threads before
+// they hand P over: P is 0 there, but 0 times another document's NaN is not.
+// With few items (few rows over long keys) a cluster of S CTAs shares the keys
+// of one item and joins its partial O, maximum and sum through distributed
+// shared memory, in the order of the ranks.
 // All waits are bounded (2 s) and report LTX_ERR_TIMEOUT through the flag.
 #include <cuda.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "attention_packed.cuh"
 #include "device_common.cuh"
@@ -43,6 +50,13 @@ namespace ltx {
 namespace {
 
 constexpr int kThreads = 320;
+// The same value, unknown to the compiler: what is computed from it inside a
+// loop is not kept in registers around the loop.
+__device__ __forceinline__ int fresh(int v) {
+    asm volatile("" : "+r"(v));
+    return v;
+}
+constexpr int kNoRow = 1 << 30;   // keys left of a thread without a row (no document has as many)
 
 // D 128: 16-bit K and V tiles of 32 KB (two 64-column swizzle blocks), D 64: 16 KB.
 template <int D>
@@ -52,8 +66,8 @@ struct Smem {
     static constexpr int Q = 0, RING = 2 * TILE, BAR = RING + RING_SLOTS * TILE;
     // float2 [2][128], a row's maximum and sum (splits > 1): where Q was, which no product reads any more
     static constexpr int ML = Q;
-    static constexpr int BYTES = BAR + 256 + 1024;
-    static_assert((8 + 2 * RING_SLOTS) * 8 + 8 + 32 <= 256, "barriers and document words exceed their block");
+    static constexpr int BYTES = BAR + 384 + 1024;
+    static_assert((14 + 2 * RING_SLOTS) * 8 + 16 + 2 * sizeof(Item) <= 384, "barriers and items exceed their block");
     static_assert(2 * 128 * D * 4 <= RING_SLOTS * TILE, "the f32 partials of both tiles fit the ring");
     static_assert(BYTES <= 232448, "shared memory exceeds the per-CTA limit");
 };
@@ -93,6 +107,30 @@ __device__ __forceinline__ bool find_item(const PackedParams &p, int pair, int l
     return false;
 }
 
+// Cluster launch control: asks for a CTA of the grid that has not been launched
+// yet; the 16-byte answer lands in shared memory and counts on the mbarrier.
+__device__ __forceinline__ void ask_next_cta(void *answer, uint64_t *bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_u32(answer)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+// The index of the CTA taken over, -1 when none was left.
+__device__ __forceinline__ int next_cta(const void *answer) {
+    uint32_t got, x;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 a;\n\t"
+        "ld.shared.b128 a, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "mov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n\t}"
+        : "=r"(got), "=r"(x)
+        : "r"(smem_u32(answer))
+        : "memory");
+    return got ? (int)x : -1;
+}
+
 __device__ __forceinline__ void cluster_sync() {
     __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -116,9 +154,237 @@ __device__ __forceinline__ float2 ld_peer2(uint32_t addr) {
     return v;
 }
 
-// VF16: V (and so P) are f16, otherwise bf16; Q and K are bf16.  MOD: scores
-// are capped or biased.
-template <int D, bool VF16, bool MOD>
+// A CTA's share of an item: K/V tiles [j0, j0 + cnt[t]) for query tile t (what
+// its last token sees, cut to this rank of the cluster), `all` of them loaded.
+struct Share {
+    int cnt[2], j0, all, nt, prefix;
+    __device__ __forceinline__ Share(const PackedParams &p, const Item &it, int split) {
+        prefix = p.causal && p.prefix ? min(max(p.prefix[it.doc], 0), it.lk) : 0;
+        nt = it.lq > (it.tile0 + 1) * p.tile_tokens ? 2 : 1;   // query tiles that hold tokens
+        int n[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            n[t] = t < nt ? (limit_of(p, it, min((it.tile0 + t + 1) * p.tile_tokens, it.lq) - 1, prefix) + BKV - 1) / BKV : 0;
+        const int most = max(n[0], n[1]);
+        const int per = p.splits == 1 ? most : (most + p.splits - 1) / p.splits;
+        j0 = split * per;
+        const int j1 = min(most, j0 + per);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) cnt[t] = max(0, min(j1, n[t]) - j0);
+        all = max(cnt[0], cnt[1]);
+    }
+};
+
+// What changes a row's scores: nothing but the scale, a bias by distance, or a cap
+// (and perhaps a bias).
+enum Mode { kPlain = 0, kBias = 1, kCap = 2 };
+
+// Scores of one row in the log2 domain.  The scale goes with the log2e, and the
+// bias is linear on either side of the key the row stands beside, so a tile that
+// lies on one side for every row of the warp needs one multiply-add more.
+template <int MODE>
+struct RowScores {
+    float2 sc;              // kPlain, kBias: scale log2e; kCap: scale / cap
+    float cap2;             // kCap: cap log2e
+    float slope;            // slope log2e, 0 without
+    float place;            // the row's key less the tile's first
+    int side;               // 1: the tile's keys lie before it for every row, -1: behind, 0: both
+    __device__ __forceinline__ void set_tile(int pl) {
+        if constexpr (MODE != kPlain) {
+            place = (float)pl;
+            side = __all_sync(0xffffffffu, pl >= BKV - 1) ? 1 : __all_sync(0xffffffffu, pl <= 0) ? -1 : 0;
+        }
+    }
+    // 32 scores, keys e0 + 0..31: raw products to the log2 domain (kPlain: as they are)
+    __device__ __forceinline__ void apply(uint32_t (&r)[32], int e0) const {
+        if constexpr (MODE == kPlain) return;
+        float2 v[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+            v[u] = __fmul2_rn(make_float2(__uint_as_float(r[2 * u]), __uint_as_float(r[2 * u + 1])), sc);
+        if constexpr (MODE == kCap) {
+            float big = 0.f;
+#pragma unroll
+            for (int u = 0; u < 16; ++u) big = fmaxf(big, fmaxf(fabsf(v[u].x), fabsf(v[u].y)));
+            if (!__any_sync(0xffffffffu, big > 1.f)) {
+#pragma unroll
+                for (int u = 0; u < 16; ++u) v[u] = __fmul2_rn(tanh_poly2(v[u]), make_float2(cap2, cap2));
+            } else {   // tanh(u) = 1 - 2 / (2^(2u log2e) + 1): right at both ends
+#pragma unroll
+                for (int u = 0; u < 16; ++u) {
+                    v[u].x = cap2 * (1.f - __fdividef(2.f, ex2(v[u].x * (2.f * kLog2e)) + 1.f));
+                    v[u].y = cap2 * (1.f - __fdividef(2.f, ex2(v[u].y * (2.f * kLog2e)) + 1.f));
+                }
+            }
+        }
+        if (MODE == kBias || slope != 0.f) {
+            if (side != 0) {
+                const float s = side > 0 ? slope : -slope, base = s * ((float)e0 - place);
+#pragma unroll
+                for (int u = 0; u < 16; ++u)
+                    v[u] = __fadd2_rn(v[u], __ffma2_rn(make_float2(s, s), make_float2(2.f * u, 2.f * u + 1.f), make_float2(base, base)));
+            } else {
+#pragma unroll
+                for (int u = 0; u < 16; ++u) {
+                    v[u].x -= slope * fabsf(place - (float)(e0 + 2 * u));
+                    v[u].y -= slope * fabsf(place - (float)(e0 + 2 * u + 1));
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+            r[2 * u] = __float_as_uint(v[u].x);
+            r[2 * u + 1] = __float_as_uint(v[u].y);
+        }
+    }
+};
+
+// Of a row's 16 pairs of exponentials per 32 keys, those computed on the FMA pipe
+// (exp2_poly2): the special-function unit alone, at 6 cycles a warp, is as busy as
+// the tensor cores at head_dim 128 and busier at 64.
+template <int D>
+constexpr uint32_t kPolyPairs = D == 128 ? 0x1111u : 0x5555u;
+
+// One row's 128 scores of a K/V tile: S from TMEM, the row's maximum, P back
+// into TMEM, the row's sum.  `left` keys are the row's to see (`masked`: some row
+// of the warp does not see all); O is moved along when the reference grows.
+template <int D, bool VF16, int MODE>
+__device__ __forceinline__ void softmax_tile(uint32_t s_tmem, uint32_t o_tmem, const RowScores<MODE> &rs, int left,
+                                             bool masked, float &m_ref, float &l) {
+    auto mask = [&](uint32_t (&r)[32], int e0) {
+        if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                if (e0 + e >= left) r[e] = __float_as_uint(-INFINITY);
+        }
+    };
+    // pass 1: the row max over the 128 scores.  Keys 64..127 stay in registers
+    // (rh) for pass 2; keys 0..63 are read again (kCap: they are put back changed).
+    uint32_t rh[2][32];
+    float m8[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) m8[u] = -INFINITY;
+    auto look = [&](const uint32_t (&r)[32]) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) m8[e & 7] = fmaxf(m8[e & 7], __uint_as_float(r[e]));
+    };
+    if constexpr (MODE != kPlain) {
+        tmem_ld_32x32b_x32(s_tmem + 64, rh[0]);
+        tmem_ld_32x32b_x32(s_tmem + 96, rh[1]);
+        tmem_ld_wait_regs(rh[0]);
+        tmem_ld_wait_regs(rh[1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            rs.apply(rh[h], 64 + 32 * h);
+            mask(rh[h], 64 + 32 * h);
+            look(rh[h]);
+        }
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(s_tmem + c, r);
+            tmem_ld_wait_regs(r);
+            rs.apply(r, c);
+            mask(r, c);
+            look(r);
+            if constexpr (MODE == kCap) tmem_st_32x32b_x32(s_tmem + c, r);
+        }
+    } else {
+        uint32_t r01[2][32];
+        tmem_ld_32x32b_x32(s_tmem + 0, r01[0]);
+        tmem_ld_32x32b_x32(s_tmem + 32, r01[1]);
+        tmem_ld_32x32b_x32(s_tmem + 64, rh[0]);
+        tmem_ld_32x32b_x32(s_tmem + 96, rh[1]);
+        tmem_ld_wait_regs(r01[0]);
+        tmem_ld_wait_regs(r01[1]);
+        tmem_ld_wait_regs(rh[0]);
+        tmem_ld_wait_regs(rh[1]);
+        mask(r01[0], 0);
+        mask(r01[1], 32);
+        mask(rh[0], 64);
+        mask(rh[1], 96);
+        look(r01[0]);
+        look(r01[1]);
+        look(rh[0]);
+        look(rh[1]);
+    }
+    float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
+    if constexpr (MODE == kPlain) mx *= rs.sc.x;   // scale > 0: max(s * scale) = scale * max(s)
+    // The rows of one warp decide together: tcgen05.ld/st are
+    // warp-collective (.sync.aligned), so the O rescale runs for the
+    // whole warp when any of its rows needs it; a row that does not
+    // keeps its reference (alpha = 1).
+    const bool grow = mx > m_ref + kRescaleLog2;
+    if (__any_sync(0xffffffffu, grow)) {
+        // O_t and l are relative to m_ref; move them to mx (the P.V before
+        // was issued before this tile's QK, whose completion was waited for).
+        const float alpha = grow ? ex2(m_ref - mx) : 1.0f;   // 0 when m_ref = -inf
+        // (in an item's first tile O holds the item before's and is about to be overwritten)
+        if (__any_sync(0xffffffffu, l != 0.f)) {
+            const float2 a2 = make_float2(alpha, alpha);
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld_32x32b_x32(o_tmem + c * 32, o);
+                tmem_ld_wait_regs(o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float2 v = __fmul2_rn(make_float2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1])), a2);
+                    o[2 * e] = __float_as_uint(v.x);
+                    o[2 * e + 1] = __float_as_uint(v.y);
+                }
+                tmem_st_32x32b_x32(o_tmem + c * 32, o);
+            }
+            tmem_st_wait();
+        }
+        l *= alpha;
+        if (grow) m_ref = mx;
+    }
+    if constexpr (MODE == kCap) tmem_st_wait();
+    // pass 2: P = 2^(s - m_ref), at most 2^kRescaleLog2, in f32, stored as
+    // packed 16-bit pairs (key 2c in the low half of column c) into columns
+    // 64..127 of S_t, which pass 1 has read.  A row that has seen no key yet has
+    // m_ref = -inf and P = 2^-inf = 0.  Masked tiles take no polynomial: it
+    // does not go to 0.
+    const float base = m_ref == -INFINITY ? 0.f : -m_ref;
+    const float2 nm2 = make_float2(base, base);
+    float2 sum2 = make_float2(0.f, 0.f);
+    auto p_store = [&](const uint32_t (&r)[32], uint32_t col, auto with_poly) {   // 32 keys -> 16 columns
+        uint32_t pk[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+            const float2 s = make_float2(__uint_as_float(r[2 * u]), __uint_as_float(r[2 * u + 1]));
+            const float2 x = MODE == kPlain ? __ffma2_rn(s, rs.sc, nm2) : __fadd2_rn(s, nm2);
+            const float2 pf = decltype(with_poly)::value && ((kPolyPairs<D> >> u) & 1u) ? exp2_poly2(x) : make_float2(ex2(x.x), ex2(x.y));
+            sum2 = __fadd2_rn(sum2, pf);
+            pk[u] = pack16<VF16>(pf);
+        }
+        tmem_st_32x32b_x16(s_tmem + col, pk);
+    };
+    auto pass2 = [&](auto with_poly) {
+        uint32_t r0[2][32];
+        tmem_ld_32x32b_x32(s_tmem + 0, r0[0]);
+        tmem_ld_32x32b_x32(s_tmem + 32, r0[1]);
+        p_store(rh[0], 96, with_poly);
+        p_store(rh[1], 112, with_poly);
+        tmem_ld_wait_regs(r0[0]);
+        tmem_ld_wait_regs(r0[1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (MODE == kBias) rs.apply(r0[h], 32 * h);
+            if constexpr (MODE != kCap) mask(r0[h], 32 * h);
+            p_store(r0[h], 64 + 16 * h, with_poly);
+        }
+    };
+    if (masked) pass2(std::false_type{});
+    else pass2(std::true_type{});
+    l += sum2.x + sum2.y;
+    tmem_st_wait();             // P_t in TMEM ...
+    tc_fence_before();          // ... and ordered before the arrive for the MMA thread
+}
+
+// VF16: V (and so P) are f16, otherwise bf16; Q and K are bf16.
+template <int D, bool VF16, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
     packed_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, PackedParams p) {
@@ -128,29 +394,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     unsigned char *sQ = smem + L::Q, *sRing = smem + L::RING;
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::BAR);
-    uint64_t *q_full = bars, *v_clean = bars + 1;
+    uint64_t *q_full = bars, *q_empty = bars + 1;
     uint64_t *s_full = bars + 2, *p_full = bars + 4, *pv_done = bars + 6;   // [2] each
-    uint64_t *slot_full = bars + 8, *slot_empty = slot_full + kRing;        // [kRing] each
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(slot_empty + kRing);
-    Item *s_item = reinterpret_cast<Item *>(tmem_slot + 2);
-    int *s_found = reinterpret_cast<int *>(s_item + 1);
+    uint64_t *i_full = bars + 8, *i_empty = bars + 10;                      // [2] each: items told
+    uint64_t *slot_full = bars + 12, *slot_empty = slot_full + kRing;       // [kRing] each
+    uint64_t *a_full = slot_empty + kRing;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(a_full + 1);
+    uint64_t *answer = a_full + 2;                                          // 16 bytes: 14 + 2 kRing is even
+    Item *s_item = reinterpret_cast<Item *>(answer + 2);                    // [2]
     float2 *s_ml = reinterpret_cast<float2 *>(smem + L::ML);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int item = blockIdx.x / p.splits, split = blockIdx.x % p.splits;
-    const int kvh = item / p.pairs;
-
-    if (warp == 1) {
-        Item it{};
-        const bool found = find_item(p, item % p.pairs, lane, it);
-        if (lane == 0) {
-            *s_item = it;
-            *s_found = found;
-        }
-    }
+    const int split = blockIdx.x % p.splits;
+    const int tt = p.tile_tokens;
     if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tmQ);
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
         mbar_init(q_full, 1);
-        mbar_init(v_clean, 32);
+        mbar_init(q_empty, 1);
+        mbar_init(a_full, 1);
         for (int s = 0; s < kRing; ++s) {
             mbar_init(&slot_full[s], 1);
             mbar_init(&slot_empty[s], 1);
@@ -159,361 +422,301 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
             mbar_init(&pv_done[i], 1);
+            mbar_init(&i_full[i], 1);
+            mbar_init(&i_empty[i], 9);
         }
         fence_barrier_init();
     }
-    __syncthreads();
-    if (!*s_found) return;   // the whole cluster: its CTAs have one item
-    if (warp == 0) {
+    if (warp == 1) {
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
-    const Item it = *s_item;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     bool aborted = false;
 
-    const int tt = p.tile_tokens;
-    const int prefix = p.causal && p.prefix ? min(max(p.prefix[it.doc], 0), it.lk) : 0;
-    const int nt = it.lq > (it.tile0 + 1) * tt ? 2 : 1;   // query tiles of this CTA
-    // K/V tiles [j0, j0 + cnt[t]) of query tile t: what its last token sees, and this CTA's share of it
-    int cnt[2], j0, all;
-    {
-        int n[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-            n[t] = t < nt ? (limit_of(p, it, min((it.tile0 + t + 1) * tt, it.lq) - 1, prefix) + BKV - 1) / BKV : 0;
-        const int most = max(n[0], n[1]);
-        const int per = (most + p.splits - 1) / p.splits;
-        j0 = split * per;
-        const int j1 = min(most, j0 + per);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) cnt[t] = max(0, min(j1, n[t]) - j0);
-        all = max(cnt[0], cnt[1]);
-    }
-    // the document ends inside the last tile loaded here
-    const int tail = it.lk - (j0 + all - 1) * BKV;
-    const bool cleans = all > 0 && tail < BKV;
-
     if (warp == 0) {
-        if (all > 0 && elect_one()) {
-            tma_prefetch_desc(&tmQ);
-            tma_prefetch_desc(&tmK);
-            tma_prefetch_desc(&tmV);
-            mbar_arrive_expect_tx(q_full, nt * (D / 64) * tt * p.group * 128);
-            for (int t = 0; t < nt; ++t)
-                for (int x = 0; x < D; x += 64)
-                    tma_load_3d(sQ + t * L::TILE + (x / 64) * L::HALF, &tmQ, q_full, x, kvh * p.group,
-                                it.qs + (it.tile0 + t) * tt);
-            // load sequence: s = 2j -> K_j, s = 2j + 1 -> V_j, slot s % kRing
-            int issued = 0;
-            for (int s = 0; s < 2 * all; ++s, ++issued) {
-                const int slot = s % kRing;
-                if (!mbar_wait(&slot_empty[slot], ((s / kRing) & 1) ^ 1, p.flag, 301, &aborted)) break;
-                mbar_arrive_expect_tx(&slot_full[slot], L::TILE);
-                for (int x = 0; x < D; x += 64)
-                    tma_load_3d(sRing + slot * L::TILE + (x / 64) * L::HALF, (s & 1) ? &tmV : &tmK, &slot_full[slot], x,
-                                kvh, it.ks + (j0 + (s >> 1)) * BKV);
+        uint32_t issued = 0, n_items = 0, n_q = 0, n_asked = 0;
+        int i = blockIdx.x / p.splits;
+        // The next item, asked for when the loads of the one at hand are issued
+        // (the ring holds a few microseconds of products then): earlier, a CTA
+        // with a long item would sit on a second one.  A cluster has one item.
+        auto next = [&]() {
+            if (p.splits > 1) return -1;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(a_full, 16);
+                ask_next_cta(answer, a_full);
             }
-            // Wait for every copy this thread started before the CTA can exit.
-            bool a2 = false;
-            mbar_wait(q_full, 0, nullptr, 0, &a2);
-            for (int s = issued > kRing ? issued - kRing : 0; s < issued; ++s)
-                mbar_wait(&slot_full[s % kRing], (s / kRing) & 1, nullptr, 0, &a2);
-        }
-        aborted = __any_sync(0xffffffffu, aborted);
-        if (cleans && !aborted) {
-            const int s = 2 * all - 1;
-            mbar_wait(&slot_full[s % kRing], (s / kRing) & 1, p.flag, 302, &aborted);
-            unsigned char *v = sRing + (s % kRing) * L::TILE;
-            constexpr int kChunks = D / 64 * 8;   // 16-byte pieces of a row
-            for (int i = tail * kChunks + lane; i < BKV * kChunks; i += 32)
-                *reinterpret_cast<uint4 *>(v + (i % kChunks) / 8 * L::HALF + i / kChunks * 128 + (i % 8) * 16) =
-                    make_uint4(0, 0, 0, 0);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            mbar_arrive(v_clean);
+            if (!warp_wait(a_full, n_asked++ & 1, p.flag, 315, &aborted)) return -1;
+            const int x = next_cta(answer);
+            __syncwarp();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // read before the next answer lands
+            return x;
+        };
+        for (;;) {
+            Item it{};
+            bool more = false;
+            while (i >= 0) {
+                if ((more = find_item(p, i % p.pairs, lane, it))) break;
+                i = next();
+            }
+            it.kvh = more ? i / p.pairs : -1;   // -1: no more
+            it.load0 = issued;
+            const uint32_t b = n_items & 1;
+            if (!warp_wait(&i_empty[b], ((n_items >> 1) & 1) ^ 1, p.flag, 300, &aborted)) break;
+            if (lane == 0) {
+                s_item[b] = it;
+                mbar_arrive(&i_full[b]);
+            }
+            __syncwarp();
+            ++n_items;
+            if (!more) break;
+            const Share sh(p, it, split);
+            if (sh.all > 0) {
+                if (elect_one() && mbar_wait(q_empty, (n_q & 1) ^ 1, p.flag, 304, &aborted)) {
+                    mbar_arrive_expect_tx(q_full, sh.nt * (D / 64) * tt * p.group * 128);
+                    for (int t = 0; t < sh.nt; ++t)
+                        for (int x = 0; x < D; x += 64)
+                            tma_load_3d(sQ + t * L::TILE + (x / 64) * L::HALF, &tmQ, q_full, x, it.kvh * p.group,
+                                        it.qs + (it.tile0 + t) * tt);
+                    for (int s = 0; s < 2 * sh.all; ++s, ++issued) {   // K_j, V_j, the last tile first
+                        const int slot = issued % kRing;
+                        if (!mbar_wait(&slot_empty[slot], ((issued / kRing) & 1) ^ 1, p.flag, 301, &aborted)) break;
+                        mbar_arrive_expect_tx(&slot_full[slot], L::TILE);
+                        for (int x = 0; x < D; x += 64)
+                            tma_load_3d(sRing + slot * L::TILE + (x / 64) * L::HALF, (s & 1) ? &tmV : &tmK,
+                                        &slot_full[slot], x, it.kvh, it.ks + (sh.j0 + sh.all - 1 - (s >> 1)) * BKV);
+                    }
+                    if (aborted) {   // let the copies already issued land before the CTA exits
+                        bool a2 = false;
+                        mbar_wait(q_full, n_q & 1, nullptr, 0, &a2);
+                        a2 = false;
+                        for (uint32_t s = issued > (uint32_t)kRing ? issued - kRing : 0; s < issued; ++s)
+                            mbar_wait(&slot_full[s % kRing], (s / kRing) & 1, nullptr, 0, &a2);
+                    }
+                }
+                ++n_q;
+            }
+            // every lane goes on from the elected one's count
+            issued = __reduce_max_sync(0xffffffffu, issued);
+            aborted = __any_sync(0xffffffffu, aborted);
+            if (aborted) break;
+            i = next();
         }
     } else if (warp == 1) {
-        if (all > 0 && elect_one()) {
+        if (elect_one()) {
             constexpr uint32_t idesc_qk = idesc_f16(BQ, BKV, true, false);
             constexpr uint32_t idesc_pv = idesc_f16(BQ, D, !VF16, true);   // A = P (TMEM), B = V, MN-major
             const uint32_t q_addr = smem_u32(sQ);
-            auto wait_slot = [&](int s, int code) {
-                return mbar_wait(&slot_full[s % kRing], (s / kRing) & 1, p.flag, code, &aborted);
-            };
-            auto issue_qk = [&](int t, int j) {   // S_t = Q_t K_j^T
-                const uint32_t k_addr = smem_u32(sRing + (2 * j) % kRing * L::TILE);
-#pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = (kk >> 2) * L::HALF + (kk & 3) * 32;
-                    umma_f16_ss(tmem + t * 128, sdesc_sw128(q_addr + t * L::TILE + off, 16, 1024),
-                                sdesc_sw128(k_addr + off, 16, 1024), idesc_qk, kk ? 1u : 0u);
+            uint32_t n_items = 0, n_q = 0, n_p[2] = {0, 0};
+            while (!aborted) {
+                const uint32_t b = n_items & 1;
+                if (!mbar_wait(&i_full[b], (n_items >> 1) & 1, p.flag, 302, &aborted)) break;
+                const Item it = s_item[b];
+                mbar_arrive(&i_empty[b]);
+                ++n_items;
+                if (it.kvh < 0) break;
+                const Share sh(p, it, split);
+                const uint32_t used = it.load0;
+                if (sh.all == 0) {   // nothing to see: O is final as it is
+                    umma_commit(&pv_done[0]);
+                    umma_commit(&pv_done[1]);
+                    continue;
                 }
-                umma_commit(&s_full[t]);
-            };
-            auto issue_pv = [&](int t, int j) {   // O_t (+)= P_t V_j; P_t: TMEM columns 64..127 of S_t
-                const uint32_t v_addr = smem_u32(sRing + (2 * j + 1) % kRing * L::TILE);
+                auto wait_load = [&](uint32_t s, int code) {
+                    return mbar_wait(&slot_full[s % kRing], (s / kRing) & 1, p.flag, code, &aborted);
+                };
+                auto issue_qk = [&](int t, int j) {   // S_t = Q_t K_j^T
+                    const uint32_t k_addr = smem_u32(sRing + (used + 2 * j) % kRing * L::TILE);
 #pragma unroll
-                for (int kk = 0; kk < BKV / 16; ++kk) {   // 16 keys = 8 packed columns per MMA
-                    const uint64_t bd = sdesc_sw128(v_addr + kk * 2048, L::HALF, 1024);
-                    umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + 64 + kk * 8, bd, idesc_pv,
-                                (j > 0 || kk > 0) ? 1u : 0u);
-                }
-            };
-            bool ok = mbar_wait(q_full, 0, p.flag, 305, &aborted) && wait_slot(0, 306);
-            if (ok) {
-                tc_fence_after();
-                for (int t = 0; t < 2; ++t)
-                    if (cnt[t] > 0) issue_qk(t, 0);
-                umma_commit(&slot_empty[0]);   // K_0 read by both
-            }
-            for (int j = 0; ok && j < all; ++j) {
-                // Per tile: PV_t(j) once the softmax has stored P_t(j) (p_full),
-                // then QK_t(j+1) into the same columns: MMAs of one thread run
-                // in issue order, so P_t(j) is read before S_t(j+1) lands.
-                if (!wait_slot(2 * j + 1, 307)) break;
-                const bool next = j + 1 < all;
-                if (next && !wait_slot(2 * j + 2, 308)) break;
-                if (!next && cleans && !mbar_wait(v_clean, 0, p.flag, 303, &aborted)) break;
-                for (int t = 0; t < 2; ++t) {
-                    if (j >= cnt[t]) continue;
-                    if (!mbar_wait(&p_full[t], j & 1, p.flag, 309 + t, &aborted)) {
-                        ok = false;
-                        break;
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t off = (kk >> 2) * L::HALF + (kk & 3) * 32;
+                        umma_f16_ss(tmem + t * 128, sdesc_sw128(q_addr + t * L::TILE + off, 16, 1024),
+                                    sdesc_sw128(k_addr + off, 16, 1024), idesc_qk, kk ? 1u : 0u);
                     }
+                    umma_commit(&s_full[t]);
+                };
+                // tile t works on loads j >= skip(t): its tokens do not see the last keys
+                auto skip = [&](int t) { return sh.all - sh.cnt[t]; };
+                bool ok = mbar_wait(q_full, n_q & 1, p.flag, 305, &aborted) && wait_load(used, 306);
+                ++n_q;
+                if (ok) {
                     tc_fence_after();
-                    issue_pv(t, j);
-                    if (j + 1 < cnt[t])
-                        issue_qk(t, j + 1);
-                    else
-                        umma_commit(&pv_done[t]);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        if (skip(t) == 0) issue_qk(t, 0);
+                    umma_commit(&slot_empty[used % kRing]);   // K_0 read
                 }
-                if (!ok) break;
-                umma_commit(&slot_empty[(2 * j + 1) % kRing]);             // V_j read
-                if (next) umma_commit(&slot_empty[(2 * j + 2) % kRing]);   // K_{j+1} read
-            }
-        }
-    }
-
-    // Softmax warps: tile t = 0 (warps 2-5) or 1 (warps 6-9), row quad*32 + lane.
-    const int t = (warp - 2) >> 2;
-    const int quad = warp & 3;
-    const int r_in = quad * 32 + lane;
-    const int token = (it.tile0 + t) * tt + r_in / p.group;   // in the document
-    const bool row_ok = warp >= 2 && t < nt && r_in < tt * p.group && token < it.lq;
-    const int head = kvh * p.group + r_in % p.group;
-    const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    const uint32_t o_tmem = tmem + lane_base + 256 + t * 128;
-    float m_ref = -INFINITY;   // the max P is taken against (log2 domain)
-    float l = 0.f;
-    if (warp >= 2) {
-        const int n_mine = t ? cnt[1] : cnt[0];
-        const uint32_t s_tmem = tmem + lane_base + t * 128;
-        const int lim = row_ok ? limit_of(p, it, token, prefix) : 0x7fffffff;
-        const int lim_min = __reduce_min_sync(0xffffffffu, lim);
-        const bool active = lim_min != 0x7fffffff;   // the warp holds rows
-        ScoreMod mod{};
-        float sc = p.scale * kLog2e;
-        if constexpr (MOD) {
-            mod.scale = p.scale;
-            mod.twice_over_cap = p.softcap > 0.f ? 2.f * kLog2e / p.softcap : 0.f;
-            mod.cap2 = p.softcap * kLog2e;
-            mod.slope2 = p.slopes && row_ok ? p.slopes[head] * kLog2e : 0.f;
-            sc = 1.f;
-        }
-        const float2 sl2 = make_float2(sc, sc);
-        for (int j = 0; j < n_mine && !aborted; ++j) {
-            // warp-uniform outcome: the tcgen05.ld/st below are warp-collective
-            if (!warp_wait(&s_full[t], j & 1, p.flag, 311, &aborted)) break;
-            if (!active) {   // no row here: P may hold anything, its O is not read
-                if (lane == 0) mbar_arrive(&p_full[t]);
-                continue;
-            }
-            tc_fence_after();
-            const int kv0 = (j0 + j) * BKV;
-            const int left = lim - kv0;                       // keys of this tile the row sees
-            const bool masked = lim_min < kv0 + BKV;          // not all of them for every row of the warp
-            if constexpr (MOD) mod.place = (float)((int64_t)token + it.lk - it.lq - kv0);
-            // pass 1: the row max over the 128 scores.  Keys 64..127 stay in
-            // registers (rh) for pass 2; keys 0..63 are read again (MOD: they
-            // are put back changed).
-            uint32_t rh[2][32];
-            float mx;
-            {
-                uint32_t r01[2][32];
-                tmem_ld_32x32b_x32(s_tmem + 0, r01[0]);
-                tmem_ld_32x32b_x32(s_tmem + 32, r01[1]);
-                tmem_ld_32x32b_x32(s_tmem + 64, rh[0]);
-                tmem_ld_32x32b_x32(s_tmem + 96, rh[1]);
-                tmem_ld_wait_regs(r01[0]);
-                tmem_ld_wait_regs(r01[1]);
-                tmem_ld_wait_regs(rh[0]);
-                tmem_ld_wait_regs(rh[1]);
-                if constexpr (MOD) {
+                for (int j = 0; ok && j < sh.all; ++j) {
+                    // Per tile: PV_t(j) once the softmax has stored P_t(j) (p_full),
+                    // then QK_t(j+1) into the same columns: MMAs of one thread run
+                    // in issue order, so P_t(j) is read before S_t(j+1) lands.
+                    const uint32_t v = used + 2 * j + 1;
+                    if (!wait_load(v, 307)) break;
+                    const bool next = j + 1 < sh.all;
+                    if (next && !wait_load(v + 1, 308)) break;
 #pragma unroll
-                    for (int e = 0; e < 64; ++e) {
-                        r01[e >> 5][e & 31] = __float_as_uint(mod(__uint_as_float(r01[e >> 5][e & 31]), e));
-                        rh[e >> 5][e & 31] = __float_as_uint(mod(__uint_as_float(rh[e >> 5][e & 31]), 64 + e));
-                    }
-                }
-                if (masked) {
+                    for (int t = 0; t < 2; ++t) {
+                        if (j >= skip(t)) {
+                            if (!mbar_wait(&p_full[t], n_p[t] & 1, p.flag, 309 + t, &aborted)) {
+                                ok = false;
+                                break;
+                            }
+                            ++n_p[t];
+                            tc_fence_after();
+                            const uint32_t v_addr = smem_u32(sRing + v % kRing * L::TILE);
 #pragma unroll
-                    for (int e = 0; e < 64; ++e) {
-                        if (e >= left) r01[e >> 5][e & 31] = __float_as_uint(-INFINITY);
-                        if (64 + e >= left) rh[e >> 5][e & 31] = __float_as_uint(-INFINITY);
-                    }
-                }
-                if constexpr (MOD) {
-                    tmem_st_32x32b_x32(s_tmem + 0, r01[0]);
-                    tmem_st_32x32b_x32(s_tmem + 32, r01[1]);
-                }
-                float m8[8];
-#pragma unroll
-                for (int u = 0; u < 8; ++u) m8[u] = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < 64; ++e) {
-                    m8[e & 7] = fmaxf(m8[e & 7], __uint_as_float(r01[e >> 5][e & 31]));
-                    m8[(e + 4) & 7] = fmaxf(m8[(e + 4) & 7], __uint_as_float(rh[e >> 5][e & 31]));
-                }
-                mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
-            }
-            mx *= sc;   // scale > 0: max(s * scale) = scale * max(s)
-            // The rows of one warp decide together: tcgen05.ld/st are
-            // warp-collective (.sync.aligned), so the O rescale runs for the
-            // whole warp when any of its rows needs it; a row that does not
-            // keeps its reference (alpha = 1).
-            const bool grow = mx > m_ref + kRescaleLog2;
-            if (__any_sync(0xffffffffu, grow)) {
-                // O_t and l are relative to m_ref; move them to mx (PV_t(j-1)
-                // was issued before QK_t(j), whose completion was waited for).
-                const float alpha = grow ? ex2(m_ref - mx) : 1.0f;   // 0 when m_ref = -inf
-                if (j > 0) {
-                    const float2 a2 = make_float2(alpha, alpha);
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld_32x32b_x32(o_tmem + c * 32, o);
-                        tmem_ld_wait_regs(o);
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float2 v = __fmul2_rn(make_float2(__uint_as_float(o[2 * e]), __uint_as_float(o[2 * e + 1])), a2);
-                            o[2 * e] = __float_as_uint(v.x);
-                            o[2 * e + 1] = __float_as_uint(v.y);
+                            for (int kk = 0; kk < BKV / 16; ++kk)   // O_t (+)= P_t V_j: 16 keys = 8 packed columns per MMA
+                                umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + 64 + kk * 8,
+                                            sdesc_sw128(v_addr + kk * 2048, L::HALF, 1024), idesc_pv,
+                                            (j > skip(t) || kk > 0) ? 1u : 0u);
                         }
-                        tmem_st_32x32b_x32(o_tmem + c * 32, o);
+                        if (!next) umma_commit(&pv_done[t]);
+                        if (next && j + 1 >= skip(t)) issue_qk(t, j + 1);
                     }
-                    tmem_st_wait();
-                }
-                l *= alpha;
-                if (grow) m_ref = mx;
-            }
-            if constexpr (MOD) tmem_st_wait();
-            // pass 2: P = 2^(s - m_ref), at most 2^kRescaleLog2, in f32, stored as
-            // packed 16-bit pairs (key 2c in the low half of column c) into
-            // columns 64..127 of S_t, which pass 1 has read.  A row that has seen
-            // no key yet has m_ref = -inf and P = 2^-inf = 0.
-            const float base = m_ref == -INFINITY ? 0.f : -m_ref;
-            const float2 nm2 = make_float2(base, base);
-            float2 sum2 = make_float2(0.f, 0.f);
-            auto p_store = [&](const uint32_t (&r)[32], uint32_t col) {   // 32 keys -> 16 columns
-                uint32_t pk[16];
-#pragma unroll
-                for (int u = 0; u < 16; ++u) {
-                    const float2 x = __ffma2_rn(make_float2(__uint_as_float(r[2 * u]), __uint_as_float(r[2 * u + 1])),
-                                                sl2, nm2);
-                    const float2 pf = make_float2(ex2(x.x), ex2(x.y));
-                    sum2 = __fadd2_rn(sum2, pf);
-                    if constexpr (VF16) {
-                        uint32_t out;
-                        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(out) : "f"(pf.y), "f"(pf.x));
-                        pk[u] = out;
-                    } else {
-                        __nv_bfloat162 hv = __floats2bfloat162_rn(pf.x, pf.y);
-                        pk[u] = *reinterpret_cast<uint32_t *>(&hv);
-                    }
-                }
-                tmem_st_32x32b_x16(s_tmem + col, pk);
-            };
-            {
-                uint32_t r0[2][32];
-                tmem_ld_32x32b_x32(s_tmem + 0, r0[0]);
-                tmem_ld_32x32b_x32(s_tmem + 32, r0[1]);
-                p_store(rh[0], 96);
-                p_store(rh[1], 112);
-                tmem_ld_wait_regs(r0[0]);
-                tmem_ld_wait_regs(r0[1]);
-                if (!MOD && masked) {
-#pragma unroll
-                    for (int e = 0; e < 64; ++e)
-                        if (e >= left) r0[e >> 5][e & 31] = __float_as_uint(-INFINITY);
-                }
-                p_store(r0[0], 64);
-                p_store(r0[1], 80);
-            }
-            l += sum2.x + sum2.y;
-            tmem_st_wait();             // P_t(j) in TMEM ...
-            tc_fence_before();          // ... and ordered before the arrive for the MMA thread
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t]);
-        }
-        // O_t is final once the last P.V has completed; the ring is free once both tiles' have.
-        for (int u = 0; u < 2; ++u)
-            if (cnt[u] > 0) warp_wait(&pv_done[u], 0, p.flag, 312, &aborted);
-        tc_fence_after();
-    }
-
-    __nv_bfloat16 *dst = p.out + (int64_t)(it.qs + token) * p.ldo + head * D;
-    const bool any_o = warp >= 2 && (t ? cnt[1] : cnt[0]) > 0;   // warp-uniform
-    if (p.splits == 1) {
-        if (warp >= 2 && !aborted) {
-            const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);   // a row that saw no key is 0, NaN stays
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t r[32];
-                if (any_o) {
-                    tmem_ld_32x32b_x32(o_tmem + c * 32, r);
-                    tmem_ld_wait_regs(r);
-                }
-                if (!row_ok) continue;
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        __nv_bfloat162 hv = __floats2bfloat162_rn(__uint_as_float(r[g * 8 + 2 * e]) * inv,
-                                                                  __uint_as_float(r[g * 8 + 2 * e + 1]) * inv);
-                        w[e] = any_o ? *reinterpret_cast<uint32_t *>(&hv) : 0u;
-                    }
-                    *reinterpret_cast<uint4 *>(dst + c * 32 + g * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (!ok) break;
+                    umma_commit(&slot_empty[v % kRing]);                     // V_j read
+                    if (next) umma_commit(&slot_empty[(v + 1) % kRing]);     // K_{j+1} read
+                    if (j + 2 == sh.all || sh.all == 1) umma_commit(q_empty);   // the last QK has been issued
                 }
             }
         }
     } else {
-        // Join the cluster's partial results.  Every CTA publishes its rows'
-        // (maximum, sum) and, weighted by them, its O in the ring's place; then
-        // rank s sums columns [s D/S, (s+1) D/S) over the ranks, in their order.
-        if (warp >= 2) s_ml[t * 128 + r_in] = make_float2(m_ref, l);
-        cluster_sync();
-        float w_own = 0.f;
-        if (row_ok) {
-            float top = -INFINITY;
-            for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ld_peer2(peer_addr(&s_ml[t * 128 + r_in], s)).x);
-            float total = 0.f;
-            for (int s = 0; s < p.splits; ++s) {
-                const float2 ml = ld_peer2(peer_addr(&s_ml[t * 128 + r_in], s));
-                total += ml.y * (ml.x == -INFINITY ? 0.f : ex2(ml.x - top));
+        // Softmax warps: tile t = 0 (warps 2-5) or 1 (warps 6-9), row quad*32 + lane.
+        const int t = (warp - 2) >> 2;
+        const int quad = warp & 3;
+        const int r_thread = quad * 32 + lane;
+        const uint32_t s_tmem = tmem + ((uint32_t)(quad * 32) << 16) + t * 128, o_tmem = s_tmem + 256;
+        RowScores<MODE> rs{};
+        const float sc = MODE == kCap ? p.scale / p.softcap : p.scale * kLog2e;
+        rs.sc = make_float2(sc, sc);
+        if constexpr (MODE == kCap) rs.cap2 = p.softcap * kLog2e;
+        uint32_t n_items = 0, n_s = 0;
+        float m_ref = -INFINITY, l = 0.f;   // a row's maximum that P is taken against (log2 domain), its sum
+        bool row_ok = false, any_o = false, join = false;
+        __nv_bfloat16 *dst = nullptr;
+        while (!aborted) {
+            // The item stays in shared memory (volatile: read again behind the
+            // tiles, not kept in registers through them).
+            const volatile Item &it = s_item[n_items & 1];
+            if (!warp_wait(&i_full[n_items & 1], (n_items >> 1) & 1, p.flag, 303, &aborted)) break;
+            if (it.kvh < 0) break;
+            const int r_in = fresh(r_thread);
+            int n_mine, left, left_min, place, clean = BKV;   // keys a row sees in the tile at hand, the warp's least
+            {
+                const Item i{it.qs, it.lq, it.ks, it.lk, it.tile0, it.doc, it.kvh, 0};
+                const Share sh(p, i, split);
+                const int token = (i.tile0 + t) * tt + r_in / p.group;   // in the document
+                const bool ok = t < sh.nt && r_in < tt * p.group && token < i.lq;
+                n_mine = t ? sh.cnt[1] : sh.cnt[0];
+                const int top = (sh.j0 + n_mine - 1) * BKV;       // first key of the tile to begin with
+                row_ok = ok;
+                left = ok ? limit_of(p, i, token, sh.prefix) - top : kNoRow;
+                left_min = __reduce_min_sync(0xffffffffu, left);
+                place = token + i.lk - i.lq - top;
+                if constexpr (MODE != kPlain)
+                    rs.slope = p.slopes && ok ? p.slopes[i.kvh * p.group + r_in % p.group] * kLog2e : 0.f;
+                // V rows behind the document's end, in the first tile loaded: tile
+                // A's threads zero theirs, B's where A skips that tile
+                if (top + BKV > i.lk && (t == 0 || sh.cnt[0] < sh.cnt[1])) clean = i.lk - top;
             }
-            // no key seen anywhere: all weights 0; a NaN sum stays NaN
-            if (m_ref != -INFINITY) w_own = ex2(m_ref - top) / total;
-            else if (l != l) w_own = l;
+            any_o = n_mine > 0;   // warp-uniform
+            m_ref = -INFINITY;
+            l = 0.f;
+            const bool active = left_min != kNoRow;   // the warp holds rows
+            for (; n_mine > 0; --n_mine, left += BKV, left_min += BKV, place += BKV) {
+                // warp-uniform outcome: the tcgen05.ld/st below are warp-collective
+                if (!warp_wait(&s_full[t], n_s & 1, p.flag, 311, &aborted)) break;
+                ++n_s;
+                if (active) {
+                    tc_fence_after();
+                    rs.set_tile(place);
+                    softmax_tile<D, VF16, MODE>(s_tmem, o_tmem, rs, left, left_min < BKV, m_ref, l);
+                }
+                if (clean < BKV) {
+                    if (r_in >= clean) {
+                        const uint32_t s = it.load0 + 1;
+                        mbar_wait(&slot_full[s % kRing], (s / kRing) & 1, p.flag, 313, &aborted);
+                        unsigned char *v = sRing + (s % kRing) * L::TILE + r_in * 128;
+#pragma unroll
+                        for (int x = 0; x < D / 64; ++x)
+#pragma unroll
+                            for (int c = 0; c < 8; ++c)
+                                *reinterpret_cast<uint4 *>(v + x * L::HALF + c * 16) = make_uint4(0, 0, 0, 0);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                    aborted = __any_sync(0xffffffffu, aborted);
+                    clean = BKV;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t]);
+            }
+            // O_t is final once the last P.V has completed; in a cluster the ring is free once both tiles' have.
+            warp_wait(&pv_done[t], n_items & 1, p.flag, 312, &aborted);
+            if (p.splits > 1) warp_wait(&pv_done[t ^ 1], n_items & 1, p.flag, 314, &aborted);
+            tc_fence_after();
+            const int r_now = fresh(r_thread);
+            dst = p.out + ((int64_t)it.qs + (it.tile0 + t) * tt + r_now / p.group) * p.ldo +
+                  (it.kvh * p.group + r_now % p.group) * D;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&i_empty[n_items & 1]);
+            ++n_items;
+            if (p.splits > 1) {   // one item: joined below
+                join = !aborted;
+                break;
+            }
+            if (!aborted && any_o) {
+                const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);   // a row that saw no key is 0, NaN stays
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t r[32];
+                    tmem_ld_32x32b_x32(o_tmem + c * 32, r);
+                    tmem_ld_wait_regs(r);
+                    if (!row_ok) continue;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = pack16<false>(make_float2(__uint_as_float(r[g * 8 + 2 * e]) * inv, __uint_as_float(r[g * 8 + 2 * e + 1]) * inv));
+                        *reinterpret_cast<uint4 *>(dst + c * 32 + g * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            } else if (!aborted && row_ok) {   // no row of the tile sees a key
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4 *>(dst + c * 8) = make_uint4(0, 0, 0, 0);
+            }
+            tc_fence_before();   // O_t has been read: the next item's first P.V, after p_full, may write it
         }
-        float4 *part = reinterpret_cast<float4 *>(sRing) + (t * 128 + r_in) * (D / 4);
-        if (warp >= 2) {
+        if (p.splits > 1 && !join) {   // no item, or a wait that gave up: meet the others all the same
+            cluster_sync();
+            cluster_sync();
+            cluster_sync();
+        } else if (p.splits > 1) {
+            // Join the cluster's partial results.  Every CTA publishes its rows'
+            // (maximum, sum) and, weighted by them, its O in the ring's place; then
+            // rank s sums columns [s D/S, (s+1) D/S) over the ranks, in their order.
+            s_ml[t * 128 + r_thread] = make_float2(m_ref, l);
+            cluster_sync();
+            float w_own = 0.f;
+            if (row_ok) {
+                float top = -INFINITY;
+                for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ld_peer2(peer_addr(&s_ml[t * 128 + r_thread], s)).x);
+                float total = 0.f;
+                for (int s = 0; s < p.splits; ++s) {
+                    const float2 ml = ld_peer2(peer_addr(&s_ml[t * 128 + r_thread], s));
+                    total += ml.y * (ml.x == -INFINITY ? 0.f : ex2(ml.x - top));
+                }
+                // no key seen anywhere: all weights 0; a NaN sum stays NaN
+                if (m_ref != -INFINITY) w_own = ex2(m_ref - top) / total;
+                else if (l != l) w_own = l;
+            }
+            float4 *part = reinterpret_cast<float4 *>(sRing) + (t * 128 + r_thread) * (D / 4);
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
-                uint32_t r[32];
+                uint32_t r[32] = {};
                 if (any_o) {
                     tmem_ld_32x32b_x32(o_tmem + c * 32, r);
                     tmem_ld_wait_regs(r);
@@ -525,43 +728,52 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (any_o && w_own != 0.f)
                         v = make_float4(__uint_as_float(r[4 * q]) * w_own, __uint_as_float(r[4 * q + 1]) * w_own,
                                         __uint_as_float(r[4 * q + 2]) * w_own, __uint_as_float(r[4 * q + 3]) * w_own);
-                    part[(c * 8 + q) ^ (r_in & 7)] = v;
+                    part[(c * 8 + q) ^ (r_thread & 7)] = v;
                 }
             }
+            cluster_sync();
+            if (row_ok && !aborted) {
+                const int per = D / 4 / p.splits;   // 16-byte pieces of a row for each rank
+                for (int i = split * per; i < (split + 1) * per; ++i) {
+                    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int s = 0; s < p.splits; ++s) {
+                        const float4 v = ld_peer4(peer_addr(&part[i ^ (r_thread & 7)], s));
+                        a.x += v.x;
+                        a.y += v.y;
+                        a.z += v.z;
+                        a.w += v.w;
+                    }
+                    __nv_bfloat162 h0 = __floats2bfloat162_rn(a.x, a.y), h1 = __floats2bfloat162_rn(a.z, a.w);
+                    *reinterpret_cast<uint2 *>(dst + i * 4) =
+                        make_uint2(*reinterpret_cast<uint32_t *>(&h0), *reinterpret_cast<uint32_t *>(&h1));
+                }
+            }
+            cluster_sync();   // the peers have read this CTA's shared memory
         }
+    }
+    if (p.splits > 1 && warp < 2) {   // the softmax warps' three
         cluster_sync();
-        if (row_ok && !aborted) {
-            const int per = D / 4 / p.splits;   // 16-byte pieces of a row for each rank
-            for (int i = split * per; i < (split + 1) * per; ++i) {
-                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int s = 0; s < p.splits; ++s) {
-                    const float4 v = ld_peer4(peer_addr(&part[i ^ (r_in & 7)], s));
-                    a.x += v.x;
-                    a.y += v.y;
-                    a.z += v.z;
-                    a.w += v.w;
-                }
-                __nv_bfloat162 h0 = __floats2bfloat162_rn(a.x, a.y), h1 = __floats2bfloat162_rn(a.z, a.w);
-                *reinterpret_cast<uint2 *>(dst + i * 4) =
-                    make_uint2(*reinterpret_cast<uint32_t *>(&h0), *reinterpret_cast<uint32_t *>(&h1));
-            }
-        }
-        cluster_sync();   // the peers have read this CTA's shared memory
+        cluster_sync();
+        cluster_sync();
     }
 
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) {
+    if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
 }
 
 template <int D>
-cudaError_t launch_packed(bool f16, bool mod, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
+cudaError_t launch_packed(bool f16, Mode mode, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
                           const PackedParams &p, cudaStream_t st) {
-    auto kern = f16 ? (mod ? packed_kernel<D, true, true> : packed_kernel<D, true, false>)
-                    : (mod ? packed_kernel<D, false, true> : packed_kernel<D, false, false>);
+    auto kern = f16 ? (mode == kCap    ? packed_kernel<D, true, kCap>
+                       : mode == kBias ? packed_kernel<D, true, kBias>
+                                       : packed_kernel<D, true, kPlain>)
+                    : (mode == kCap    ? packed_kernel<D, false, kCap>
+                       : mode == kBias ? packed_kernel<D, false, kBias>
+                                       : packed_kernel<D, false, kPlain>);
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::BYTES);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
@@ -627,7 +839,7 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const void *q_dev, int64_t
     if (docs < 0 || rows_q < 0 || rows_k < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads)
         return fail(ctx, LTX_ERR_SHAPE, "%s: %d documents, %d x %d rows, %d heads over %d key heads", w, docs, rows_q,
                     rows_k, heads, kv_heads);
-    if (rows_q > 1 << 30 || rows_k > 1 << 30) return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: more than 2^30 rows", w);
+    if (rows_q > 1 << 29 || rows_k > 1 << 29) return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: more than 2^29 rows", w);
     if (heads / kv_heads > 128) return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: more than 128 heads per key head", w);
     if (!(scale > 0.f) || !std::isfinite(scale) || !(softcap >= 0.f) || !std::isfinite(softcap))
         return fail(ctx, LTX_ERR_INVALID_ARG, "%s: scale must be finite and > 0, softcap finite and >= 0", w);
@@ -666,8 +878,8 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const void *q_dev, int64_t
     // tiles each if one document had them all.
     while (p.splits < 8 && items * p.splits * 2 <= ctx->sm_count && (int64_t)p.splits * 4 * BKV <= rows_k) p.splits *= 2;
     p.pairs = (int)pairs;
-    const bool mod = softcap > 0.f || slopes_dev;
-    const cudaError_t e = head_dim == 64 ? launch_packed<64>(v_dtype == LTX_F16, mod, tq, tk, tv, p, ctx->stream)
-                                         : launch_packed<128>(v_dtype == LTX_F16, mod, tq, tk, tv, p, ctx->stream);
+    const Mode mode = softcap > 0.f ? kCap : slopes_dev ? kBias : kPlain;
+    const cudaError_t e = head_dim == 64 ? launch_packed<64>(v_dtype == LTX_F16, mode, tq, tk, tv, p, ctx->stream)
+                                         : launch_packed<128>(v_dtype == LTX_F16, mode, tq, tk, tv, p, ctx->stream);
     return e == cudaSuccess ? LTX_OK : cuda_fail(ctx, e, w);
 }

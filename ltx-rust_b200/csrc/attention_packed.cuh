@@ -23,9 +23,11 @@ struct PackedParams {
     int *flag;
 };
 
-// A document's rows, and the first query tile a CTA works on there.
+// A document's rows, the first query tile and the key head a CTA works on there;
+// how many K and V tiles the CTA loaded before it.
 struct Item {
-    int qs, lq, ks, lk, tile0, doc;
+    int qs, lq, ks, lk, tile0, doc, kvh;
+    uint32_t load0;
 };
 
 // Document i's rows [s, e) of an offsets array, kept inside [0, rows] whatever
@@ -55,6 +57,47 @@ struct ScoreMod {
         return s - slope2 * fabsf(place - (float)e);
     }
 };
+
+// 2^x on the FMA pipe, two at a time, as exp2_fma2 of attention.cu: x = n + f with
+// n = rint(x), 2^f by a cubic (7.7e-5 relative, under f16's half step), 2^n added
+// to the exponent; below 2^-30 it stays there.  A NaN stays one.
+__device__ __forceinline__ float2 exp2_poly2(float2 x) {
+    constexpr float kRound = 12582912.0f;   // 1.5 * 2^23
+    constexpr float c0 = 0x1.fff682p-1f, c1 = 0x1.62f1e0p-1f, c2 = 0x1.f0e03ap-3f, c3 = 0x1.c46242p-5f;
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-30.f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-30.f));
+    const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
+    const float2 n = __fadd2_rn(t, make_float2(-kRound, -kRound));
+    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+    float2 q = __ffma2_rn(make_float2(c3, c3), f, make_float2(c2, c2));
+    q = __ffma2_rn(q, f, make_float2(c1, c1));
+    q = __ffma2_rn(q, f, make_float2(c0, c0));
+    return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(t.x) << 23)),
+                       __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(t.y) << 23)));
+}
+
+// tanh(u) for |u| <= 1, two at a time: u q(u^2), q of degree 5 fitted here to the
+// least absolute error of tanh (3.0e-7).
+__device__ __forceinline__ float2 tanh_poly2(float2 u) {
+    constexpr float t0 = 0x1.ffff96p-1f, t1 = -0x1.553ce0p-2f, t2 = 0x1.0f6ea4p-3f, t3 = -0x1.a191d8p-5f,
+                    t4 = 0x1.0803c6p-6f, t5 = -0x1.742ca4p-9f;
+    const float2 z = __fmul2_rn(u, u);
+    float2 q = __ffma2_rn(make_float2(t5, t5), z, make_float2(t4, t4));
+    q = __ffma2_rn(q, z, make_float2(t3, t3));
+    q = __ffma2_rn(q, z, make_float2(t2, t2));
+    q = __ffma2_rn(q, z, make_float2(t1, t1));
+    q = __ffma2_rn(q, z, make_float2(t0, t0));
+    return __fmul2_rn(q, u);
+}
+
+// Two f32 to a pair of f16 or bf16, the first in the low half.
+template <bool F16>
+__device__ __forceinline__ uint32_t pack16(float2 v) {
+    uint32_t r;
+    if constexpr (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(v.y), "f"(v.x));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(v.y), "f"(v.x));
+    return r;
+}
 
 // attention_packed_few.cu: few query rows per document, as rows_per_doc counts
 // them (heads of a group included).  Enqueues the attention and the join of
