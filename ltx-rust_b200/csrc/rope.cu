@@ -31,37 +31,51 @@ struct TableParams {
     float *cos_out, *sin_out;
 };
 
-// The angle in turns, pos * g_i / 2pi, is reduced to [-1/2, 1/2] in f64 (a
-// position of 2^24 has 2.7 million turns) and only the fraction goes to f32:
-// its rounding is at most 2^-26 turns, 1e-7 of the unit circle.
-//
+// sin and cos of `quarters` quarter turns.  The whole quarters are split off in
+// f64 by adding 1.5 * 2^52 (a position of 2^24 has 11 million); only the rest r,
+// |r| <= 1/2, goes to f32, its rounding at most 2^-26 quarters.  sin(pi r/2) =
+// r S(r^2) and cos(pi r/2) = C(r^2) with S of degree 3 and C of degree 4, fitted
+// here to the least absolute error: with the f32 roundings 9.4e-8 at most, 2e-8
+// root mean square.
+__device__ __forceinline__ void sincos_quarters(double quarters, float &s, float &c) {
+    constexpr double kRound = 6755399441055744.0;
+    constexpr float s0 = 0x1.921fb4p+0f, s1 = -0x1.4abba8p-1f, s2 = 0x1.465a3ep-4f, s3 = -0x1.2cf5d4p-8f;
+    constexpr float c1 = -0x1.3bd3ccp+0f, c2 = 0x1.03c1dcp-2f, c3 = -0x1.55c57cp-6f, c4 = 0x1.d9c364p-11f;
+    const double t = quarters + kRound;
+    const unsigned q = (unsigned)__double2loint(t);
+    const float r = (float)(quarters - (t - kRound)), z = r * r;
+    const float sn = r * fmaf(fmaf(fmaf(s3, z, s2), z, s1), z, s0);
+    const float cs = fmaf(fmaf(fmaf(fmaf(c4, z, c3), z, c2), z, c1), z, 1.f);
+    const float a = q & 1 ? cs : sn, b = q & 1 ? sn : cs;
+    s = __uint_as_float(__float_as_uint(a) ^ ((q & 2) << 30));
+    c = __uint_as_float(__float_as_uint(b) ^ (((q + 1) & 2) << 30));
+}
+
 // A thread keeps VEC neighbouring frequencies of its own and walks down the
 // rows: no division per value, 16-byte stores (VEC 4; 1 where rot_dim / 2 is
-// no multiple of 4).
+// no multiple of 4).  A value costs some 25 instructions, so the stores bound it.
 template <int VEC>
 __global__ void __launch_bounds__(256) rope_table_1d_kernel(TableParams p) {
-    __shared__ double s_turns[kMaxRot / 2];
+    __shared__ double s_quarters[kMaxRot / 2];   // per position
     for (int i = threadIdx.x; i < p.half; i += blockDim.x) {
         const double f = exp2(-p.log2_theta * i / p.half);   // theta^(-2i/rot)
         const double w = p.orig_turns > 0 ? fmin(fmax((p.orig_turns * f - p.turns_low) * p.inv_span, 0.0), 1.0) : 0.0;
-        s_turns[i] = f * (w + (1.0 - w) * p.inv_factor) * 0.15915494309189533577;   // 1/2pi
+        s_quarters[i] = f * (w + (1.0 - w) * p.inv_factor) * 0.63661977236758134308;   // 2/pi
     }
     __syncthreads();
     const int per_row = p.half / VEC, rows_at_once = 256 / per_row;   // per_row <= 256: rot_dim <= 512
     const int i = threadIdx.x % per_row * VEC;
     if (threadIdx.x / per_row >= rows_at_once) return;
-    double turns[VEC];
+    double quarters[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) turns[v] = s_turns[i + v];
+    for (int v = 0; v < VEC; ++v) quarters[v] = s_quarters[i + v];
     for (int64_t r = (int64_t)blockIdx.x * rows_at_once + threadIdx.x / per_row; r < p.rows;
          r += (int64_t)gridDim.x * rows_at_once) {
         const double pos = p.pos ? p.pos[r] : (int)r;
         float c[VEC], s[VEC];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
-            double t = pos * turns[v];
-            t -= rint(t);
-            sincospif(2.f * (float)t, &s[v], &c[v]);
+            sincos_quarters(pos * quarters[v], s[v], c[v]);
             c[v] *= p.amplitude;
             s[v] *= p.amplitude;
         }
@@ -160,29 +174,65 @@ __global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(NormRopeParams p)
 
 // The same with 16-byte accesses: a lane holds 8 neighbouring values, LANES
 // lanes a head (the power of two that covers head_dim / 8), and a warp works on
-// 32 / LANES heads of one row at a time, kHeadsDeep times, with all of its
-// loads issued before the first sum.  A pair of the half layout lies rot_dim/16
-// lanes apart (a shuffle), one of the interleaved layout in one lane.
+// 32 / LANES heads of one row at a time, kHeadsDeep times, all of queries or all
+// of keys, with every load issued before the first sum.  gamma is folded into the
+// rotation once per warp: out = (x c gamma + partner s gamma') / rms, so a
+// value costs a conversion, its square, two products and its share of the
+// partner's fetch (packed: a pair of the half layout lies rot_dim/16 lanes apart,
+// one of the interleaved layout in the same word).
 constexpr int kHeadsDeep = 4;
 
 template <typename T>
 struct Vec8 {
-    uint4 w[sizeof(T) / 2];
+    static constexpr int kWords = 2 * sizeof(T);
+    uint32_t w[kWords];
     __device__ __forceinline__ void load(const T *p) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4 *>(p)[i];
+        for (int i = 0; i < kWords; i += 4) *reinterpret_cast<uint4 *>(w + i) = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint32_t *>(p) + i);
     }
     __device__ __forceinline__ void get(float (&v)[8]) const {
-        const T *e = reinterpret_cast<const T *>(w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
+            else if constexpr (std::is_same_v<T, __half>) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            } else {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
     }
     __device__ __forceinline__ void put(const float (&v)[8], T *p) {
-        T *e = reinterpret_cast<T *>(w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+            else if constexpr (std::is_same_v<T, __half>) {
+                const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t *>(&h);
+            }
+        }
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(p)[i] = w[i];
+        for (int i = 0; i < kWords; i += 4) *reinterpret_cast<uint4 *>(reinterpret_cast<uint32_t *>(p) + i) = *reinterpret_cast<uint4 *>(w + i);
+    }
+    // the values of the lane `from`, or (interleaved) the neighbours in the pairs
+    __device__ __forceinline__ Vec8 partner(bool interleaved, int from) const {
+        Vec8 o;
+        if (!interleaved) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) o.w[i] = __shfl_sync(0xffffffffu, w[i], from);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                if constexpr (sizeof(T) == 4) o.w[i] = w[i ^ 1];
+                else o.w[i] = (w[i] << 16) | (w[i] >> 16);
+            }
+        }
+        return o;
     }
 };
 
@@ -192,38 +242,44 @@ __device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
 
-template <typename T, int LANES>
+template <typename T, int LANES, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) qk_norm_rope_vec_kernel(NormRopeParams p) {
     constexpr int kSide = 32 / LANES;   // heads side by side in a warp
     const int lane = threadIdx.x & 31, sub = lane / LANES, e0 = lane % LANES * 8;
-    const int all = p.heads + p.kv_heads, per_row = (all + kSide * kHeadsDeep - 1) / (kSide * kHeadsDeep);
-    const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t row64 = item / per_row;
+    const int64_t row64 = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row64 >= p.rows) return;
-    const int row = (int)row64, h0 = (int)(item % per_row) * kSide * kHeadsDeep + sub;
+    const int row = (int)row64;
+    const int q_chunks = (p.heads + kSide * kHeadsDeep - 1) / (kSide * kHeadsDeep);
+    const bool is_q = (int)blockIdx.y < q_chunks;
+    const int heads = is_q ? p.heads : p.kv_heads;
+    const int h0 = ((int)blockIdx.y - (is_q ? 0 : q_chunks)) * kSide * kHeadsDeep + sub;
+    const T *in = static_cast<const T *>(is_q ? p.q : p.k) + (int64_t)row * (is_q ? p.ldq : p.ldk) + h0 * p.d + e0;
+    T *out = static_cast<T *>(is_q ? p.qo : p.ko) + (int64_t)row * (is_q ? p.ldqo : p.ldko) + h0 * p.d + e0;
+    const int step = kSide * p.d;
     const bool in_head = e0 < p.d;
 
     Vec8<T> x[kHeadsDeep];
 #pragma unroll
     for (int u = 0; u < kHeadsDeep; ++u) {
-        const int h = h0 + u * kSide;
-        if (in_head && h < all)
-            x[u].load(h < p.heads ? static_cast<const T *>(p.q) + (int64_t)row * p.ldq + h * p.d + e0
-                                  : static_cast<const T *>(p.k) + (int64_t)row * p.ldk + (h - p.heads) * p.d + e0);
-        else x[u] = Vec8<T>{};
+        x[u] = Vec8<T>{};
+        if (in_head && h0 + u * kSide < heads) x[u].load(in + u * step);
     }
-    // rotation of this lane's 8 values: out = x * c + partner * s
-    const int rot = 2 * p.half;
-    const bool turns = e0 < rot;
-    const int apart = p.half / 8;                                 // half layout: lanes between a pair
-    const bool second = !p.interleaved && turns && e0 >= p.half;
-    float c[8], s[8];
+    // this lane's 8 values: out = x * a + partner * b, gamma included
+    const int rot = 2 * p.half, apart = p.half / 8;   // half layout: lanes between a pair
+    const bool turns = e0 < rot, second = !INTERLEAVED && turns && e0 >= p.half;
+    const int from = (second ? lane - apart : lane + apart) & 31;
+    float a[8], b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = 1.f;
+    const float *g = p.norm ? (is_q ? p.gq : p.gk) : nullptr;
+    if (g && in_head) load8(g + e0, a);
     if (turns) {
+        float c[8];
         const int64_t at = table_row(p, row) * p.half;
-        if (!p.interleaved) {
+        if constexpr (!INTERLEAVED) {
             const int j = second ? e0 - p.half : e0;
             load8(p.cos_t + at + j, c);
-            load8(p.sin_t + at + j, s);
+            load8(p.sin_t + at + j, b);
         } else {
             const float4 c4 = __ldg(reinterpret_cast<const float4 *>(p.cos_t + at + e0 / 2));
             const float4 s4 = __ldg(reinterpret_cast<const float4 *>(p.sin_t + at + e0 / 2));
@@ -231,62 +287,45 @@ __global__ void __launch_bounds__(256) qk_norm_rope_vec_kernel(NormRopeParams p)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 c[i] = cc[i / 2];
-                s[i] = sv[i / 2];
+                b[i] = sv[i / 2];
             }
         }
+        float gp[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (p.interleaved ? !(i & 1) : !second) s[i] = -s[i];
+        for (int i = 0; i < 8; ++i) gp[i] = INTERLEAVED ? a[i ^ 1] : 1.f;
+        if (!INTERLEAVED && g) load8(g + (second ? e0 - p.half : e0 + p.half), gp);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            b[i] *= (INTERLEAVED ? !(i & 1) : !second) ? -gp[i] : gp[i];
+            a[i] *= c[i];
+        }
     }
+    const float inv_d = 1.f / (float)p.d;
 #pragma unroll
     for (int u = 0; u < kHeadsDeep; ++u) {
-        const int h = h0 + u * kSide;
-        const bool is_q = h < p.heads;
-        float v[8];
+        float v[8], w[8], inv = 1.f;
         x[u].get(v);
+        if (rot) x[u].partner(INTERLEAVED, from).get(w);
         if (p.norm) {
             float ss = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss += v[i] * v[i];
+            for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
 #pragma unroll
             for (int o = LANES / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float inv = 1.f / sqrtf(ss / (float)p.d + p.eps);
-            const float *g = is_q ? p.gq : p.gk;
-            if (g && in_head) {
-                float gv[8];
-                load8(g + e0, gv);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= inv * gv[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= inv;
-            }
+            inv = rsqrtf(fmaf(ss, inv_d, p.eps));
         }
-        if (rot) {
-            float w[8];
-            if (!p.interleaved) {
-                const int from = second ? lane - apart : lane + apart;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = __shfl_sync(0xffffffffu, v[i], from & 31);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = v[i ^ 1];
-            }
-            if (turns)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = v[i] * c[i] + w[i] * s[i];
-        }
-        if (in_head && h < all)
-            x[u].put(v, is_q ? static_cast<T *>(p.qo) + (int64_t)row * p.ldqo + h * p.d + e0
-                             : static_cast<T *>(p.ko) + (int64_t)row * p.ldko + (h - p.heads) * p.d + e0);
+        for (int i = 0; i < 8; ++i) v[i] = (turns ? fmaf(w[i], b[i], v[i] * a[i]) : v[i] * a[i]) * inv;
+        if (in_head && h0 + u * kSide < heads) x[u].put(v, out + u * step);
     }
 }
 
 template <typename T, int LANES>
 void launch_vec(const NormRopeParams &p, cudaStream_t st) {
-    const int heads = 32 / LANES * kHeadsDeep;
-    const int64_t items = (int64_t)p.rows * ((p.heads + p.kv_heads + heads - 1) / heads);
-    qk_norm_rope_vec_kernel<T, LANES><<<(unsigned)((items + 7) / 8), 256, 0, st>>>(p);
+    constexpr int kHeads = 32 / LANES * kHeadsDeep;
+    const dim3 grid((unsigned)((p.rows + 7) / 8), (unsigned)((p.heads + kHeads - 1) / kHeads + (p.kv_heads + kHeads - 1) / kHeads));
+    if (p.interleaved) qk_norm_rope_vec_kernel<T, LANES, true><<<grid, 256, 0, st>>>(p);
+    else qk_norm_rope_vec_kernel<T, LANES, false><<<grid, 256, 0, st>>>(p);
 }
 
 template <typename T>
@@ -297,7 +336,8 @@ void launch_norm_rope(const NormRopeParams &p, cudaStream_t st) {
     const uintptr_t bases = (uintptr_t)p.q | (uintptr_t)p.qo | (uintptr_t)p.k | (uintptr_t)p.ko | (uintptr_t)p.gq |
                             (uintptr_t)p.gk | (uintptr_t)p.cos_t | (uintptr_t)p.sin_t;
     const int64_t lds = p.ldq | p.ldqo | p.ldk | p.ldko;
-    if (p.d % 8 == 0 && p.d <= 256 && p.half % (p.interleaved ? 4 : 8) == 0 && !(bases & 15) && lds % kAlign == 0) {
+    if (p.d % 8 == 0 && p.d <= 256 && p.half % (p.interleaved ? 4 : 8) == 0 && !(bases & 15) && lds % kAlign == 0 &&
+        p.heads + (int64_t)p.kv_heads <= 65535) {   // the grid's second dimension
         if (p.d <= 32) launch_vec<T, 4>(p, st);
         else if (p.d <= 64) launch_vec<T, 8>(p, st);
         else if (p.d <= 128) launch_vec<T, 16>(p, st);
