@@ -160,16 +160,17 @@ __device__ __forceinline__ void split_bf16(float v, __nv_bfloat16 &hi, __nv_bflo
 // ranks behind one another in its 128 rows, so a mixed tile reads x once; with
 // few tiles, lanes of CTAs share a tile's adapters instead.
 
+// A stage is x's tile and the ranks in hand (a_bytes of them); the product reads
+// 128 rows from there whatever is behind (rows that nothing reads), so a pad ends
+// the ring.  Small, so that these CTAs share SMs with project_kernel's.
 template <int TN>
 struct LowCfg {
-    static constexpr int A_BYTES = BM * 128, STAGE = A_BYTES + TN * 128;
-    static constexpr int STAGES = TN == 64 ? 4 : 5;   // two CTAs per SM
-    static constexpr int RING = STAGES * STAGE;
-    static constexpr int LIST = RING + 256;
-    static constexpr int BYTES = 1024 + LIST + (int)sizeof(TileList<TN>) + (int)sizeof(ListScratch<TN>);
+    static constexpr int X_BYTES = TN * 128, PAD = BM * 128;
+    static constexpr int STAGES = TN == 64 ? 4 : 5;
+    static int ring(int a_bytes) { return STAGES * (X_BYTES + a_bytes) + PAD; }
+    static int bytes(int a_bytes) { return 1024 + ring(a_bytes) + 256 + (int)sizeof(TileList<TN>) + (int)sizeof(ListScratch<TN>); }
     static constexpr int COLS = TN < 32 ? 32 : TN;
-    static_assert(TN * BM * 4 <= RING, "the f32 partials fit the ring");
-    static_assert(2 * (BYTES + 1024) <= 228 * 1024, "two CTAs share an SM");
+    static_assert(TN * BM * 4 <= STAGES * (X_BYTES + 1024) + PAD, "the f32 partials fit the ring");
 };
 constexpr int kLowThreads = 192;
 
@@ -179,10 +180,12 @@ __global__ void __launch_bounds__(kLowThreads)
     using C = LowCfg<TN>;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::RING), *empty = full + C::STAGES, *done = empty + C::STAGES;
+    const int box = min(p.rank, BM), a_bytes = p.unit * box * 128, stage = C::X_BYTES + a_bytes;   // rank % 8 == 0: whole swizzle blocks
+    unsigned char *behind = smem + C::STAGES * stage + C::PAD;
+    uint64_t *full = reinterpret_cast<uint64_t *>(behind), *empty = full + C::STAGES, *done = empty + C::STAGES;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
-    TileList<TN> &list = *reinterpret_cast<TileList<TN> *>(smem + C::LIST);
-    ListScratch<TN> &scratch = *reinterpret_cast<ListScratch<TN> *>(smem + C::LIST + sizeof(TileList<TN>));
+    TileList<TN> &list = *reinterpret_cast<TileList<TN> *>(behind + 256);
+    ListScratch<TN> &scratch = *reinterpret_cast<ListScratch<TN> *>(behind + 256 + sizeof(TileList<TN>));
     float *part = reinterpret_cast<float *>(smem);   // partial sums in the ring's place
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -212,7 +215,7 @@ __global__ void __launch_bounds__(kLowThreads)
 
     const int kb = (p.k + 63) / 64;
     const int k0 = kb * split / p.splits, k1 = kb * (split + 1) / p.splits;
-    const int m_blocks = (p.rank + BM - 1) / BM, box = min(p.rank, BM);   // unit is 1 where m_blocks is not
+    const int m_blocks = (p.rank + BM - 1) / BM;   // unit is 1 where m_blocks is not
     const int units = (list.count + p.unit - 1) / p.unit * m_blocks;
     uint32_t it = 0, turn = 0;
     for (int u = job % p.tile_lanes; u < units; u += p.tile_lanes, ++turn) {
@@ -228,9 +231,9 @@ __global__ void __launch_bounds__(kLowThreads)
                     if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, p.flag, 401, &aborted)) break;
                     mbar_arrive_expect_tx(&full[s], n_here * box * 128 + TN * 128);
                     for (int i = 0; i < n_here; ++i)
-                        tma_load_2d(smem + s * C::STAGE + i * box * 128, &tmA, &full[s], kk * 64,
+                        tma_load_2d(smem + s * stage + C::X_BYTES + i * box * 128, &tmA, &full[s], kk * 64,
                                     list.ids[first + i] * p.rank + r0);
-                    tma_load_2d(smem + s * C::STAGE + C::A_BYTES, &tmX, &full[s], kk * 64, m0);
+                    tma_load_2d(smem + s * stage, &tmX, &full[s], kk * 64, m0);
                 }
         } else if (warp == 1) {
             if (elect_one()) {
@@ -239,7 +242,7 @@ __global__ void __launch_bounds__(kLowThreads)
                     const int s = it % C::STAGES;
                     if (!mbar_wait(&full[s], (it / C::STAGES) & 1, p.flag, 402, &aborted)) break;
                     tc_fence_after();
-                    const uint32_t ad = smem_u32(smem + s * C::STAGE), bd = ad + C::A_BYTES;
+                    const uint32_t bd = smem_u32(smem + s * stage), ad = bd + C::X_BYTES;
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
                         umma_f16_ss(tmem, sdesc_sw128(ad + q * 32, 16, 1024), sdesc_sw128(bd + q * 32, 16, 1024), idesc,
@@ -322,8 +325,10 @@ __global__ void __launch_bounds__(kLowThreads)
 template <int TN>
 struct ProjCfg {
     static constexpr int A_BYTES = BM * 128, B_BYTES = TN * 128, STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = TN == 256 ? 4 : TN == 128 ? 6 : TN == 64 ? 8 : 10;
-    static constexpr int BUFS = TN == 256 ? 1 : TN == 128 ? 2 : 4;   // rows of low
+    // up to 128 tokens: as deep as HBM's latency asks (96 KB and more), and no
+    // deeper, so that low_kernel's CTAs run beside these
+    static constexpr int STAGES = TN == 256 ? 4 : TN == 128 ? 3 : TN == 64 ? 4 : TN == 32 ? 6 : 7;
+    static constexpr int BUFS = TN == 256 ? 1 : TN <= 32 ? 4 : 2;   // rows of low
     static constexpr int RING = STAGES * STAGE, BUF = RING, BAR = BUF + BUFS * B_BYTES;
     static constexpr int LIST = BAR + ((2 * STAGES + 8 + 2 * BUFS) * 8 + 8 + 15) / 16 * 16;
     static constexpr int BYTES = 1024 + LIST + 2 * (int)sizeof(TileList<TN>) + (int)sizeof(ListScratch<TN>);
@@ -342,17 +347,15 @@ __device__ __forceinline__ void tile_at(const AdapterParams &p, int t, int &mt, 
     nt = r / gm;
 }
 
-// One tile's blocks in order: `nk` of the main product, `na` of the adapters'
-// spread evenly among them (so that a builder has time for each) or, where
-// low_kernel still runs while the weights stream, behind them.
+// One tile's blocks in order: `nk` of the main product with `na` of the adapters'
+// spread evenly among them, so that the builder has time for each.
 template <typename F, typename G>
-__device__ __forceinline__ void blocks_in_order(int nk, int na, bool behind, F main_block, G adapter_block) {
-    auto place = [&](int i) { return behind ? nk : (i + 1) * nk / (na + 1); };   // block i comes before main block place(i)
-    int i = 0, next = na > 0 ? place(0) : nk + 1;
+__device__ __forceinline__ void blocks_in_order(int nk, int na, F main_block, G adapter_block) {
+    int i = 0, next = na > 0 ? nk / (na + 1) : nk + 1;   // adapter block i comes before main block `next`
     for (int k = 0; k <= nk; ++k) {
         while (next == k) {
             if (!adapter_block(i)) return;
-            next = ++i < na ? place(i) : nk + 1;
+            next = ++i < na ? (i + 1) * nk / (na + 1) : nk + 1;
         }
         if (k < nk && !main_block(k)) return;
     }
@@ -431,9 +434,20 @@ __global__ void __launch_bounds__(kProjThreads, 1)
         a0 = all * split / p.splits;
         na = all * (split + 1) / p.splits - a0;
     };
+    // A cluster's one tile: the weights start to stream before anything else, and
+    // the adapters' blocks follow them.
     const bool behind = p.splits > 1;
+    int mt0, nt0;
+    tile_at(p, first, mt0, nt0);
+    uint32_t it = 0;   // ring uses of the producer or the MMA thread
+    auto load_main = [&](int k, int mt, int nt, int s) {
+        tma_load_2d(smem + s * C::STAGE, &tmW, &full[s], (k0 + k) * 64, nt * BM);
+        tma_load_2d(smem + s * C::STAGE + C::A_BYTES, &tmX, &full[s], (k0 + k) * 64, mt * TN);
+    };
 
     if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tmW);
+        tma_prefetch_desc(&tmX);
         for (int s = 0; s < C::STAGES; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
@@ -449,8 +463,17 @@ __global__ void __launch_bounds__(kProjThreads, 1)
             mbar_init(&bempty[i], 1);
         }
         fence_barrier_init();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // for the loads of this very thread
+        if (behind)
+            for (; it < (uint32_t)min(nk, C::STAGES); ++it) {
+                mbar_arrive_expect_tx(&full[it], C::STAGE);
+                load_main(it, mt0, nt0, it);
+            }
     }
-    if (warp == 0) {
+    float bias0 = 0.f;   // the cluster's epilogue: fetched now
+    if (behind && warp >= 2 && warp < 6 && p.bias && nt0 * BM + (warp & 3) * 32 + lane < p.n)
+        bias0 = __ldg(p.bias + nt0 * BM + (warp & 3) * 32 + lane);
+    if (warp == 1) {
         tmem_alloc(tmem_slot, C::COLS);
         tmem_relinquish();
     }
@@ -461,18 +484,13 @@ __global__ void __launch_bounds__(kProjThreads, 1)
     bool aborted = false;
 
     if (warp == 0) {
-        if (elect_one()) {
-            tma_prefetch_desc(&tmW);
-            tma_prefetch_desc(&tmX);
+        if (lane == 0) {
             if (p.adapters) tma_prefetch_desc(&tmB);
-            uint32_t it = 0, i = 0;
+            uint32_t i = 0;
             for (int t = first; t < tiles && !aborted; t += stride, ++i) {
                 int mt, nt;
                 tile_at(p, t, mt, nt);
                 const TileList<TN> &list = lists[i & 1];
-                if (!mbar_wait(&lfull[i & 1], (i >> 1) & 1, p.flag, 411, &aborted)) break;
-                int a0, na;
-                share(list.count, a0, na);
                 auto take = [&](uint32_t bytes) {
                     const int s = it % C::STAGES;
                     if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, p.flag, 412, &aborted)) return -1;
@@ -480,22 +498,26 @@ __global__ void __launch_bounds__(kProjThreads, 1)
                     ++it;
                     return s;
                 };
-                blocks_in_order(
-                    nk, na, behind,
-                    [&](int k) {
-                        const int s = take(C::STAGE);
-                        if (s < 0) return false;
-                        tma_load_2d(smem + s * C::STAGE, &tmW, &full[s], (k0 + k) * 64, nt * BM);
-                        tma_load_2d(smem + s * C::STAGE + C::A_BYTES, &tmX, &full[s], (k0 + k) * 64, mt * TN);
-                        return true;
-                    },
-                    [&](int b) {
-                        const int s = take(C::A_BYTES);
-                        if (s < 0) return false;
-                        const int e = a0 + b, rb = e % per_adapter / p.parts;
-                        tma_load_2d(smem + s * C::STAGE, &tmB, &full[s], rb * 64, list.ids[e / per_adapter] * p.n + nt * BM);
-                        return true;
-                    });
+                auto main_block = [&](int k) {
+                    const int s = take(C::STAGE);
+                    if (s < 0) return false;
+                    load_main(k, mt, nt, s);
+                    return true;
+                };
+                int a0, na;
+                auto adapter_block = [&](int b) {
+                    const int s = take(C::A_BYTES);
+                    if (s < 0) return false;
+                    const int e = a0 + b, rb = e % per_adapter / p.parts;
+                    tma_load_2d(smem + s * C::STAGE, &tmB, &full[s], rb * 64, list.ids[e / per_adapter] * p.n + nt * BM);
+                    return true;
+                };
+                if (behind)
+                    for (int k = it; k < nk; ++k)
+                        if (!main_block(k)) break;
+                if (aborted || !mbar_wait(&lfull[i & 1], (i >> 1) & 1, p.flag, 411, &aborted)) break;
+                share(list.count, a0, na);
+                blocks_in_order(behind ? 0 : nk, na, main_block, adapter_block);
                 mbar_arrive(&lempty[i & 1]);
             }
             if (aborted) {   // let the copies already issued land before the CTA exits
@@ -507,12 +529,9 @@ __global__ void __launch_bounds__(kProjThreads, 1)
     } else if (warp == 1) {
         if (elect_one()) {
             constexpr uint32_t idesc = idesc_f16(BM, TN, true);
-            uint32_t it = 0, i = 0, built = 0;
+            uint32_t i = 0, built = 0;
             for (int t = first; t < tiles && !aborted; t += stride, ++i) {
                 const uint32_t acc = i & 1;
-                if (!mbar_wait(&lfull[acc], (i >> 1) & 1, p.flag, 413, &aborted)) break;
-                int a0, na;
-                share(lists[acc].count, a0, na);
                 if (!mbar_wait(&tempty[acc], ((i >> 1) & 1) ^ 1, p.flag, 414, &aborted)) break;
                 tc_fence_after();
                 const uint32_t d = tmem + acc * C::ACC;
@@ -530,25 +549,30 @@ __global__ void __launch_bounds__(kProjThreads, 1)
                     umma_commit(&empty[s]);
                     ++it;
                 };
-                blocks_in_order(
-                    nk, na, behind,
-                    [&](int) {
-                        if (!mbar_wait(&full[it % C::STAGES], (it / C::STAGES) & 1, p.flag, 415, &aborted)) return false;
-                        tc_fence_after();
-                        multiply(0);
-                        return true;
-                    },
-                    [&](int) {
-                        const int b = built % C::BUFS;
-                        if (!mbar_wait(&full[it % C::STAGES], (it / C::STAGES) & 1, p.flag, 416, &aborted) ||
-                            !mbar_wait(&bfull[b], (built / C::BUFS) & 1, p.flag, 417, &aborted))
-                            return false;
-                        tc_fence_after();
-                        multiply(smem_u32(smem + C::BUF + b * C::B_BYTES));
-                        umma_commit(&bempty[b]);
-                        ++built;
-                        return true;
-                    });
+                auto main_block = [&](int) {
+                    if (!mbar_wait(&full[it % C::STAGES], (it / C::STAGES) & 1, p.flag, 415, &aborted)) return false;
+                    tc_fence_after();
+                    multiply(0);
+                    return true;
+                };
+                auto adapter_block = [&](int) {
+                    const int b = built % C::BUFS;
+                    if (!mbar_wait(&full[it % C::STAGES], (it / C::STAGES) & 1, p.flag, 416, &aborted) ||
+                        !mbar_wait(&bfull[b], (built / C::BUFS) & 1, p.flag, 417, &aborted))
+                        return false;
+                    tc_fence_after();
+                    multiply(smem_u32(smem + C::BUF + b * C::B_BYTES));
+                    umma_commit(&bempty[b]);
+                    ++built;
+                    return true;
+                };
+                if (behind)
+                    for (int k = 0; k < nk; ++k)
+                        if (!main_block(k)) break;
+                if (aborted || !mbar_wait(&lfull[acc], (i >> 1) & 1, p.flag, 413, &aborted)) break;
+                int a0, na;
+                share(lists[acc].count, a0, na);
+                blocks_in_order(behind ? 0 : nk, na, main_block, adapter_block);
                 if (aborted) break;
                 mbar_arrive(&lempty[acc]);
                 umma_commit(&tfull[acc]);
@@ -662,9 +686,7 @@ __global__ void __launch_bounds__(kProjThreads, 1)
     }
 
     if (p.splits > 1) {   // one tile per cluster; all its loads have been read
-        const int row = (warp & 3) * 32 + lane, per = TN / p.splits;
-        int mt, nt;
-        tile_at(p, first, mt, nt);
+        const int row = (warp & 3) * 32 + lane, per = TN / p.splits, mt = mt0, nt = nt0;
         cluster_sync();   // the partials take the ring's place in every CTA
         if (warp >= 2 && warp < 6 && !aborted)
             send_partials<TN>(tmem + ((uint32_t)((warp & 3) * 32) << 16), row, part, p.splits, split,
@@ -672,7 +694,6 @@ __global__ void __launch_bounds__(kProjThreads, 1)
         cluster_sync();
         if (warp >= 2 && warp < 6 && !aborted) {
             const int n = nt * BM + row;
-            const float bias = p.bias && n < p.n ? p.bias[n] : 0.f;
             for (int j0 = 0; j0 < per; j0 += 16) {
                 const int m = mt * TN + split * per + j0, count = min(per - j0, p.m - m);
                 if (count <= 0) break;
@@ -685,13 +706,13 @@ __global__ void __launch_bounds__(kProjThreads, 1)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[q + j] = half[j];
                 }
-                finish16<EPI>(p, m, count, n, bias, v, h);
+                finish16<EPI>(p, m, count, n, bias0, v, h);
             }
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) {
+    if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, C::COLS);
     }
@@ -765,7 +786,7 @@ cudaError_t run_low(AdapterParams p, const CUtensorMap &ta, const CUtensorMap &t
     const int blocks = (p.rank + BM - 1) / BM, most = std::min({p.adapters, TN, p.m});
     p.tile_lanes = std::max(1, std::min(room / (tiles * p.splits), most * blocks));
     p.unit = blocks > 1 ? 1 : std::min(BM / p.rank, (most + p.tile_lanes - 1) / p.tile_lanes);
-    return launch(low_kernel<TN>, tiles * p.tile_lanes * p.splits, kLowThreads, LowCfg<TN>::BYTES, p.splits, false, st, ta, tx, p);
+    return launch(low_kernel<TN>, tiles * p.tile_lanes * p.splits, kLowThreads, LowCfg<TN>::bytes(p.unit * std::min(p.rank, BM) * 128), p.splits, false, st, ta, tx, p);
 }
 
 template <int TN>
