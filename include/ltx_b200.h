@@ -330,11 +330,17 @@ int ltx_rope_table(ltx_ctx *ctx, const int32_t *pos_dev, int32_t rows, int32_t r
  * the next ltx_ctx_synchronize.  rot_dim 0 (cos/sin NULL) rotates nothing.  k
  * may be NULL with kv_heads 0.  An output may be its input (same pointer and
  * leading dimension); otherwise it may not overlap one.  head_dim 1..512. */
-int ltx_qk_norm_rope(ltx_ctx *ctx, int32_t dtype, const void *q_dev, int64_t ldq, const void *k_dev, int64_t ldk,
-                     void *q_out_dev, int64_t ldqo, void *k_out_dev, int64_t ldko, int32_t rows, int32_t heads,
-                     int32_t kv_heads, int32_t head_dim, int32_t norm, float eps, const float *gamma_q_dev,
-                     const float *gamma_k_dev, const float *cos_dev, const float *sin_dev, int32_t table_rows,
-                     int32_t rot_dim, int32_t layout, const int32_t *pos_dev);
+typedef struct {
+    const void *q_dev, *k_dev;                            /* [rows, heads * head_dim], [rows, kv_heads * head_dim]      */
+    void *q_out_dev, *k_out_dev;
+    const float *gamma_q_dev, *gamma_k_dev;               /* [head_dim] or NULL                                          */
+    const float *cos_dev, *sin_dev;                       /* [table_rows, rot_dim/2]                                     */
+    const int32_t *pos_dev;                               /* [rows] or NULL                                              */
+    int64_t ldq, ldk, ldqo, ldko;
+    int32_t dtype, rows, heads, kv_heads, head_dim, norm, table_rows, rot_dim, layout;
+    float eps;
+} ltx_norm_rope;
+int ltx_qk_norm_rope(ltx_ctx *ctx, const ltx_norm_rope *args);
 
 /* out = epilogue(x[m,k] . W[n,k]^T + low) with low[r] = coeff[a] (x[r] . A_a^T) . B_a^T,
  * a = adapter_idx[r]: the projection of ltx_gemm_bf16 with every row's own
@@ -354,11 +360,17 @@ int ltx_qk_norm_rope(ltx_ctx *ctx, int32_t dtype, const void *q_dev, int64_t ldq
  * from the context's pool in stream order. */
 #define LTX_MAX_ADAPTERS 2048
 #define LTX_MAX_ADAPTER_RANK 256
-int ltx_gemm_adapters(ltx_ctx *ctx, const void *x_dev, int64_t ldx, const void *w_dev, int64_t ldw, int32_t m,
-                      int32_t n, int32_t k, int32_t epilogue, const float *bias_dev, void *out_dev, int64_t ldo,
-                      const float *gate_dev, const int32_t *gate_idx_dev, int64_t ld_gate,
-                      const int32_t *adapter_idx_dev, const void *lora_a_dev, const void *lora_b_dev,
-                      const float *coeff_dev, int32_t adapters, int32_t rank);
+typedef struct {
+    const void *x_dev, *w_dev;                            /* bf16 [m, k], [n, k]                                         */
+    void *out_dev;                                        /* [m, n], as the epilogue says                                */
+    const float *bias_dev, *gate_dev;                     /* as ltx_gemm_bf16, or NULL                                   */
+    const int32_t *gate_idx_dev, *adapter_idx_dev;        /* [m]                                                         */
+    const void *lora_a_dev, *lora_b_dev;
+    const float *coeff_dev;
+    int64_t ldx, ldw, ldo, ld_gate;
+    int32_t m, n, k, epilogue, adapters, rank;
+} ltx_adapter_gemm;
+int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args);
 
 /* out = softmax(s) v per head over packed documents: document i is rows
  * [q_offsets[i], q_offsets[i+1]) of q and out and [k_offsets[i],
@@ -379,11 +391,16 @@ int ltx_gemm_adapters(ltx_ctx *ctx, const void *x_dev, int64_t ldx, const void *
  * or 128; out overlaps no input.  What k and v hold outside the documents, or
  * in other documents, never reaches a row, NaN and infinities included; a
  * non-finite v row inside a document may reach every row of the document. */
-int ltx_attention_packed_fwd(ltx_ctx *ctx, const void *q_dev, int64_t ldq, const void *k_dev, int64_t ldk,
-                             const void *v_dev, int64_t ldv, int32_t v_dtype, const int32_t *q_offsets_dev,
-                             const int32_t *k_offsets_dev, int32_t docs, int32_t rows_q, int32_t rows_k, int32_t heads,
-                             int32_t kv_heads, int32_t head_dim, float scale, float softcap, const float *slopes_dev,
-                             int32_t causal, const int32_t *prefix_dev, void *out_dev, int64_t ldo);
+typedef struct {
+    const void *q_dev, *k_dev, *v_dev;
+    void *out_dev;
+    const int32_t *q_offsets_dev, *k_offsets_dev, *prefix_dev;
+    const float *slopes_dev;
+    int64_t ldq, ldk, ldv, ldo;
+    int32_t v_dtype, docs, rows_q, rows_k, heads, kv_heads, head_dim, causal;
+    float scale, softcap;
+} ltx_packed_attention;
+int ltx_attention_packed_fwd(ltx_ctx *ctx, const ltx_packed_attention *args);
 
 /* ── ltx-weights: the weight store ─────────────────────────────────────────── */
 

@@ -828,14 +828,13 @@ int tokens_for(int m) {
 
 }  // namespace ltx
 
-extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const void *x_dev, int64_t ldx, const void *w_dev, int64_t ldw, int32_t m,
-                                 int32_t n, int32_t k, int32_t epilogue, const float *bias_dev, void *out_dev,
-                                 int64_t ldo, const float *gate_dev, const int32_t *gate_idx_dev, int64_t ld_gate,
-                                 const int32_t *adapter_idx_dev, const void *lora_a_dev, const void *lora_b_dev,
-                                 const float *coeff_dev, int32_t adapters, int32_t rank) {
+extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args) {
     using namespace ltx;
     if (!ctx) return LTX_ERR_INVALID_ARG;
     const char *w = "gemm_adapters";
+    if (!args) return fail(ctx, LTX_ERR_INVALID_ARG, "%s: null arguments", w);
+    const auto &[x_dev, w_dev, out_dev, bias_dev, gate_dev, gate_idx_dev, adapter_idx_dev, lora_a_dev, lora_b_dev, coeff_dev,
+                 ldx, ldw, ldo, ld_gate, m, n, k, epilogue, adapters, rank] = *args;
     if (epilogue < LTX_EPI_BF16 || epilogue > LTX_EPI_RESID)
         return fail(ctx, LTX_ERR_INVALID_ARG, "%s: bad epilogue %d", w, epilogue);
     if (m < 0 || n < 1 || k < 1 || k > 1 << 24) return fail(ctx, LTX_ERR_SHAPE, "%s: %d x %d x %d", w, m, n, k);

@@ -824,15 +824,13 @@ bool packed_map(CUtensorMap *m, const void *ptr, int64_t rows, int heads, int d,
 
 }  // namespace ltx
 
-extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const void *q_dev, int64_t ldq, const void *k_dev, int64_t ldk,
-                                        const void *v_dev, int64_t ldv, int32_t v_dtype, const int32_t *q_offsets_dev,
-                                        const int32_t *k_offsets_dev, int32_t docs, int32_t rows_q, int32_t rows_k,
-                                        int32_t heads, int32_t kv_heads, int32_t head_dim, float scale, float softcap,
-                                        const float *slopes_dev, int32_t causal, const int32_t *prefix_dev,
-                                        void *out_dev, int64_t ldo) {
+extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const ltx_packed_attention *args) {
     using namespace ltx;
     if (!ctx) return LTX_ERR_INVALID_ARG;
     const char *w = "attention_packed";
+    if (!args) return fail(ctx, LTX_ERR_INVALID_ARG, "%s: null arguments", w);
+    const auto &[q_dev, k_dev, v_dev, out_dev, q_offsets_dev, k_offsets_dev, prefix_dev, slopes_dev, ldq, ldk, ldv, ldo, v_dtype,
+                 docs, rows_q, rows_k, heads, kv_heads, head_dim, causal, scale, softcap] = *args;
     if (v_dtype != LTX_BF16 && v_dtype != LTX_F16) return fail(ctx, LTX_ERR_DTYPE, "%s: V must be BF16 or F16", w);
     if (head_dim != 64 && head_dim != 128)
         return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", w, head_dim);

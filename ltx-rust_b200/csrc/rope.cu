@@ -379,14 +379,12 @@ extern "C" int ltx_rope_table(ltx_ctx *ctx, const int32_t *pos_dev, int32_t rows
     return e == cudaSuccess ? LTX_OK : cuda_fail(ctx, e, "rope_table launch");
 }
 
-extern "C" int ltx_qk_norm_rope(ltx_ctx *ctx, int32_t dtype, const void *q_dev, int64_t ldq, const void *k_dev,
-                                int64_t ldk, void *q_out_dev, int64_t ldqo, void *k_out_dev, int64_t ldko, int32_t rows,
-                                int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t norm, float eps,
-                                const float *gamma_q_dev, const float *gamma_k_dev, const float *cos_dev,
-                                const float *sin_dev, int32_t table_rows, int32_t rot_dim, int32_t layout,
-                                const int32_t *pos_dev) {
+extern "C" int ltx_qk_norm_rope(ltx_ctx *ctx, const ltx_norm_rope *args) {
     using namespace ltx;
     if (!ctx) return LTX_ERR_INVALID_ARG;
+    if (!args) return fail(ctx, LTX_ERR_INVALID_ARG, "qk_norm_rope: null arguments");
+    const auto &[q_dev, k_dev, q_out_dev, k_out_dev, gamma_q_dev, gamma_k_dev, cos_dev, sin_dev, pos_dev, ldq, ldk, ldqo, ldko,
+                 dtype, rows, heads, kv_heads, head_dim, norm, table_rows, rot_dim, layout, eps] = *args;
     if (dtype != LTX_BF16 && dtype != LTX_F16 && dtype != LTX_F32)
         return fail(ctx, LTX_ERR_DTYPE, "qk_norm_rope: dtype %d (BF16, F16 or F32)", dtype);
     if (rows < 0 || heads < 0 || kv_heads < 0 || head_dim < 1 || head_dim > kMaxHeadDim)
