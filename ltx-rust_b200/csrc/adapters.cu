@@ -750,15 +750,17 @@ bool make_map(CUtensorMap *m, const void *ptr, int64_t rows, int64_t cols, int64
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// `most`: the largest dynamic shared memory any call of the kernel asks for.
 template <typename K, typename... Args>
-cudaError_t launch(K kern, int grid, int threads, int smem, int cluster, bool dependent, cudaStream_t st, const Args &...args) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+cudaError_t launch(const ltx_ctx *ctx, K kern, int grid, int threads, int smem, int most, int cluster, bool dependent,
+                   const Args &...args) {
+    cudaError_t e = allow_smem(ctx, reinterpret_cast<const void *>(kern), most);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
+    cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster;
@@ -779,19 +781,21 @@ int splits_for(int64_t jobs, int room, int kb) {
 }
 
 template <int TN>
-cudaError_t run_low(AdapterParams p, const CUtensorMap &ta, const CUtensorMap &tx, int sms, cudaStream_t st) {
-    const int tiles = (p.m + TN - 1) / TN, room = 2 * sms;
+cudaError_t run_low(const ltx_ctx *ctx, AdapterParams p, const CUtensorMap &ta, const CUtensorMap &tx) {
+    const int tiles = (p.m + TN - 1) / TN, room = 2 * ctx->sm_count;
     p.splits = splits_for(tiles, room, (p.k + 63) / 64);
     // the SMs left over share the adapters of a tile; what one takes goes together
     const int blocks = (p.rank + BM - 1) / BM, most = std::min({p.adapters, TN, p.m});
     p.tile_lanes = std::max(1, std::min(room / (tiles * p.splits), most * blocks));
     p.unit = blocks > 1 ? 1 : std::min(BM / p.rank, (most + p.tile_lanes - 1) / p.tile_lanes);
-    return launch(low_kernel<TN>, tiles * p.tile_lanes * p.splits, kLowThreads, LowCfg<TN>::bytes(p.unit * std::min(p.rank, BM) * 128), p.splits, false, st, ta, tx, p);
+    return launch(ctx, low_kernel<TN>, tiles * p.tile_lanes * p.splits, kLowThreads,
+                  LowCfg<TN>::bytes(p.unit * std::min(p.rank, BM) * 128), LowCfg<TN>::bytes(BM * 128), p.splits, false, ta, tx, p);
 }
 
 template <int TN>
-cudaError_t run_project(AdapterParams p, int epilogue, const CUtensorMap &tw, const CUtensorMap &tx, const CUtensorMap &tb,
-                        int sms, cudaStream_t st) {
+cudaError_t run_project(const ltx_ctx *ctx, AdapterParams p, int epilogue, const CUtensorMap &tw, const CUtensorMap &tx,
+                        const CUtensorMap &tb) {
+    const int sms = ctx->sm_count;
     p.m_tiles = (p.m + TN - 1) / TN;
     p.n_tiles = (p.n + BM - 1) / BM;
     const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
@@ -805,7 +809,7 @@ cudaError_t run_project(AdapterParams p, int epilogue, const CUtensorMap &tw, co
                     : (int)std::max<int64_t>(1, std::min<int64_t>(p.m_tiles, kPanel / ((int64_t)TN * p.k * 2)));
     const int grid = p.splits > 1 ? (int)tiles * p.splits : (int)std::min<int64_t>(tiles, sms);
     auto go = [&](auto kern) {
-        return launch(kern, grid, kProjThreads, ProjCfg<TN>::BYTES, p.splits, p.adapters > 0, st, tw, tx, tb, p);
+        return launch(ctx, kern, grid, kProjThreads, ProjCfg<TN>::BYTES, ProjCfg<TN>::BYTES, p.splits, p.adapters > 0, tw, tx, tb, p);
     };
     switch (epilogue) {
     case LTX_EPI_BF16: return go(project_kernel<TN, LTX_EPI_BF16>);
@@ -885,16 +889,16 @@ extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args) {
         const int rc = work_alloc(ctx, (size_t)p.parts * m * p.rank_blocks * 128, &low);
         if (rc != LTX_OK) return rc;
         p.low = static_cast<__nv_bfloat16 *>(low);
-        e = tl == 16   ? run_low<16>(p, ta, txl, ctx->sm_count, ctx->stream)
-            : tl == 32 ? run_low<32>(p, ta, txl, ctx->sm_count, ctx->stream)
-                       : run_low<64>(p, ta, txl, ctx->sm_count, ctx->stream);
+        e = tl == 16   ? run_low<16>(ctx, p, ta, txl)
+            : tl == 32 ? run_low<32>(ctx, p, ta, txl)
+                       : run_low<64>(ctx, p, ta, txl);
     }
     if (e == cudaSuccess)
-        e = tn == 16    ? run_project<16>(p, epilogue, tw, tx, tb, ctx->sm_count, ctx->stream)
-            : tn == 32  ? run_project<32>(p, epilogue, tw, tx, tb, ctx->sm_count, ctx->stream)
-            : tn == 64  ? run_project<64>(p, epilogue, tw, tx, tb, ctx->sm_count, ctx->stream)
-            : tn == 128 ? run_project<128>(p, epilogue, tw, tx, tb, ctx->sm_count, ctx->stream)
-                        : run_project<256>(p, epilogue, tw, tx, tb, ctx->sm_count, ctx->stream);
+        e = tn == 16    ? run_project<16>(ctx, p, epilogue, tw, tx, tb)
+            : tn == 32  ? run_project<32>(ctx, p, epilogue, tw, tx, tb)
+            : tn == 64  ? run_project<64>(ctx, p, epilogue, tw, tx, tb)
+            : tn == 128 ? run_project<128>(ctx, p, epilogue, tw, tx, tb)
+                        : run_project<256>(ctx, p, epilogue, tw, tx, tb);
     const int rc = work_free(ctx, low);
     return e == cudaSuccess ? rc : cuda_fail(ctx, e, w);
 }

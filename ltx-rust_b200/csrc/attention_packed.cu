@@ -766,21 +766,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <int D>
-cudaError_t launch_packed(bool f16, Mode mode, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
-                          const PackedParams &p, cudaStream_t st) {
+cudaError_t launch_packed(const ltx_ctx *ctx, bool f16, Mode mode, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
+                          const PackedParams &p) {
     auto kern = f16 ? (mode == kCap    ? packed_kernel<D, true, kCap>
                        : mode == kBias ? packed_kernel<D, true, kBias>
                                        : packed_kernel<D, true, kPlain>)
                     : (mode == kCap    ? packed_kernel<D, false, kCap>
                        : mode == kBias ? packed_kernel<D, false, kBias>
                                        : packed_kernel<D, false, kPlain>);
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::BYTES);
+    cudaError_t e = allow_smem(ctx, reinterpret_cast<const void *>(kern), Smem<D>::BYTES);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)((int64_t)p.pairs * p.kv_heads * p.splits));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = Smem<D>::BYTES;
-    cfg.stream = st;
+    cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = p.splits;
@@ -877,7 +877,7 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const ltx_packed_attention
     while (p.splits < 8 && items * p.splits * 2 <= ctx->sm_count && (int64_t)p.splits * 4 * BKV <= rows_k) p.splits *= 2;
     p.pairs = (int)pairs;
     const Mode mode = softcap > 0.f ? kCap : slopes_dev ? kBias : kPlain;
-    const cudaError_t e = head_dim == 64 ? launch_packed<64>(v_dtype == LTX_F16, mode, tq, tk, tv, p, ctx->stream)
-                                         : launch_packed<128>(v_dtype == LTX_F16, mode, tq, tk, tv, p, ctx->stream);
+    const cudaError_t e = head_dim == 64 ? launch_packed<64>(ctx, v_dtype == LTX_F16, mode, tq, tk, tv, p)
+                                         : launch_packed<128>(ctx, v_dtype == LTX_F16, mode, tq, tk, tv, p);
     return e == cudaSuccess ? LTX_OK : cuda_fail(ctx, e, w);
 }

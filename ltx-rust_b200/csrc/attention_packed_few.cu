@@ -596,7 +596,7 @@ int run_few(ltx_ctx *ctx, const CUtensorMap &tq, const CUtensorMap &tk, const CU
     if (rc != LTX_OK) return rc;
     const Partials part{static_cast<float *>(work), reinterpret_cast<float2 *>(static_cast<char *>(work) + o_bytes)};
     auto kern = v_f16 ? few_kernel<D, true, N> : few_kernel<D, false, N>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, FewSmem<D, N>::BYTES);
+    cudaError_t e = allow_smem(ctx, reinterpret_cast<const void *>(kern), FewSmem<D, N>::BYTES);
     if (e == cudaSuccess) {
         kern<<<ctas, kFewThreads, FewSmem<D, N>::BYTES, ctx->stream>>>(tq, tk, tv, p, part);
         e = cudaGetLastError();

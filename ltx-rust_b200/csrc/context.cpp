@@ -2,6 +2,8 @@
 #include <algorithm>
 #include <cstring>
 #include <new>
+#include <set>
+#include <utility>
 
 #include "internal.hpp"
 #include "kernels.hpp"
@@ -22,28 +24,59 @@ int ensure_scratch(ltx_ctx *ctx, size_t bytes) {
     return LTX_OK;
 }
 
+// Workspaces up to this size stay with the context between eager calls.
+constexpr size_t kKeptWorkBytes = 64u << 20;
+
 int work_alloc(ltx_ctx *ctx, size_t bytes, void **out) {
     *out = nullptr;
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    LTX_CUDA_TRY(ctx, cudaStreamIsCapturing(ctx->stream, &capturing));
+    const bool keep = capturing == cudaStreamCaptureStatusNone && bytes <= kKeptWorkBytes;
+    if (keep && ctx->kept_bytes >= bytes) {
+        *out = ctx->kept;
+        return LTX_OK;
+    }
     if (!ctx->pool) {
         cudaMemPoolProps props{};
         props.allocType = cudaMemAllocationTypePinned;
         props.location.type = cudaMemLocationTypeDevice;
         props.location.id = ctx->device;
         LTX_CUDA_TRY(ctx, cudaMemPoolCreate(&ctx->pool, &props));
-        uint64_t keep = ~0ull;   // freed blocks stay in the pool for the next call
-        LTX_CUDA_TRY(ctx, cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &keep));
+        uint64_t hold = ~0ull;   // freed blocks stay in the pool for the next call
+        LTX_CUDA_TRY(ctx, cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &hold));
+    }
+    if (keep && ctx->kept) {   // behind the calls that use it
+        void *old = ctx->kept;
+        ctx->kept = nullptr;
+        ctx->kept_bytes = 0;
+        LTX_CUDA_TRY(ctx, cudaFreeAsync(old, ctx->stream));
     }
     const cudaError_t e = cudaMallocFromPoolAsync(out, bytes, ctx->pool, ctx->stream);
     if (e == cudaErrorMemoryAllocation) {
         cudaGetLastError();   // reported here, not by the next launch check
         return fail(ctx, LTX_ERR_OOM, "workspace of %zu bytes: %s", bytes, cudaGetErrorString(e));
     }
-    return e == cudaSuccess ? LTX_OK : cuda_fail(ctx, e, "workspace");
+    if (e != cudaSuccess) return cuda_fail(ctx, e, "workspace");
+    if (keep) {
+        ctx->kept = *out;
+        ctx->kept_bytes = bytes;
+    }
+    return LTX_OK;
 }
 
 int work_free(ltx_ctx *ctx, void *p) {
-    if (p) LTX_CUDA_TRY(ctx, cudaFreeAsync(p, ctx->stream));
+    if (p && p != ctx->kept) LTX_CUDA_TRY(ctx, cudaFreeAsync(p, ctx->stream));
     return LTX_OK;
+}
+
+cudaError_t allow_smem(const ltx_ctx *ctx, const void *kernel, int bytes) {
+    static std::mutex lock;
+    static std::set<std::pair<const void *, int>> done;
+    const std::lock_guard<std::mutex> hold(lock);
+    if (done.count({kernel, ctx->device})) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.insert({kernel, ctx->device});
+    return e;
 }
 
 int upload(ltx_ctx *ctx, void *dst_dev, const void *src_host, size_t bytes) {
@@ -99,7 +132,11 @@ extern "C" void ltx_ctx_destroy(ltx_ctx *ctx) {
     cudaSetDevice(ctx->device);
     cudaStreamSynchronize(ctx->stream);
     ltx::comm_release(ctx, false);
-    if (ctx->pool) cudaMemPoolDestroy(ctx->pool);
+    if (ctx->kept) cudaFreeAsync(ctx->kept, ctx->stream);
+    if (ctx->pool) {
+        cudaStreamSynchronize(ctx->stream);
+        cudaMemPoolDestroy(ctx->pool);
+    }
     if (ctx->scratch) cudaFree(ctx->scratch);
     if (ctx->work) cudaFree(ctx->work);
     if (ctx->pinned) cudaFreeHost(ctx->pinned);

@@ -57,8 +57,11 @@ struct ltx_ctx {
     // Forward/step workspace (activations), grown on demand and reused.
     void *work = nullptr;
     size_t work_bytes = 0;
-    // Pool of the per-call workspaces (work_alloc), made by the first of them.
+    // Pool of the workspaces of work_alloc, made by the first of them, and the
+    // one that eager calls use in turn.
     cudaMemPool_t pool = nullptr;
+    void *kept = nullptr;
+    size_t kept_bytes = 0;
     // Pinned host staging for the small per-call uploads (timestep index),
     // so they do not serialise the host with the stream.
     void *pinned = nullptr;
@@ -119,12 +122,16 @@ struct DeviceGuard {
 
 // Makes sure ctx->scratch holds at least `bytes`; returns a status.
 int ensure_scratch(ltx_ctx *ctx, size_t bytes);
-// A workspace for one call, allocated and freed in the order of the context's
-// stream.  Unlike the scratch buffer it belongs to that call alone: one captured
-// into a CUDA graph is the graph's own, so graphs do not share it and nothing
-// frees it under them.
+// A workspace for one call, in the order of the context's stream: work_free
+// gives it back behind the call's kernels.  Eager calls, which that stream
+// orders, share one that the context keeps; a call captured into a CUDA graph
+// gets memory of the graph's own, so graphs do not share it with each other or
+// with eager calls, and nothing frees it under them.
 int work_alloc(ltx_ctx *ctx, size_t bytes, void **out);
 int work_free(ltx_ctx *ctx, void *p);
+// Lets a kernel use up to `bytes` of dynamic shared memory on the context's
+// device (asked of the runtime once; every call for a kernel names the same bytes).
+cudaError_t allow_smem(const ltx_ctx *ctx, const void *kernel, int bytes);
 // Copies host bytes to the device through the context's pinned staging
 // buffer (waits for the previous upload from that buffer to finish first).
 int upload(ltx_ctx *ctx, void *dst_dev, const void *src_host, size_t bytes);
