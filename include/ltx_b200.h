@@ -358,7 +358,7 @@ int ltx_qk_norm_rope(ltx_ctx *ctx, const ltx_norm_rope *args);
  * low-rank sums stay in f32; for the f32 epilogues the product with B is
  * taken in two bf16 parts that together keep 16 bits of it.  Scratch comes
  * from the context's pool in stream order. */
-#define LTX_MAX_ADAPTERS 2048
+#define LTX_MAX_ADAPTERS 1024
 #define LTX_MAX_ADAPTER_RANK 256
 typedef struct {
     const void *x_dev, *w_dev;                            /* bf16 [m, k], [n, k]                                         */

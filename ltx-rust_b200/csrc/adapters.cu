@@ -166,7 +166,7 @@ __device__ __forceinline__ void split_bf16(float v, __nv_bfloat16 &hi, __nv_bflo
 template <int TN>
 struct LowCfg {
     static constexpr int X_BYTES = TN * 128, PAD = BM * 128;
-    static constexpr int STAGES = TN == 64 ? 4 : 5;
+    static constexpr int STAGES = TN == 64 ? 3 : 5;   // three CTAs per SM at ranks up to 64
     static int ring(int a_bytes) { return STAGES * (X_BYTES + a_bytes) + PAD; }
     static int bytes(int a_bytes) { return 1024 + ring(a_bytes) + 256 + (int)sizeof(TileList<TN>) + (int)sizeof(ListScratch<TN>); }
     static constexpr int COLS = TN < 32 ? 32 : TN;
@@ -372,6 +372,13 @@ struct Ahead {
 #pragma unroll
         for (int j = 0; j < 16; ++j) x[j] = in && j < count ? static_cast<const float *>(p.out)[o + j * p.ldo] : 0.f;
         if (!p.gate) return;
+        const int g0 = __shfl_sync(0xffffffffu, gidx, at), l = threadIdx.x & 31;
+        if (__all_sync(0xffffffffu, l < at || l >= at + 16 || gidx == g0)) {   // one row for all, as tokens of one request have
+            const float one = in ? __ldg(p.gate + g0 * p.ld_gate + n) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) g[j] = one;
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             const int64_t row = __shfl_sync(0xffffffffu, gidx, at + j) * p.ld_gate;
@@ -406,6 +413,66 @@ __device__ __forceinline__ void finish16(const AdapterParams &p, int m, int coun
         for (int j = 0; j < 16; ++j)
             if (j < count) o[j * p.ldo] = EPI == LTX_EPI_RESID ? h.x[j] + (v[j] + bias) * (p.gate ? h.g[j] : 1.f) : v[j] + bias;
     }
+}
+
+// A tile's epilogue, every other 32 tokens of it from `side` on, by a warp whose
+// lanes hold 32 weight rows.
+template <int EPI>
+struct TileEpilogue {
+    Ahead cur, next;
+    int gidx = 0;
+    __device__ __forceinline__ void begin(const AdapterParams &p, int m0, int tokens, int n, int side, int lane) {
+        if (EPI == LTX_EPI_RESID && side < tokens) {
+            gidx = gate_rows(p, m0 + side, lane);
+            next.fetch(p, m0 + side, tokens - side, n, gidx, 0);
+        }
+    }
+    __device__ __forceinline__ void run(const AdapterParams &p, uint32_t acc, int m0, int tokens, int n, int side, int lane,
+                                        float bias) {
+#pragma unroll 1
+        for (int c = side; c < tokens; c += 64) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32(acc + c, r);
+            int gnext = 0;
+            if (EPI == LTX_EPI_RESID && c + 64 < tokens) gnext = gate_rows(p, m0 + c + 64, lane);
+            tmem_ld_wait_regs(r);
+#pragma unroll
+            for (int h = 0; h < 32; h += 16) {
+                if (c + h >= tokens) break;
+                if constexpr (EPI == LTX_EPI_RESID) {
+                    cur = next;
+                    const int to = h ? c + 64 : c + 16;
+                    if (to < tokens) next.fetch(p, m0 + to, tokens - to, n, h ? gnext : gidx, h ? 0 : 16);
+                }
+                float v[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[h + j]);
+                finish16<EPI>(p, m0 + c + h, tokens - c - h, n, bias, v, cur);
+            }
+            gidx = gnext;
+        }
+    }
+};
+
+// One block of `low` for the product with adapter a's columns of B, by a warp:
+// rows of ROWS tokens from m0 on, zeros for tokens of other adapters and behind
+// the rank.  `which`: 64 ranks and the bf16 part.  Asynchronous (one commit group).
+template <int ROWS>
+__device__ __forceinline__ void copy_low(const AdapterParams &p, int a, int which, int m0, const int16_t *tok, int lane,
+                                         unsigned char *to) {
+    const int ld = p.rank_blocks * 64, rb = which / p.parts;
+    const __nv_bfloat16 *src = p.low + (which % p.parts ? (int64_t)p.m * ld : 0) + rb * 64;
+    const uint32_t dst = smem_u32(to);
+#pragma unroll 8
+    for (int x = lane; x < ROWS * 8; x += 32) {   // 16-byte piece c of token j sits at c ^ (j % 8)
+        const int j = x >> 3, c = x & 7;
+        const bool mine = tok[j] == a && rb * 64 + c * 8 < p.rank;
+        const __nv_bfloat16 *from = mine ? src + (int64_t)(m0 + j) * ld + c * 8 : p.low;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + j * 128 + ((c ^ (j & 7)) << 4)), "l"(from),
+                     "r"(mine ? 16 : 0)
+                     : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
 }
 
 template <int TN, int EPI>
@@ -579,7 +646,6 @@ __global__ void __launch_bounds__(kProjThreads, 1)
             }
         }
     } else if (warp == 10) {
-        const int ld = p.rank_blocks * 64;
         bool waited = false;
         uint32_t i = 0, built = 0;
         for (int t = first; t < tiles && !aborted; t += stride, ++i) {
@@ -608,19 +674,8 @@ __global__ void __launch_bounds__(kProjThreads, 1)
             for (int b = 0; b < na; ++b, ++built) {
                 const int buf = built % C::BUFS;
                 if (!warp_wait(&bempty[buf], ((built / C::BUFS) & 1) ^ 1, p.flag, 419, &aborted)) break;
-                const int e = a0 + b, a = list.ids[e / per_adapter], rest = e % per_adapter, rb = rest / p.parts;
-                const __nv_bfloat16 *src = p.low + (rest % p.parts ? (int64_t)p.m * ld : 0) + rb * 64;
-                const uint32_t dst = smem_u32(smem + C::BUF + buf * C::B_BYTES);
-#pragma unroll 8
-                for (int x = lane; x < TN * 8; x += 32) {   // 16-byte piece c of token j sits at c ^ (j % 8)
-                    const int j = x >> 3, c = x & 7;
-                    const bool mine = scratch.tok[j] == a && rb * 64 + c * 8 < p.rank;   // ranks behind the last: 0
-                    const __nv_bfloat16 *from = mine ? src + (int64_t)(m0 + j) * ld + c * 8 : p.low;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + j * 128 + ((c ^ (j & 7)) << 4)),
-                                 "l"(from), "r"(mine ? 16 : 0)
-                                 : "memory");
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
+                const int e = a0 + b;
+                copy_low<TN>(p, list.ids[e / per_adapter], e % per_adapter, m0, scratch.tok, lane, smem + C::BUF + buf * C::B_BYTES);
                 if constexpr (C::BUFS == 1) {
                     asm volatile("cp.async.wait_group 0;" ::: "memory");
                     hand_over(built);
@@ -629,10 +684,8 @@ __global__ void __launch_bounds__(kProjThreads, 1)
                     hand_over(built - 1);
                 }
             }
-            if (C::BUFS > 1 && na > 0 && !aborted) {
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                hand_over(built - 1);
-            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            if (C::BUFS > 1 && na > 0 && !aborted) hand_over(built - 1);
         }
         grid_dep_wait();   // low_kernel has ended before this kernel does: the workspace is free behind it
     } else {
@@ -646,39 +699,12 @@ __global__ void __launch_bounds__(kProjThreads, 1)
             const int n = nt * BM + quad * 32 + lane, m0 = mt * TN;
             const float bias = p.bias && n < p.n ? p.bias[n] : 0.f;
             const int tokens = min(TN, p.m - m0);
-            Ahead cur, next;
-            int gidx = 0;
-            if (EPI == LTX_EPI_RESID && p.splits == 1 && side < tokens) {   // under the products
-                gidx = gate_rows(p, m0 + side, lane);
-                next.fetch(p, m0 + side, tokens - side, n, gidx, 0);
-            }
+            TileEpilogue<EPI> out;
+            if (p.splits == 1) out.begin(p, m0, tokens, n, side, lane);   // under the products
             if (!warp_wait(&tfull[acc], (i >> 1) & 1, p.flag, 420, &aborted)) break;
             tc_fence_after();
-            if (p.splits == 1) {
-                const uint32_t d = tmem + ((uint32_t)(quad * 32) << 16) + acc * C::ACC;
-#pragma unroll 1
-                for (int c = side; c < tokens; c += 64) {
-                    uint32_t r[32];
-                    tmem_ld_32x32b_x32(d + c, r);
-                    int gnext = 0;
-                    if (EPI == LTX_EPI_RESID && c + 64 < tokens) gnext = gate_rows(p, m0 + c + 64, lane);
-                    tmem_ld_wait_regs(r);
-#pragma unroll
-                    for (int h = 0; h < 32; h += 16) {
-                        if (c + h >= tokens) break;
-                        if constexpr (EPI == LTX_EPI_RESID) {
-                            cur = next;
-                            const int to = h ? c + 64 : c + 16;
-                            if (to < tokens) next.fetch(p, m0 + to, tokens - to, n, h ? gnext : gidx, h ? 0 : 16);
-                        }
-                        float v[16];
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[h + j]);
-                        finish16<EPI>(p, m0 + c + h, tokens - c - h, n, bias, v, cur);
-                    }
-                    gidx = gnext;
-                }
-            }
+            if (p.splits == 1)
+                out.run(p, tmem + ((uint32_t)(quad * 32) << 16) + acc * C::ACC, m0, tokens, n, side, lane, bias);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&tempty[acc]);
@@ -715,6 +741,271 @@ __global__ void __launch_bounds__(kProjThreads, 1)
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, C::COLS);
+    }
+}
+
+// ── the projection, many tokens ──────────────────────────────────────────────
+//
+// The same with two SMs on one tile of 256 weight rows x 256 tokens
+// (cta_group::2): each CTA of a cluster of two loads its 128 weight rows and half
+// of the tokens, so a block of 64 K costs an SM 32 KB of loads instead of 48 for
+// the same products (one-SM tiles are held up by L2).  The even CTA's thread issues
+// the products for both; both CTAs' loads count on its barriers.  Accumulators,
+// epilogue and builder are each CTA's own: it holds its 128 weight rows for all 256
+// tokens.
+struct PairCfg {
+    static constexpr int TOKENS = 256, HALF = 128;
+    static constexpr int A_BYTES = BM * 128, B_BYTES = HALF * 128, STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = 6, BUFS = 2;
+    static constexpr int RING = STAGES * STAGE, BUF = RING, BAR = BUF + BUFS * B_BYTES;
+    static constexpr int LIST = BAR + ((2 * STAGES + 8 + 2 * BUFS) * 8 + 8 + 15) / 16 * 16;
+    static constexpr int BYTES = 1024 + LIST + 2 * (int)sizeof(TileList<TOKENS>) + (int)sizeof(ListScratch<TOKENS>);
+    static_assert(BYTES <= 232448, "shared memory exceeds the per-CTA limit");
+};
+
+__device__ __forceinline__ void mbar_arrive_at(uint64_t *bar, uint32_t rank) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(peer_addr(bar, rank)) : "memory");
+}
+// mbar_wait for a barrier on which another CTA of the cluster arrives.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity, int *flag, int code, bool *aborted) {
+    if (*aborted) return false;
+    uint64_t t0 = 0;
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (!t0) t0 = global_ns();
+        else if (global_ns() - t0 > kWaitLimitNs) {
+            atomicExch(flag, code);
+            *aborted = true;
+            return false;
+        }
+    }
+}
+// A load into this CTA's shared memory that counts on the barrier at `bar`, an
+// address in the pair's even CTA.
+__device__ __forceinline__ void pair_load(void *dst, const void *tmap, uint32_t bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+            smem_u32(dst)),
+        "l"(tmap), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+__device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+// Arrives on `bar` of both CTAs when the products issued so far are done.
+__device__ __forceinline__ void pair_commit(uint64_t *bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+
+template <int EPI>
+__global__ void __launch_bounds__(kProjThreads, 1)
+    project_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                        const __grid_constant__ CUtensorMap tmB, AdapterParams p) {
+    using C = PairCfg;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::BAR), *empty = full + C::STAGES;
+    uint64_t *tfull = empty + C::STAGES, *tempty = tfull + 2, *lfull = tempty + 2, *lempty = lfull + 2;
+    uint64_t *bfull = lempty + 2, *bempty = bfull + C::BUFS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bempty + C::BUFS);
+    TileList<C::TOKENS> *lists = reinterpret_cast<TileList<C::TOKENS> *>(smem + C::LIST);
+    ListScratch<C::TOKENS> &scratch = *reinterpret_cast<ListScratch<C::TOKENS> *>(smem + C::LIST + 2 * sizeof(TileList<C::TOKENS>));
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = blockIdx.x & 1;
+    const int first = blockIdx.x / 2, stride = gridDim.x / 2, tiles = p.m_tiles * p.n_tiles;
+    const int nk = (p.k + 63) / 64, per_adapter = p.rank_blocks * p.parts;
+    if (threadIdx.x == 0) {
+        tma_prefetch_desc(&tmW);
+        tma_prefetch_desc(&tmX);
+        if (p.adapters) tma_prefetch_desc(&tmB);
+        for (int s = 0; s < C::STAGES; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&tfull[i], 1);
+            mbar_init(&tempty[i], 16);
+            mbar_init(&lfull[i], 32);
+            mbar_init(&lempty[i], rank == 0 ? 2 : 1);
+        }
+        for (int i = 0; i < C::BUFS; ++i) {
+            mbar_init(&bfull[i], 2);
+            mbar_init(&bempty[i], 1);
+        }
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+    }
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    bool aborted = false;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0, i = 0;
+            for (int t = first; t < tiles && !aborted; t += stride, ++i) {
+                int mt, nt;
+                tile_at(p, t, mt, nt);
+                const TileList<C::TOKENS> &list = lists[i & 1];
+                if (!mbar_wait(&lfull[i & 1], (i >> 1) & 1, p.flag, 431, &aborted)) break;
+                const int na = list.count * per_adapter, n0 = nt * 2 * BM + rank * BM;
+                auto take = [&](uint32_t bytes) {   // bytes that both CTAs load
+                    const int s = it % C::STAGES;
+                    if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, p.flag, 432, &aborted)) return -1;
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
+                    ++it;
+                    return s;
+                };
+                blocks_in_order(
+                    nk, na,
+                    [&](int k) {
+                        const int s = take(2 * C::STAGE);
+                        if (s < 0) return false;
+                        const uint32_t bar = peer_addr(&full[s], 0);
+                        pair_load(smem + s * C::STAGE, &tmW, bar, k * 64, n0);
+                        pair_load(smem + s * C::STAGE + C::A_BYTES, &tmX, bar, k * 64, mt * C::TOKENS + rank * C::HALF);
+                        return true;
+                    },
+                    [&](int e) {
+                        const int s = take(2 * C::A_BYTES);
+                        if (s < 0) return false;
+                        pair_load(smem + s * C::STAGE, &tmB, peer_addr(&full[s], 0), e % per_adapter / p.parts * 64,
+                                  list.ids[e / per_adapter] * p.n + n0);
+                        return true;
+                    });
+                mbar_arrive(&lempty[i & 1]);
+            }
+            if (aborted && rank == 0) {   // let the copies already issued land before the CTA exits
+                bool a2 = false;
+                for (uint32_t j = it > (uint32_t)C::STAGES ? it - C::STAGES : 0; j < it; ++j)
+                    mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, nullptr, 0, &a2);
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            constexpr uint32_t idesc = idesc_f16(2 * BM, C::TOKENS, true);
+            uint32_t it = 0, i = 0, built = 0;
+            for (int t = first; t < tiles && !aborted; t += stride, ++i) {
+                const uint32_t acc = i & 1;
+                if (!mbar_wait(&lfull[acc], (i >> 1) & 1, p.flag, 433, &aborted)) break;
+                const int na = lists[acc].count * per_adapter;
+                if (!mbar_wait_cluster(&tempty[acc], ((i >> 1) & 1) ^ 1, p.flag, 435, &aborted)) break;
+                tc_fence_after();
+                const uint32_t d = tmem + acc * C::TOKENS;
+                uint32_t more = 0;
+                auto multiply = [&](uint32_t b_addr) {
+                    const int s = it % C::STAGES;
+                    if (!mbar_wait_cluster(&full[s], (it / C::STAGES) & 1, p.flag, 436, &aborted)) return false;
+                    tc_fence_after();
+                    const uint32_t a_addr = smem_u32(smem + s * C::STAGE);
+                    if (!b_addr) b_addr = a_addr + C::A_BYTES;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        pair_mma(d, sdesc_sw128(a_addr + q * 32, 16, 1024), sdesc_sw128(b_addr + q * 32, 16, 1024), idesc, more);
+                        more = 1;
+                    }
+                    pair_commit(&empty[s]);
+                    ++it;
+                    return true;
+                };
+                blocks_in_order(
+                    nk, na, [&](int) { return multiply(0); },
+                    [&](int) {
+                        const int b = built % C::BUFS;
+                        if (!mbar_wait_cluster(&bfull[b], (built / C::BUFS) & 1, p.flag, 437, &aborted) ||
+                            !multiply(smem_u32(smem + C::BUF + b * C::B_BYTES)))
+                            return false;
+                        pair_commit(&bempty[b]);
+                        ++built;
+                        return true;
+                    });
+                if (aborted) break;
+                pair_commit(&tfull[acc]);
+                mbar_arrive(&lempty[acc]);
+            }
+        }
+    } else if (warp == 10) {
+        bool waited = false;
+        uint32_t i = 0, built = 0;
+        for (int t = first; t < tiles && !aborted; t += stride, ++i) {
+            int mt, nt;
+            tile_at(p, t, mt, nt);
+            const int m0 = mt * C::TOKENS;
+            TileList<C::TOKENS> &list = lists[i & 1];
+            if (!warp_wait(&lempty[i & 1], ((i >> 1) & 1) ^ 1, p.flag, 438, &aborted)) break;
+            if (p.adapters) build_list<C::TOKENS, 32>(p, m0, lane, list, scratch);
+            else if (lane == 0) list.count = 0;
+            mbar_arrive(&lfull[i & 1]);
+            __syncwarp();
+            const int na = list.count * per_adapter;
+            if (na > 0 && !waited) {
+                grid_dep_wait();
+                waited = true;
+            }
+            auto hand_over = [&](uint32_t which) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive_at(&bfull[which % C::BUFS], 0);
+            };
+            for (int e = 0; e < na; ++e, ++built) {
+                const int buf = built % C::BUFS;
+                if (!warp_wait(&bempty[buf], ((built / C::BUFS) & 1) ^ 1, p.flag, 439, &aborted)) break;
+                copy_low<C::HALF>(p, list.ids[e / per_adapter], e % per_adapter, m0 + rank * C::HALF, scratch.tok + rank * C::HALF, lane,
+                                  smem + C::BUF + buf * C::B_BYTES);
+                if (e > 0) {   // the one before, while this one is on its way
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    hand_over(built - 1);
+                }
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            if (na > 0 && !aborted) hand_over(built - 1);
+        }
+        grid_dep_wait();   // low_kernel has ended before this kernel does: the workspace is free behind it
+    } else {
+        // warps 2-5 and 6-9 take every other 32 tokens of a tile
+        const int quad = warp & 3, side = warp >= 6 ? 32 : 0;
+        uint32_t i = 0;
+        for (int t = first; t < tiles && !aborted; t += stride, ++i) {
+            int mt, nt;
+            tile_at(p, t, mt, nt);
+            const uint32_t acc = i & 1;
+            const int n = nt * 2 * BM + rank * BM + quad * 32 + lane, m0 = mt * C::TOKENS, tokens = min(C::TOKENS, p.m - m0);
+            const float bias = p.bias && n < p.n ? p.bias[n] : 0.f;
+            TileEpilogue<EPI> out;
+            out.begin(p, m0, tokens, n, side, lane);   // under the products
+            if (!warp_wait(&tfull[acc], (i >> 1) & 1, p.flag, 440, &aborted)) break;
+            tc_fence_after();
+            out.run(p, tmem + ((uint32_t)(quad * 32) << 16) + acc * C::TOKENS, m0, tokens, n, side, lane, bias);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_at(&tempty[acc], 0);
+        }
+    }
+
+    tc_fence_before();
+    cluster_sync();   // neither CTA exits, or frees its TMEM, while the other still uses it
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
 }
 
@@ -782,7 +1073,7 @@ int splits_for(int64_t jobs, int room, int kb) {
 
 template <int TN>
 cudaError_t run_low(const ltx_ctx *ctx, AdapterParams p, const CUtensorMap &ta, const CUtensorMap &tx) {
-    const int tiles = (p.m + TN - 1) / TN, room = 2 * ctx->sm_count;
+    const int tiles = (p.m + TN - 1) / TN, room = (p.rank <= 64 ? 3 : 2) * ctx->sm_count;   // CTAs at once
     p.splits = splits_for(tiles, room, (p.k + 63) / 64);
     // the SMs left over share the adapters of a tile; what one takes goes together
     const int blocks = (p.rank + BM - 1) / BM, most = std::min({p.adapters, TN, p.m});
@@ -790,6 +1081,15 @@ cudaError_t run_low(const ltx_ctx *ctx, AdapterParams p, const CUtensorMap &ta, 
     p.unit = blocks > 1 ? 1 : std::min(BM / p.rank, (most + p.tile_lanes - 1) / p.tile_lanes);
     return launch(ctx, low_kernel<TN>, tiles * p.tile_lanes * p.splits, kLowThreads,
                   LowCfg<TN>::bytes(p.unit * std::min(p.rank, BM) * 128), LowCfg<TN>::bytes(BM * 128), p.splits, false, ta, tx, p);
+}
+
+// A weight within 48 MB stays in L2: then the weight tiles of one token tile run
+// back to back.  Otherwise as many token tiles go together as keep their rows of x
+// within 48 MB, and the weights stream once per group.
+int group_of(const AdapterParams &p, int tokens) {
+    constexpr int64_t kPanel = 48 << 20;
+    return (int64_t)p.n * p.k * 2 <= kPanel ? 1
+                                            : (int)std::max<int64_t>(1, std::min<int64_t>(p.m_tiles, kPanel / ((int64_t)tokens * p.k * 2)));
 }
 
 template <int TN>
@@ -800,13 +1100,7 @@ cudaError_t run_project(const ltx_ctx *ctx, AdapterParams p, int epilogue, const
     p.n_tiles = (p.n + BM - 1) / BM;
     const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
     p.splits = splits_for(tiles, sms, (p.k + 63) / 64);
-    // A weight within 48 MB stays in L2: then the weight tiles of one token
-    // tile run back to back.  Otherwise as many token tiles go together as keep
-    // their rows of x within 48 MB, and the weights stream once per group.
-    constexpr int64_t kPanel = 48 << 20;
-    p.group_m = (int64_t)p.n * p.k * 2 <= kPanel
-                    ? 1
-                    : (int)std::max<int64_t>(1, std::min<int64_t>(p.m_tiles, kPanel / ((int64_t)TN * p.k * 2)));
+    p.group_m = group_of(p, TN);
     const int grid = p.splits > 1 ? (int)tiles * p.splits : (int)std::min<int64_t>(tiles, sms);
     auto go = [&](auto kern) {
         return launch(ctx, kern, grid, kProjThreads, ProjCfg<TN>::BYTES, ProjCfg<TN>::BYTES, p.splits, p.adapters > 0, tw, tx, tb, p);
@@ -816,6 +1110,24 @@ cudaError_t run_project(const ltx_ctx *ctx, AdapterParams p, int epilogue, const
     case LTX_EPI_GELU_BF16: return go(project_kernel<TN, LTX_EPI_GELU_BF16>);
     case LTX_EPI_F32: return go(project_kernel<TN, LTX_EPI_F32>);
     default: return go(project_kernel<TN, LTX_EPI_RESID>);
+    }
+}
+
+cudaError_t run_pair(const ltx_ctx *ctx, AdapterParams p, int epilogue, const CUtensorMap &tw, const CUtensorMap &tx,
+                     const CUtensorMap &tb) {
+    p.m_tiles = (p.m + PairCfg::TOKENS - 1) / PairCfg::TOKENS;
+    p.n_tiles = (p.n + 2 * BM - 1) / (2 * BM);
+    p.splits = 1;
+    p.group_m = group_of(p, PairCfg::TOKENS);
+    const int grid = 2 * (int)std::min<int64_t>((int64_t)p.m_tiles * p.n_tiles, ctx->sm_count / 2);
+    auto go = [&](auto kern) {
+        return launch(ctx, kern, grid, kProjThreads, PairCfg::BYTES, PairCfg::BYTES, 2, p.adapters > 0, tw, tx, tb, p);
+    };
+    switch (epilogue) {
+    case LTX_EPI_BF16: return go(project_pair_kernel<LTX_EPI_BF16>);
+    case LTX_EPI_GELU_BF16: return go(project_pair_kernel<LTX_EPI_GELU_BF16>);
+    case LTX_EPI_F32: return go(project_pair_kernel<LTX_EPI_F32>);
+    default: return go(project_pair_kernel<LTX_EPI_RESID>);
     }
 }
 
@@ -875,8 +1187,10 @@ extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args) {
     p.out = out_dev;
     p.flag = ctx->timeout_flag;
     const int tn = tokens_for(m), tl = std::min(tn, 64);
+    // enough 256 x 256 tiles for every pair of SMs
+    const bool pair = tn == 256 && (int64_t)((m + 255) / 256) * ((n + 255) / 256) * 2 > ctx->sm_count;
     CUtensorMap tw, tx, txl, ta, tb;
-    bool ok = make_map(&tw, w_dev, n, k, ldw, BM) && make_map(&tx, x_dev, m, k, ldx, tn);
+    bool ok = make_map(&tw, w_dev, n, k, ldw, BM) && make_map(&tx, x_dev, m, k, ldx, pair ? 128 : tn);
     ta = tb = txl = tx;
     if (adapters)
         ok = ok && make_map(&txl, x_dev, m, k, ldx, tl) &&
@@ -894,7 +1208,8 @@ extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args) {
                        : run_low<64>(ctx, p, ta, txl);
     }
     if (e == cudaSuccess)
-        e = tn == 16    ? run_project<16>(ctx, p, epilogue, tw, tx, tb)
+        e = pair        ? run_pair(ctx, p, epilogue, tw, tx, tb)
+            : tn == 16  ? run_project<16>(ctx, p, epilogue, tw, tx, tb)
             : tn == 32  ? run_project<32>(ctx, p, epilogue, tw, tx, tb)
             : tn == 64  ? run_project<64>(ctx, p, epilogue, tw, tx, tb)
             : tn == 128 ? run_project<128>(ctx, p, epilogue, tw, tx, tb)

@@ -229,6 +229,15 @@ def test_gemm_adapters(ctx, m, n, k, rank, adapters, lengths, epi):
                  gate=(0, 1, 2)[m % 3])
 
 
+@pytest.mark.parametrize("epi", [0, 1, 2, 3])
+@pytest.mark.parametrize("m,n,k,rank,adapters,lengths", [
+    (2100, 2601, 192, 40, 5, [300, 1, 70]), (1025, 4480, 64, 8, 3, [1024]), (513, 6500, 200, 256, 2, [400]),
+    (5000, 1100, 320, 64, 40, [1])])
+def test_gemm_adapters_many_tokens(ctx, m, n, k, rank, adapters, lengths, epi):
+    """Enough tiles for two SMs to share one each, the last of them ragged both ways."""
+    adapter_case(ctx, m, n, k, rank, runs(m, lengths, adapters, start=1), epi, adapters, bias=m % 2 == 0, gate=2)
+
+
 @pytest.mark.parametrize("epi", [0, 3])
 def test_gemm_adapters_strides_and_odd_rows(ctx, epi):
     adapter_case(ctx, 45, 77, 96, 16, runs(45, [4, 9], 3), epi, 3, x_pad=8, o_pad=3)
