@@ -176,21 +176,25 @@ struct Share {
 };
 
 // What changes a row's scores: nothing but the scale, a bias by distance, or a cap
-// (and perhaps a bias).
-enum Mode { kPlain = 0, kBias = 1, kCap = 2 };
+// (and perhaps a bias).  kCapFixed: a cap alone, of at most kFixedCap in the log2
+// domain, with bf16 V: 2^score fits f32 and bf16 as it is, so no maximum is kept
+// and the scores are gone through once.
+enum Mode { kPlain = 0, kBias = 1, kCap = 2, kCapFixed = 3 };
+constexpr float kFixedCap = 100.f;   // 2^100 by 2^29 keys stays within f32
 
 // Scores of one row in the log2 domain.  The scale goes with the log2e, and the
 // bias is linear on either side of the key the row stands beside, so a tile that
 // lies on one side for every row of the warp needs one multiply-add more.
 template <int MODE>
 struct RowScores {
-    float2 sc;              // kPlain, kBias: scale log2e; kCap: scale / cap
-    float cap2;             // kCap: cap log2e
+    static constexpr bool kCapped = MODE == kCap || MODE == kCapFixed;
+    float2 sc;              // kPlain, kBias: scale log2e; capped: scale / cap
+    float cap2;             // capped: cap log2e
     float slope;            // slope log2e, 0 without
     float place;            // the row's key less the tile's first
     int side;               // 1: the tile's keys lie before it for every row, -1: behind, 0: both
     __device__ __forceinline__ void set_tile(int pl) {
-        if constexpr (MODE != kPlain) {
+        if constexpr (MODE == kBias || MODE == kCap) {
             place = (float)pl;
             side = __all_sync(0xffffffffu, pl >= BKV - 1) ? 1 : __all_sync(0xffffffffu, pl <= 0) ? -1 : 0;
         }
@@ -202,7 +206,7 @@ struct RowScores {
 #pragma unroll
         for (int u = 0; u < 16; ++u)
             v[u] = __fmul2_rn(make_float2(__uint_as_float(r[2 * u]), __uint_as_float(r[2 * u + 1])), sc);
-        if constexpr (MODE == kCap) {
+        if constexpr (kCapped) {
             float big = 0.f;
 #pragma unroll
             for (int u = 0; u < 16; ++u) big = fmaxf(big, fmaxf(fabsf(v[u].x), fabsf(v[u].y)));
@@ -217,7 +221,7 @@ struct RowScores {
                 }
             }
         }
-        if (MODE == kBias || slope != 0.f) {
+        if (MODE == kBias || (MODE == kCap && slope != 0.f)) {
             if (side != 0) {
                 const float s = side > 0 ? slope : -slope, base = s * ((float)e0 - place);
 #pragma unroll
@@ -381,6 +385,46 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_tmem, uint32_t o_tmem, c
     l += sum2.x + sum2.y;
     tmem_st_wait();             // P_t in TMEM ...
     tc_fence_before();          // ... and ordered before the arrive for the MMA thread
+}
+
+// The same for kCapFixed: P = 2^score, 32 keys at a time.
+__device__ __forceinline__ void softmax_tile_fixed(uint32_t s_tmem, const RowScores<kCapFixed> &rs, int left, bool masked,
+                                                   float &m_ref, float &l) {
+    float2 sum2 = make_float2(0.f, 0.f);
+    auto keys32 = [&](uint32_t (&r)[32], int e0, uint32_t col) {
+        rs.apply(r, e0);
+        if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                if (e0 + e >= left) r[e] = __float_as_uint(-INFINITY);
+        }
+        uint32_t pk[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+            const float2 pf = make_float2(ex2(__uint_as_float(r[2 * u])), ex2(__uint_as_float(r[2 * u + 1])));
+            sum2 = __fadd2_rn(sum2, pf);
+            pk[u] = pack16<false>(pf);
+        }
+        tmem_st_32x32b_x16(s_tmem + col, pk);
+    };
+    // P's columns 64..127 take the place of the scores of keys 64..127: those first
+    uint32_t a[32], b[32], c[32];
+    tmem_ld_32x32b_x32(s_tmem + 64, a);
+    tmem_ld_32x32b_x32(s_tmem + 96, b);
+    tmem_ld_wait_regs(a);
+    tmem_ld_wait_regs(b);
+    tmem_ld_32x32b_x32(s_tmem + 0, c);
+    keys32(a, 64, 96);
+    keys32(b, 96, 112);
+    tmem_ld_wait_regs(c);
+    tmem_ld_32x32b_x32(s_tmem + 32, a);
+    keys32(c, 0, 64);
+    tmem_ld_wait_regs(a);
+    keys32(a, 32, 80);
+    l += sum2.x + sum2.y;
+    if (left > 0) m_ref = 0.f;
+    tmem_st_wait();
+    tc_fence_before();
 }
 
 // VF16: V (and so P) are f16, otherwise bf16; Q and K are bf16.
@@ -590,9 +634,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int r_thread = quad * 32 + lane;
         const uint32_t s_tmem = tmem + ((uint32_t)(quad * 32) << 16) + t * 128, o_tmem = s_tmem + 256;
         RowScores<MODE> rs{};
-        const float sc = MODE == kCap ? p.scale / p.softcap : p.scale * kLog2e;
+        const float sc = rs.kCapped ? p.scale / p.softcap : p.scale * kLog2e;
         rs.sc = make_float2(sc, sc);
-        if constexpr (MODE == kCap) rs.cap2 = p.softcap * kLog2e;
+        if constexpr (rs.kCapped) rs.cap2 = p.softcap * kLog2e;
         uint32_t n_items = 0, n_s = 0;
         float m_ref = -INFINITY, l = 0.f;   // a row's maximum that P is taken against (log2 domain), its sum
         bool row_ok = false, any_o = false, join = false;
@@ -616,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 left = ok ? limit_of(p, i, token, sh.prefix) - top : kNoRow;
                 left_min = __reduce_min_sync(0xffffffffu, left);
                 place = token + i.lk - i.lq - top;
-                if constexpr (MODE != kPlain)
+                if constexpr (MODE == kBias || MODE == kCap)
                     rs.slope = p.slopes && ok ? p.slopes[i.kvh * p.group + r_in % p.group] * kLog2e : 0.f;
                 // V rows behind the document's end, in the first tile loaded: tile
                 // A's threads zero theirs, B's where A skips that tile
@@ -633,7 +677,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (active) {
                     tc_fence_after();
                     rs.set_tile(place);
-                    softmax_tile<D, VF16, MODE>(s_tmem, o_tmem, rs, left, left_min < BKV, m_ref, l);
+                    if constexpr (MODE == kCapFixed) softmax_tile_fixed(s_tmem, rs, left, left_min < BKV, m_ref, l);
+                    else softmax_tile<D, VF16, MODE>(s_tmem, o_tmem, rs, left, left_min < BKV, m_ref, l);
                 }
                 if (clean < BKV) {
                     if (r_in >= clean) {
@@ -771,9 +816,10 @@ cudaError_t launch_packed(const ltx_ctx *ctx, bool f16, Mode mode, const CUtenso
     auto kern = f16 ? (mode == kCap    ? packed_kernel<D, true, kCap>
                        : mode == kBias ? packed_kernel<D, true, kBias>
                                        : packed_kernel<D, true, kPlain>)
-                    : (mode == kCap    ? packed_kernel<D, false, kCap>
-                       : mode == kBias ? packed_kernel<D, false, kBias>
-                                       : packed_kernel<D, false, kPlain>);
+                    : (mode == kCap        ? packed_kernel<D, false, kCap>
+                       : mode == kCapFixed ? packed_kernel<D, false, kCapFixed>
+                       : mode == kBias     ? packed_kernel<D, false, kBias>
+                                           : packed_kernel<D, false, kPlain>);
     cudaError_t e = allow_smem(ctx, reinterpret_cast<const void *>(kern), Smem<D>::BYTES);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
@@ -876,7 +922,8 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const ltx_packed_attention
     // tiles each if one document had them all.
     while (p.splits < 8 && items * p.splits * 2 <= ctx->sm_count && (int64_t)p.splits * 4 * BKV <= rows_k) p.splits *= 2;
     p.pairs = (int)pairs;
-    const Mode mode = softcap > 0.f ? kCap : slopes_dev ? kBias : kPlain;
+    const bool fixed = !slopes_dev && v_dtype == LTX_BF16 && softcap * kLog2e <= kFixedCap;
+    const Mode mode = softcap > 0.f ? (fixed ? kCapFixed : kCap) : slopes_dev ? kBias : kPlain;
     const cudaError_t e = head_dim == 64 ? launch_packed<64>(ctx, v_dtype == LTX_F16, mode, tq, tk, tv, p)
                                          : launch_packed<128>(ctx, v_dtype == LTX_F16, mode, tq, tk, tv, p);
     return e == cudaSuccess ? LTX_OK : cuda_fail(ctx, e, w);
