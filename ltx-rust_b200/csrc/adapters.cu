@@ -30,7 +30,7 @@ constexpr int kMaxWords = LTX_MAX_ADAPTERS / 32;
 
 struct AdapterParams {
     int m, n, k, rank, adapters, rank_blocks, parts, splits, m_tiles, n_tiles, group_m;
-    int tile_lanes, unit;   // low_kernel: CTAs (clusters) per tile, adapters in one of their products
+    int tile_lanes, unit, low_stages;   // low_kernel: clusters per tile, adapters in one product, depth of its ring
     const int *idx, *gate_idx;
     const float *coeff, *bias, *gate;
     int64_t ldo, ld_gate;
@@ -160,17 +160,20 @@ __device__ __forceinline__ void split_bf16(float v, __nv_bfloat16 &hi, __nv_bflo
 // ranks behind one another in its 128 rows, so a mixed tile reads x once; with
 // few tiles, lanes of CTAs share a tile's adapters instead.
 
-// A stage is x's tile and the ranks in hand (a_bytes of them); the product reads
+// A stage is x's tile and the ranks in hand (a_bytes of them).  The product reads
 // 128 rows from there whatever is behind (rows that nothing reads), so a pad ends
-// the ring.  Small, so that these CTAs share SMs with project_kernel's.
+// the ring where they are fewer.  As many stages as the SM holds for the CTAs it
+// gets: what bounds this kernel is the latency of x.
 template <int TN>
 struct LowCfg {
-    static constexpr int X_BYTES = TN * 128, PAD = BM * 128;
-    static constexpr int STAGES = TN == 64 ? 3 : 5;   // three CTAs per SM at ranks up to 64
-    static int ring(int a_bytes) { return STAGES * (X_BYTES + a_bytes) + PAD; }
-    static int bytes(int a_bytes) { return 1024 + ring(a_bytes) + 256 + (int)sizeof(TileList<TN>) + (int)sizeof(ListScratch<TN>); }
+    static constexpr int X_BYTES = TN * 128, MAX_STAGES = 8;
+    static constexpr int REST = 256 + (int)sizeof(TileList<TN>) + (int)sizeof(ListScratch<TN>);
     static constexpr int COLS = TN < 32 ? 32 : TN;
-    static_assert(TN * BM * 4 <= STAGES * (X_BYTES + 1024) + PAD, "the f32 partials fit the ring");
+    __host__ __device__ static int ring(int a_bytes, int stages) {
+        const int bytes = stages * (X_BYTES + a_bytes) + (BM * 128 - a_bytes), partials = TN * BM * 4;
+        return bytes > partials ? bytes : partials;
+    }
+    static int bytes(int a_bytes, int stages) { return 1024 + ring(a_bytes, stages) + REST; }
 };
 constexpr int kLowThreads = 192;
 
@@ -181,8 +184,9 @@ __global__ void __launch_bounds__(kLowThreads)
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int box = min(p.rank, BM), a_bytes = p.unit * box * 128, stage = C::X_BYTES + a_bytes;   // rank % 8 == 0: whole swizzle blocks
-    unsigned char *behind = smem + C::STAGES * stage + C::PAD;
-    uint64_t *full = reinterpret_cast<uint64_t *>(behind), *empty = full + C::STAGES, *done = empty + C::STAGES;
+    const int stages = p.low_stages;
+    unsigned char *behind = smem + C::ring(a_bytes, stages);
+    uint64_t *full = reinterpret_cast<uint64_t *>(behind), *empty = full + C::MAX_STAGES, *done = empty + C::MAX_STAGES;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
     TileList<TN> &list = *reinterpret_cast<TileList<TN> *>(behind + 256);
     ListScratch<TN> &scratch = *reinterpret_cast<ListScratch<TN> *>(behind + 256 + sizeof(TileList<TN>));
@@ -195,7 +199,7 @@ __global__ void __launch_bounds__(kLowThreads)
     if (threadIdx.x == 0) {
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmX);
-        for (int s = 0; s < C::STAGES; ++s) {
+        for (int s = 0; s < stages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
@@ -227,8 +231,8 @@ __global__ void __launch_bounds__(kLowThreads)
         if (warp == 0) {
             if (elect_one())
                 for (int kk = k0; kk < k1; ++kk, ++it) {
-                    const int s = it % C::STAGES;
-                    if (!mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1, p.flag, 401, &aborted)) break;
+                    const int s = it % stages;
+                    if (!mbar_wait(&empty[s], ((it / stages) & 1) ^ 1, p.flag, 401, &aborted)) break;
                     mbar_arrive_expect_tx(&full[s], n_here * box * 128 + TN * 128);
                     for (int i = 0; i < n_here; ++i)
                         tma_load_2d(smem + s * stage + C::X_BYTES + i * box * 128, &tmA, &full[s], kk * 64,
@@ -239,8 +243,8 @@ __global__ void __launch_bounds__(kLowThreads)
             if (elect_one()) {
                 constexpr uint32_t idesc = idesc_f16(BM, TN, true);
                 for (int kk = k0; kk < k1; ++kk, ++it) {
-                    const int s = it % C::STAGES;
-                    if (!mbar_wait(&full[s], (it / C::STAGES) & 1, p.flag, 402, &aborted)) break;
+                    const int s = it % stages;
+                    if (!mbar_wait(&full[s], (it / stages) & 1, p.flag, 402, &aborted)) break;
                     tc_fence_after();
                     const uint32_t bd = smem_u32(smem + s * stage), ad = bd + C::X_BYTES;
 #pragma unroll
@@ -302,8 +306,8 @@ __global__ void __launch_bounds__(kLowThreads)
     }
     if (aborted && warp == 0) {   // let the copies already issued land before the CTA exits
         bool a2 = false;
-        for (uint32_t j = it > (uint32_t)C::STAGES ? it - C::STAGES : 0; j < it; ++j)
-            mbar_wait(&full[j % C::STAGES], (j / C::STAGES) & 1, nullptr, 0, &a2);
+        for (uint32_t j = it > (uint32_t)stages ? it - stages : 0; j < it; ++j)
+            mbar_wait(&full[j % stages], (j / stages) & 1, nullptr, 0, &a2);
     }
     tc_fence_before();
     __syncthreads();
@@ -1073,14 +1077,21 @@ int splits_for(int64_t jobs, int room, int kb) {
 
 template <int TN>
 cudaError_t run_low(const ltx_ctx *ctx, AdapterParams p, const CUtensorMap &ta, const CUtensorMap &tx) {
-    const int tiles = (p.m + TN - 1) / TN, room = (p.rank <= 64 ? 3 : 2) * ctx->sm_count;   // CTAs at once
+    const int tiles = (p.m + TN - 1) / TN, room = (p.rank <= 64 ? 3 : 2) * ctx->sm_count;   // CTAs at once, as their shared memory allows
     p.splits = splits_for(tiles, room, (p.k + 63) / 64);
     // the SMs left over share the adapters of a tile; what one takes goes together
     const int blocks = (p.rank + BM - 1) / BM, most = std::min({p.adapters, TN, p.m});
     p.tile_lanes = std::max(1, std::min(room / (tiles * p.splits), most * blocks));
     p.unit = blocks > 1 ? 1 : std::min(BM / p.rank, (most + p.tile_lanes - 1) / p.tile_lanes);
-    return launch(ctx, low_kernel<TN>, tiles * p.tile_lanes * p.splits, kLowThreads,
-                  LowCfg<TN>::bytes(p.unit * std::min(p.rank, BM) * 128), LowCfg<TN>::bytes(BM * 128), p.splits, false, ta, tx, p);
+    using C = LowCfg<TN>;
+    const int grid = tiles * p.tile_lanes * p.splits, a_bytes = p.unit * std::min(p.rank, BM) * 128;
+    // beside project_kernel's CTA (up to 128 tokens), or by themselves
+    const int here = std::max(1, std::min(3, (grid + ctx->sm_count - 1) / ctx->sm_count));
+    const int budget = p.m <= 128 ? 72 << 10 : ((227 << 10) / here - 2048);
+    p.low_stages = C::MAX_STAGES;
+    while (p.low_stages > 2 && C::bytes(a_bytes, p.low_stages) > budget) --p.low_stages;
+    return launch(ctx, low_kernel<TN>, grid, kLowThreads, C::bytes(a_bytes, p.low_stages), C::bytes(BM * 128, C::MAX_STAGES), p.splits,
+                  false, ta, tx, p);
 }
 
 // A weight within 48 MB stays in L2: then the weight tiles of one token tile run

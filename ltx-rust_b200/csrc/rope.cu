@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "device_common.cuh"
 #include "internal.hpp"
@@ -25,7 +26,8 @@ constexpr int kMaxRot = 512, kMaxHeadDim = 512;
 struct TableParams {
     const int *pos;
     int rows, half;
-    double log2_theta, inv_factor, orig_turns;   // orig_turns = original_len / 2pi, 0 = stretch every frequency
+    double powers[8];                // theta^(-2 2^b / rot_dim): a frequency is their product over the bits of its index
+    double inv_factor, orig_turns;   // orig_turns = original_len / 2pi, 0 = stretch every frequency
     double turns_low, inv_span;
     float amplitude;
     float *cos_out, *sin_out;
@@ -58,7 +60,9 @@ template <int VEC>
 __global__ void __launch_bounds__(256) rope_table_1d_kernel(TableParams p) {
     __shared__ double s_quarters[kMaxRot / 2];   // per position
     for (int i = threadIdx.x; i < p.half; i += blockDim.x) {
-        const double f = exp2(-p.log2_theta * i / p.half);   // theta^(-2i/rot)
+        double f = 1.0;   // theta^(-2i/rot)
+#pragma unroll
+        for (int b = 0; b < 8; ++b) f *= i >> b & 1 ? p.powers[b] : 1.0;
         const double w = p.orig_turns > 0 ? fmin(fmax((p.orig_turns * f - p.turns_low) * p.inv_span, 0.0), 1.0) : 0.0;
         s_quarters[i] = f * (w + (1.0 - w) * p.inv_factor) * 0.63661977236758134308;   // 2/pi
     }
@@ -367,9 +371,9 @@ extern "C" int ltx_rope_table(ltx_ctx *ctx, const int32_t *pos_dev, int32_t rows
     if (rows == 0) return LTX_OK;
     if (!cos_dev || !sin_dev) return fail(ctx, LTX_ERR_INVALID_ARG, "rope_table: null output");
     DeviceGuard guard(ctx);
-    TableParams p{pos_dev, rows, rot_dim / 2, std::log2(theta), 1.0 / factor,
-                  (double)original_len * 0.15915494309189533577, turns_low,
+    TableParams p{pos_dev, rows, rot_dim / 2, {}, 1.0 / factor, (double)original_len * 0.15915494309189533577, turns_low,
                   original_len > 0 ? 1.0 / (turns_high - turns_low) : 0.0, (float)amplitude, cos_dev, sin_dev};
+    for (int b = 0; b < 8; ++b) p.powers[b] = std::pow(theta, -(double)(1 << b) / p.half);
     const bool vec = p.half % 4 == 0 && !(((uintptr_t)cos_dev | (uintptr_t)sin_dev) & 15);
     const int at_once = 256 / (vec ? p.half / 4 : p.half);
     const int grid = std::min((rows + at_once - 1) / at_once, ctx->sm_count * 8);
