@@ -33,60 +33,71 @@ struct TableParams {
     float *cos_out, *sin_out;
 };
 
-// sin and cos of `quarters` quarter turns.  The whole quarters are split off in
-// f64 by adding 1.5 * 2^52 (a position of 2^24 has 11 million); only the rest r,
-// |r| <= 1/2, goes to f32, its rounding at most 2^-26 quarters.  sin(pi r/2) =
-// r S(r^2) and cos(pi r/2) = C(r^2) with S of degree 3 and C of degree 4, fitted
-// here to the least absolute error: with the f32 roundings 9.4e-8 at most, 2e-8
-// root mean square.
-__device__ __forceinline__ void sincos_quarters(double quarters, float &s, float &c) {
-    constexpr double kRound = 6755399441055744.0;
-    constexpr float s0 = 0x1.921fb4p+0f, s1 = -0x1.4abba8p-1f, s2 = 0x1.465a3ep-4f, s3 = -0x1.2cf5d4p-8f;
-    constexpr float c1 = -0x1.3bd3ccp+0f, c2 = 0x1.03c1dcp-2f, c3 = -0x1.55c57cp-6f, c4 = 0x1.d9c364p-11f;
-    const double t = quarters + kRound;
-    const unsigned q = (unsigned)__double2loint(t);
-    const float r = (float)(quarters - (t - kRound)), z = r * r;
-    const float sn = r * fmaf(fmaf(fmaf(s3, z, s2), z, s1), z, s0);
-    const float cs = fmaf(fmaf(fmaf(fmaf(c4, z, c3), z, c2), z, c1), z, 1.f);
-    const float a = q & 1 ? cs : sn, b = q & 1 ? sn : cs;
-    s = __uint_as_float(__float_as_uint(a) ^ ((q & 2) << 30));
-    c = __uint_as_float(__float_as_uint(b) ^ (((q + 1) & 2) << 30));
-}
+// The angle is kept as a 64-bit fraction of a turn: a frequency's turns per
+// position times 2^64, rounded from f64, times the position, modulo 2^64: whole
+// turns (2.7 million at position 2^24) fall off the top exactly, by two integer
+// multiplications.  The upper 32 bits are the angle to 2^-32 turns: two bits of
+// quarter and the rest r, |r| <= 1/2 quarter.  sin(pi r/2) = r S(r^2) and
+// cos(pi r/2) = C(r^2) with S of degree 3 and C of degree 4, fitted here to the
+// least absolute error: with the f32 roundings 9.4e-8 at most, 2e-8 root mean
+// square.  (A value took 16 f64 and conversion cycles more with the reduction in
+// f64: 18.4 us for 131072 x 64 instead of the figure below.)
+struct SinCos {
+    float s[4], c[5];   // the polynomials, the amplitude multiplied in
+    __device__ __forceinline__ explicit SinCos(float a)
+        : s{a * 0x1.921fb4p+0f, a * -0x1.4abba8p-1f, a * 0x1.465a3ep-4f, a * -0x1.2cf5d4p-8f},
+          c{a, a * -0x1.3bd3ccp+0f, a * 0x1.03c1dcp-2f, a * -0x1.55c57cp-6f, a * 0x1.d9c364p-11f} {}
+    // pos: the position's absolute value; sign: its sign bit
+    __device__ __forceinline__ void operator()(unsigned pos, unsigned sign, uint2 turns, float &sn, float &cs) const {
+        const unsigned angle = __umulhi(pos, turns.x) + pos * turns.y;   // bits 32..63 of the product
+        const unsigned q = (angle + 0x20000000u) >> 30;
+        const float r = (float)(int)(angle << 2) * 0x1p-32f, z = r * r;
+        const float a = r * fmaf(fmaf(fmaf(s[3], z, s[2]), z, s[1]), z, s[0]);
+        const float b = fmaf(fmaf(fmaf(fmaf(c[4], z, c[3]), z, c[2]), z, c[1]), z, c[0]);
+        sn = __uint_as_float(__float_as_uint(q & 1 ? b : a) ^ (((q & 2) << 30) ^ sign));
+        cs = __uint_as_float(__float_as_uint(q & 1 ? a : b) ^ (((q + 1) & 2) << 30));
+    }
+};
 
 // A thread keeps VEC neighbouring frequencies of its own and walks down the
 // rows: no division per value, 16-byte stores (VEC 4; 1 where rot_dim / 2 is
-// no multiple of 4).  A value costs some 25 instructions, so the stores bound it.
+// no multiple of 4).
 template <int VEC>
 __global__ void __launch_bounds__(256) rope_table_1d_kernel(TableParams p) {
-    __shared__ double s_quarters[kMaxRot / 2];   // per position
+    __shared__ uint2 s_turns[kMaxRot / 2];   // per position, lower and upper word
     for (int i = threadIdx.x; i < p.half; i += blockDim.x) {
         double f = 1.0;   // theta^(-2i/rot)
 #pragma unroll
         for (int b = 0; b < 8; ++b) f *= i >> b & 1 ? p.powers[b] : 1.0;
         const double w = p.orig_turns > 0 ? fmin(fmax((p.orig_turns * f - p.turns_low) * p.inv_span, 0.0), 1.0) : 0.0;
-        s_quarters[i] = f * (w + (1.0 - w) * p.inv_factor) * 0.63661977236758134308;   // 2/pi
+        double t = f * (w + (1.0 - w) * p.inv_factor) * 0.15915494309189533577;   // 1/2pi
+        t -= floor(t);
+        const unsigned long long u = t < 1.0 ? __double2ull_rn(t * 18446744073709551616.0) : 0ull;
+        s_turns[i] = make_uint2((unsigned)u, (unsigned)(u >> 32));
     }
     __syncthreads();
     const int per_row = p.half / VEC, rows_at_once = 256 / per_row;   // per_row <= 256: rot_dim <= 512
     const int i = threadIdx.x % per_row * VEC;
     if (threadIdx.x / per_row >= rows_at_once) return;
-    double quarters[VEC];
+    uint2 turns[VEC];
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) quarters[v] = s_quarters[i + v];
-    for (int64_t r = (int64_t)blockIdx.x * rows_at_once + threadIdx.x / per_row; r < p.rows;
-         r += (int64_t)gridDim.x * rows_at_once) {
-        const double pos = p.pos ? p.pos[r] : (int)r;
+    for (int v = 0; v < VEC; ++v) turns[v] = s_turns[i + v];
+    const SinCos sincos(p.amplitude);
+    // the next row's position is fetched under this one's values
+    const int step = (int)gridDim.x * rows_at_once;
+    int64_t r = (int64_t)blockIdx.x * rows_at_once + threadIdx.x / per_row;
+    int next = p.pos && r < p.rows ? p.pos[r] : (int)r;
+    for (; r < p.rows; r += step) {
+        const int at_pos = next;
+        next = !p.pos ? (int)(r + step) : r + step < p.rows ? p.pos[r + step] : 0;
+        const unsigned pos = at_pos < 0 ? 0u - (unsigned)at_pos : (unsigned)at_pos, sign = (unsigned)at_pos & 0x80000000u;
         float c[VEC], s[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            sincos_quarters(pos * quarters[v], s[v], c[v]);
-            c[v] *= p.amplitude;
-            s[v] *= p.amplitude;
-        }
+        for (int v = 0; v < VEC; ++v) sincos(pos, sign, turns[v], s[v], c[v]);
         const int64_t at = r * p.half + i;
         if constexpr (VEC == 4) {
-            *reinterpret_cast<float4 *>(p.cos_out + at) = make_float4(c[0], c[1], c[2], c[3]);
-            *reinterpret_cast<float4 *>(p.sin_out + at) = make_float4(s[0], s[1], s[2], s[3]);
+            __stcs(reinterpret_cast<float4 *>(p.cos_out + at), make_float4(c[0], c[1], c[2], c[3]));
+            __stcs(reinterpret_cast<float4 *>(p.sin_out + at), make_float4(s[0], s[1], s[2], s[3]));
         } else {
             p.cos_out[at] = c[0];
             p.sin_out[at] = s[0];
@@ -376,7 +387,7 @@ extern "C" int ltx_rope_table(ltx_ctx *ctx, const int32_t *pos_dev, int32_t rows
     for (int b = 0; b < 8; ++b) p.powers[b] = std::pow(theta, -(double)(1 << b) / p.half);
     const bool vec = p.half % 4 == 0 && !(((uintptr_t)cos_dev | (uintptr_t)sin_dev) & 15);
     const int at_once = 256 / (vec ? p.half / 4 : p.half);
-    const int grid = std::min((rows + at_once - 1) / at_once, ctx->sm_count * 8);
+    const int grid = std::min((rows + at_once - 1) / at_once, ctx->sm_count * 6);   // all at once
     if (vec) rope_table_1d_kernel<4><<<grid, 256, 0, ctx->stream>>>(p);
     else rope_table_1d_kernel<1><<<grid, 256, 0, ctx->stream>>>(p);
     const cudaError_t e = cudaGetLastError();
