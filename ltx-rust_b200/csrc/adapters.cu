@@ -1142,13 +1142,17 @@ cudaError_t run_pair(const ltx_ctx *ctx, AdapterParams p, int epilogue, const CU
     }
 }
 
-// Tokens of a tile: the least that holds them all up to 256; above, 256 (the
-// fewest bytes per product), but three tiles of 128 where two of 256 would be
-// a third empty.
-int tokens_for(int m) {
-    for (int t = 16; t < 256; t *= 2)
-        if (m <= t) return t;
-    return m > 256 && m <= 384 ? 128 : 256;
+// Tokens of a tile.  Up to 64: the least that holds them all, so that the weights
+// stream once.  More: the widest tile (the fewest bytes per product) that still
+// makes work for two SMs in five; a cluster's joined sums and a builder's wider
+// copies cost more than they save below that.  Measured, us at 256 / 128 / 64 / 32 /
+// 16 tokens: 153 x 600 x 448 50 / 34 / 22 / 16 / 13; 512 x 1024 x 2048 41 / 21 / 18 /
+// 23 / 31; 200 x 4096 x 4096 27.6 / 27.3 / 29 / 44 / 64; 512 x 4096 x 4096 37 / 39 / 47 / 76.
+int tokens_for(int m, int n, int sms) {
+    if (m <= 64) return m <= 16 ? 16 : m <= 32 ? 32 : 64;
+    for (int t = 256; t > 16; t /= 2)
+        if ((int64_t)((m + t - 1) / t) * ((n + BM - 1) / BM) * 5 >= sms * 2) return t;
+    return 16;
 }
 
 }  // namespace
@@ -1197,7 +1201,7 @@ extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args) {
     p.ld_gate = ld_gate;
     p.out = out_dev;
     p.flag = ctx->timeout_flag;
-    const int tn = tokens_for(m), tl = std::min(tn, 64);
+    const int tn = tokens_for(m, n, ctx->sm_count), tl = std::min(tn, 64);
     // enough 256 x 256 tiles for every pair of SMs
     const bool pair = tn == 256 && (int64_t)((m + 255) / 256) * ((n + 255) / 256) * 2 > ctx->sm_count;
     CUtensorMap tw, tx, txl, ta, tb;

@@ -349,7 +349,8 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_tmem, uint32_t o_tmem, c
     // packed 16-bit pairs (key 2c in the low half of column c) into columns
     // 64..127 of S_t, which pass 1 has read.  A row that has seen no key yet has
     // m_ref = -inf and P = 2^-inf = 0.  Masked tiles take no polynomial: it
-    // does not go to 0.
+    // does not go to 0.  bf16: the sum takes P as the product takes it, so a row
+    // that one key rules is exact (f16's rounding is a sixteenth of the output's).
     const float base = m_ref == -INFINITY ? 0.f : -m_ref;
     const float2 nm2 = make_float2(base, base);
     float2 sum2 = make_float2(0.f, 0.f);
@@ -360,8 +361,8 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_tmem, uint32_t o_tmem, c
             const float2 s = make_float2(__uint_as_float(r[2 * u]), __uint_as_float(r[2 * u + 1]));
             const float2 x = MODE == kPlain ? __ffma2_rn(s, rs.sc, nm2) : __fadd2_rn(s, nm2);
             const float2 pf = decltype(with_poly)::value && ((kPolyPairs<D> >> u) & 1u) ? exp2_poly2(x) : make_float2(ex2(x.x), ex2(x.y));
-            sum2 = __fadd2_rn(sum2, pf);
             pk[u] = pack16<VF16>(pf);
+            sum2 = __fadd2_rn(sum2, VF16 ? pf : unpack_bf16(pk[u]));
         }
         tmem_st_32x32b_x16(s_tmem + col, pk);
     };
@@ -402,8 +403,8 @@ __device__ __forceinline__ void softmax_tile_fixed(uint32_t s_tmem, const RowSco
 #pragma unroll
         for (int u = 0; u < 16; ++u) {
             const float2 pf = make_float2(ex2(__uint_as_float(r[2 * u])), ex2(__uint_as_float(r[2 * u + 1])));
-            sum2 = __fadd2_rn(sum2, pf);
             pk[u] = pack16<false>(pf);
+            sum2 = __fadd2_rn(sum2, unpack_bf16(pk[u]));
         }
         tmem_st_32x32b_x16(s_tmem + col, pk);
     };

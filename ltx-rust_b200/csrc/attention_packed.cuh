@@ -99,6 +99,10 @@ __device__ __forceinline__ uint32_t pack16(float2 v) {
     return r;
 }
 
+__device__ __forceinline__ float2 unpack_bf16(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
 // attention_packed_few.cu: few query rows per document, as rows_per_doc counts
 // them (heads of a group included).  Enqueues the attention and the join of
 // what several CTAs share.

@@ -457,10 +457,16 @@ __global__ void __launch_bounds__(kFewThreads, 1)
                         const int r = r4 + e;
                         // a row that has seen no key has reference -inf and all of its scores too
                         const float v = ex2(y[r] - (refs[e] == -INFINITY ? 0.f : refs[e]));
-                        l[r] += v;
                         unsigned char *to = pw + r * 128 + ((chunk ^ (r & 7)) << 4);
-                        if constexpr (VF16) *reinterpret_cast<__half *>(to) = __float2half_rn(v);
-                        else *reinterpret_cast<__nv_bfloat16 *>(to) = __float2bfloat16_rn(v);
+                        // the sum takes what the product takes: a row that one key rules is exact
+                        if constexpr (VF16) {
+                            l[r] += v;
+                            *reinterpret_cast<__half *>(to) = __float2half_rn(v);
+                        } else {
+                            const __nv_bfloat16 h = __float2bfloat16_rn(v);
+                            l[r] += __bfloat162float(h);
+                            *reinterpret_cast<__nv_bfloat16 *>(to) = h;
+                        }
                     }
                 }
                 // V rows behind the document's end: P is 0 there, but 0 times another document's NaN is not
@@ -541,6 +547,7 @@ __global__ void __launch_bounds__(128) few_join_kernel(PackedParams p, Partials 
     __shared__ Place s_place;
     __shared__ int64_t s_per;
     __shared__ int s_go;
+    __shared__ float s_acc[4][D + 1];
     const int c = blockIdx.x + 1, lane = threadIdx.x & 31;
     if (threadIdx.x < 32) {
         int64_t per, left;
@@ -564,20 +571,38 @@ __global__ void __launch_bounds__(128) few_join_kernel(PackedParams p, Partials 
     const int more = (int)((d.tiles - s_place.tile + s_per - 1) / s_per);
     grid_dep_wait();
     const int rows = min(p.tile_tokens, d.lq - token0) * p.group;
-    for (int r = threadIdx.x / 32; r < rows; r += 4) {   // a warp per row
-        auto slot = [&](int i) { return i == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + i); };
-        float top = -INFINITY;
-        for (int i = lane; i <= more; i += 32) top = fmaxf(top, part.ml[(int64_t)slot(i) * N + r].x);
+    // A warp per row, or all four on each row in turn where many CTAs share the
+    // item: then each takes every fourth partial, and warp 0 adds the four up.
+    const int warp = threadIdx.x / 32, share = more >= 4 ? 4 : 1;
+    auto slot = [&](int i) { return (int64_t)(i == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + i)); };
+    for (int r = share == 4 ? 0 : warp; r < rows; r += share == 4 ? 1 : 4) {
+        float top = -INFINITY, total = 0.f, acc[D / 32] = {};
+        for (int i = lane; i <= more; i += 32) top = fmaxf(top, part.ml[slot(i) * N + r].x);
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float total = 0.f, acc[D / 32] = {};
-        for (int i = 0; i <= more; ++i) {
-            const float2 ml = part.ml[(int64_t)slot(i) * N + r];
+#pragma unroll 4
+        for (int i = share == 4 ? warp : 0; i <= more; i += share) {
+            const float2 ml = part.ml[slot(i) * N + r];
+            const float *o = part.o + (slot(i) * N + r) * D + lane;
             const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
             total += ml.y * f;
-            const float *o = part.o + ((int64_t)slot(i) * N + r) * D + lane;
 #pragma unroll
-            for (int x = 0; x < D / 32; ++x) acc[x] += f == 0.f ? 0.f : o[x * 32] * f;
+            for (int x = 0; x < D / 32; ++x) {
+                const float v = o[x * 32];
+                acc[x] += f == 0.f ? 0.f : v * f;
+            }
+        }
+        if (share == 4) {
+            __syncthreads();
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) s_acc[warp][x * 32 + lane] = acc[x];
+            if (lane == 0) s_acc[warp][D] = total;
+            __syncthreads();
+            if (warp != 0) continue;
+            total = s_acc[0][D] + s_acc[1][D] + s_acc[2][D] + s_acc[3][D];
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x)
+                acc[x] = s_acc[0][x * 32 + lane] + s_acc[1][x * 32 + lane] + s_acc[2][x * 32 + lane] + s_acc[3][x * 32 + lane];
         }
         __nv_bfloat16 *out =
             p.out + (int64_t)(d.qs + token0 + r / p.group) * p.ldo + (kvh * p.group + r % p.group) * D + lane;

@@ -238,6 +238,15 @@ def test_gemm_adapters_many_tokens(ctx, m, n, k, rank, adapters, lengths, epi):
     adapter_case(ctx, m, n, k, rank, runs(m, lengths, adapters, start=1), epi, adapters, bias=m % 2 == 0, gate=2)
 
 
+@pytest.mark.parametrize("epi", [1, 3])
+@pytest.mark.parametrize("m,n,k,rank,adapters,lengths", [
+    (100, 16000, 64, 16, 2, [60]), (129, 16000, 136, 72, 3, [40, 1]), (250, 4500, 512, 32, 4, [1, 90]),
+    (300, 5120, 1024, 64, 3, [128]), (400, 8300, 256, 16, 20, [1, 2, 3]), (90, 4200, 2048, 128, 5, [20])])
+def test_gemm_adapters_every_tile_width(ctx, m, n, k, rank, adapters, lengths, epi):
+    """Sizes for which tiles of 64 to 256 tokens are taken, alone and shared by a cluster."""
+    adapter_case(ctx, m, n, k, rank, runs(m, lengths, adapters, start=1), epi, adapters, bias=True, gate=1)
+
+
 @pytest.mark.parametrize("epi", [0, 3])
 def test_gemm_adapters_strides_and_odd_rows(ctx, epi):
     adapter_case(ctx, 45, 77, 96, 16, runs(45, [4, 9], 3), epi, 3, x_pad=8, o_pad=3)
