@@ -210,7 +210,10 @@ struct RowScores {
             float big = 0.f;
 #pragma unroll
             for (int u = 0; u < 16; ++u) big = fmaxf(big, fmaxf(fabsf(v[u].x), fabsf(v[u].y)));
-            if (!__any_sync(0xffffffffu, big > 1.f)) {
+            if (!__any_sync(0xffffffffu, big > 0.5f)) {
+#pragma unroll
+                for (int u = 0; u < 16; ++u) v[u] = __fmul2_rn(tanh_small2(v[u]), make_float2(cap2, cap2));
+            } else if (!__any_sync(0xffffffffu, big > 1.f)) {
 #pragma unroll
                 for (int u = 0; u < 16; ++u) v[u] = __fmul2_rn(tanh_poly2(v[u]), make_float2(cap2, cap2));
             } else {   // tanh(u) = 1 - 2 / (2^(2u log2e) + 1): right at both ends
@@ -245,9 +248,10 @@ struct RowScores {
 
 // Of a row's 16 pairs of exponentials per 32 keys, those computed on the FMA pipe
 // (exp2_poly2): the special-function unit alone, at 6 cycles a warp, is as busy as
-// the tensor cores at head_dim 128 and busier at 64.
-template <int D>
-constexpr uint32_t kPolyPairs = D == 128 ? 0x1111u : 0x5555u;
+// the tensor cores at head_dim 128 and busier at 64.  A quarter of them: 768 us at
+// 8192 x 32 x 64, 817 with half, 887 with none (head_dim 128 differs by less than
+// its runs do).
+constexpr uint32_t kPolyPairs = 0x1111u;
 
 // One row's 128 scores of a K/V tile: S from TMEM, the row's maximum, P back
 // into TMEM, the row's sum.  `left` keys are the row's to see (`masked`: some row
@@ -349,8 +353,8 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_tmem, uint32_t o_tmem, c
     // packed 16-bit pairs (key 2c in the low half of column c) into columns
     // 64..127 of S_t, which pass 1 has read.  A row that has seen no key yet has
     // m_ref = -inf and P = 2^-inf = 0.  Masked tiles take no polynomial: it
-    // does not go to 0.  bf16: the sum takes P as the product takes it, so a row
-    // that one key rules is exact (f16's rounding is a sixteenth of the output's).
+    // does not go to 0.  The sum takes P before its rounding to 16 bits, at most half
+    // a step of V's type for each key: taking the rounded P costs 3 to 5%.
     const float base = m_ref == -INFINITY ? 0.f : -m_ref;
     const float2 nm2 = make_float2(base, base);
     float2 sum2 = make_float2(0.f, 0.f);
@@ -360,9 +364,9 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_tmem, uint32_t o_tmem, c
         for (int u = 0; u < 16; ++u) {
             const float2 s = make_float2(__uint_as_float(r[2 * u]), __uint_as_float(r[2 * u + 1]));
             const float2 x = MODE == kPlain ? __ffma2_rn(s, rs.sc, nm2) : __fadd2_rn(s, nm2);
-            const float2 pf = decltype(with_poly)::value && ((kPolyPairs<D> >> u) & 1u) ? exp2_poly2(x) : make_float2(ex2(x.x), ex2(x.y));
+            const float2 pf = decltype(with_poly)::value && ((kPolyPairs >> u) & 1u) ? exp2_poly2(x) : make_float2(ex2(x.x), ex2(x.y));
+            sum2 = __fadd2_rn(sum2, pf);
             pk[u] = pack16<VF16>(pf);
-            sum2 = __fadd2_rn(sum2, VF16 ? pf : unpack_bf16(pk[u]));
         }
         tmem_st_32x32b_x16(s_tmem + col, pk);
     };
@@ -388,7 +392,9 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_tmem, uint32_t o_tmem, c
     tc_fence_before();          // ... and ordered before the arrive for the MMA thread
 }
 
-// The same for kCapFixed: P = 2^score, 32 keys at a time.
+// The same for kCapFixed: P = 2^score, 32 keys at a time.  The sum takes P as the
+// product takes it, rounded: here a row's largest P is no power of two, and one
+// that a single key rules would otherwise carry that rounding into its output.
 __device__ __forceinline__ void softmax_tile_fixed(uint32_t s_tmem, const RowScores<kCapFixed> &rs, int left, bool masked,
                                                    float &m_ref, float &l) {
     float2 sum2 = make_float2(0.f, 0.f);

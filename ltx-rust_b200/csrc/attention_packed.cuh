@@ -76,8 +76,8 @@ __device__ __forceinline__ float2 exp2_poly2(float2 x) {
                        __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(t.y) << 23)));
 }
 
-// tanh(u) for |u| <= 1, two at a time: u q(u^2), q of degree 5 fitted here to the
-// least absolute error of tanh (3.0e-7).
+// tanh(u), two at a time: u q(u^2), q fitted here to the least absolute error of
+// tanh: for |u| <= 1 of degree 5 (3.0e-7), for |u| <= 1/2 of degree 3 (1.5e-7).
 __device__ __forceinline__ float2 tanh_poly2(float2 u) {
     constexpr float t0 = 0x1.ffff96p-1f, t1 = -0x1.553ce0p-2f, t2 = 0x1.0f6ea4p-3f, t3 = -0x1.a191d8p-5f,
                     t4 = 0x1.0803c6p-6f, t5 = -0x1.742ca4p-9f;
@@ -87,6 +87,14 @@ __device__ __forceinline__ float2 tanh_poly2(float2 u) {
     q = __ffma2_rn(q, z, make_float2(t2, t2));
     q = __ffma2_rn(q, z, make_float2(t1, t1));
     q = __ffma2_rn(q, z, make_float2(t0, t0));
+    return __fmul2_rn(q, u);
+}
+__device__ __forceinline__ float2 tanh_small2(float2 u) {
+    constexpr float h0 = 0x1.ffffb2p-1f, h1 = -0x1.55341ap-2f, h2 = 0x1.0d366cp-3f, h3 = -0x1.634eb0p-5f;
+    const float2 z = __fmul2_rn(u, u);
+    float2 q = __ffma2_rn(make_float2(h3, h3), z, make_float2(h2, h2));
+    q = __ffma2_rn(q, z, make_float2(h1, h1));
+    q = __ffma2_rn(q, z, make_float2(h0, h0));
     return __fmul2_rn(q, u);
 }
 
