@@ -293,9 +293,10 @@ int ltx_attention_fwd(ltx_ctx *ctx, const void *q_dev, int64_t ldq, const void *
  * mask = None (crates/ltx-dit/src/attention.rs:228-285).  All of them are
  * inference operators, take caller-owned buffers on the context's device,
  * set the context's device for the call and restore the caller's, and may be
- * captured into a CUDA graph.  Index arrays on the device are read as they
- * are: every access they lead to stays inside the buffers whatever they hold,
- * and a bad value is reported by the next ltx_ctx_synchronize. */
+ * captured into a CUDA graph.  Outputs overlap no input unless said otherwise.
+ * Index arrays on the device are read as they are: every access they lead to
+ * stays inside the buffers whatever they hold, and a bad value is reported by
+ * the next ltx_ctx_synchronize. */
 
 /* Which two values of a head's rotated part form a pair. */
 typedef enum {
@@ -311,8 +312,9 @@ typedef enum {
  *   cos_dev[r][i] = amplitude cos(pos[r] g_i), sin_dev the same.
  * factor 1 is the plain table; a larger one stretches every frequency, or
  * with original_len only those that turn fewer than turns_high times over it.
- * pos_dev int32 [rows], NULL = 0, 1, 2, ...  The angle is formed and reduced
- * in f64, so far positions keep f32's accuracy.  rot_dim even, 2..512. */
+ * pos_dev int32 [rows], NULL = 0, 1, 2, ...  Frequencies are formed in f64
+ * and angles as 64-bit fractions of a turn, so far positions keep f32's
+ * accuracy.  rot_dim even, 2..512. */
 int ltx_rope_table(ltx_ctx *ctx, const int32_t *pos_dev, int32_t rows, int32_t rot_dim, double theta, double factor,
                    int64_t original_len, double turns_low, double turns_high, double amplitude, float *cos_dev,
                    float *sin_dev);
@@ -354,10 +356,18 @@ int ltx_qk_norm_rope(ltx_ctx *ctx, const ltx_norm_rope *args);
  *   padded with zero rows of A (or zero columns of B).  rank a multiple of 8
  *   up to LTX_MAX_ADAPTER_RANK, at most LTX_MAX_ADAPTERS adapters.
  * x, W, epilogue, bias, gate and out as ltx_gemm_bf16 (x/W rows 16-byte
- * aligned, k a multiple of 8; out and gate rows of any alignment).  The
- * low-rank sums stay in f32; for the f32 epilogues the product with B is
- * taken in two bf16 parts that together keep 16 bits of it.  Scratch comes
- * from the context's pool in stream order. */
+ * aligned, k a multiple of 8 up to 2^24; out and gate rows of any alignment);
+ * a gate index outside [0, gate_rows) takes the nearest row and is reported
+ * the same way.  With adapters 0 the adapter indices are not looked at.
+ * Sums are f32, as the tensor cores add (each addition cuts what lies below
+ * f32's last bit: 4e-6 relative at k 4096).  The low-rank sums c x A^T are
+ * rounded to bf16 before the product with B, for the f32 epilogues to two
+ * bf16 parts that together keep 16 bits.  lora_b must be finite: a row of
+ * another adapter takes 0 times its values where both lie in one tile; what
+ * x, lora_a and coeff hold for one row or adapter reaches no other.  A
+ * workspace of 2 bytes x m x rank (rounded up to 64; twice for the f32
+ * epilogues) stays with the context up to 64 MB, comes from its pool in
+ * stream order above, and belongs to the graph in a captured call. */
 #define LTX_MAX_ADAPTERS 1024
 #define LTX_MAX_ADAPTER_RANK 256
 typedef struct {
@@ -369,6 +379,7 @@ typedef struct {
     const float *coeff_dev;
     int64_t ldx, ldw, ldo, ld_gate;
     int32_t m, n, k, epilogue, adapters, rank;
+    int32_t gate_rows;                                    /* rows of gate_dev                                            */
 } ltx_adapter_gemm;
 int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args);
 
@@ -390,7 +401,10 @@ int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args);
  * dimensions in elements (multiples of 8, 16-byte aligned bases); head_dim 64
  * or 128; out overlaps no input.  What k and v hold outside the documents, or
  * in other documents, never reaches a row, NaN and infinities included; a
- * non-finite v row inside a document may reach every row of the document. */
+ * non-finite v row inside a document may reach every row of the document.
+ * At most 2^29 rows.  Under a cap without slopes (bf16 v, softcap up to 51)
+ * probabilities are kept unnormalised up to e^softcap, so sums over a row of
+ * |v| have to stay under 2^52. */
 typedef struct {
     const void *q_dev, *k_dev, *v_dev;
     void *out_dev;

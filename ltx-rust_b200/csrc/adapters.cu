@@ -30,6 +30,7 @@ constexpr int kMaxWords = LTX_MAX_ADAPTERS / 32;
 
 struct AdapterParams {
     int m, n, k, rank, adapters, rank_blocks, parts, splits, m_tiles, n_tiles, group_m;
+    int gate_rows;
     int tile_lanes, unit, low_stages;   // low_kernel: clusters per tile, adapters in one product, depth of its ring
     const int *idx, *gate_idx;
     const float *coeff, *bias, *gate;
@@ -390,9 +391,14 @@ struct Ahead {
         }
     }
 };
-// The gate rows of tokens m + lane.
-__device__ __forceinline__ int gate_rows(const AdapterParams &p, int m, int lane) {
-    return p.gate && p.gate_idx && m + lane < p.m ? __ldg(p.gate_idx + m + lane) : 0;
+// The gate rows of tokens m + lane.  One outside the gate takes its nearest and raises the flag.
+__device__ __forceinline__ int gate_row(const AdapterParams &p, int m, int lane) {
+    int g = p.gate && p.gate_idx && m + lane < p.m ? __ldg(p.gate_idx + m + lane) : 0;
+    if ((unsigned)g >= (unsigned)p.gate_rows && p.gate) {
+        atomicExch(p.flag, kErrBadGate);
+        g = g < 0 ? 0 : p.gate_rows - 1;
+    }
+    return g;
 }
 
 // 16 tokens from m on (count of them inside), weight row n of this thread; a
@@ -427,7 +433,7 @@ struct TileEpilogue {
     int gidx = 0;
     __device__ __forceinline__ void begin(const AdapterParams &p, int m0, int tokens, int n, int side, int lane) {
         if (EPI == LTX_EPI_RESID && side < tokens) {
-            gidx = gate_rows(p, m0 + side, lane);
+            gidx = gate_row(p, m0 + side, lane);
             next.fetch(p, m0 + side, tokens - side, n, gidx, 0);
         }
     }
@@ -438,7 +444,7 @@ struct TileEpilogue {
             uint32_t r[32];
             tmem_ld_32x32b_x32(acc + c, r);
             int gnext = 0;
-            if (EPI == LTX_EPI_RESID && c + 64 < tokens) gnext = gate_rows(p, m0 + c + 64, lane);
+            if (EPI == LTX_EPI_RESID && c + 64 < tokens) gnext = gate_row(p, m0 + c + 64, lane);
             tmem_ld_wait_regs(r);
 #pragma unroll
             for (int h = 0; h < 32; h += 16) {
@@ -728,7 +734,7 @@ __global__ void __launch_bounds__(kProjThreads, 1)
                 const int m = mt * TN + split * per + j0, count = min(per - j0, p.m - m);
                 if (count <= 0) break;
                 Ahead h;
-                if (EPI == LTX_EPI_RESID) h.fetch(p, m, count, n, gate_rows(p, m, lane), 0);
+                if (EPI == LTX_EPI_RESID) h.fetch(p, m, count, n, gate_row(p, m, lane), 0);
                 float v[16], half[8];
 #pragma unroll
                 for (int q = 0; q < 16; q += 8) {
@@ -1165,10 +1171,11 @@ extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args) {
     const char *w = "gemm_adapters";
     if (!args) return fail(ctx, LTX_ERR_INVALID_ARG, "%s: null arguments", w);
     const auto &[x_dev, w_dev, out_dev, bias_dev, gate_dev, gate_idx_dev, adapter_idx_dev, lora_a_dev, lora_b_dev, coeff_dev,
-                 ldx, ldw, ldo, ld_gate, m, n, k, epilogue, adapters, rank] = *args;
+                 ldx, ldw, ldo, ld_gate, m, n, k, epilogue, adapters, rank, gate_rows] = *args;
     if (epilogue < LTX_EPI_BF16 || epilogue > LTX_EPI_RESID)
         return fail(ctx, LTX_ERR_INVALID_ARG, "%s: bad epilogue %d", w, epilogue);
-    if (m < 0 || n < 1 || k < 1 || k > 1 << 24) return fail(ctx, LTX_ERR_SHAPE, "%s: %d x %d x %d", w, m, n, k);
+    if (m < 0 || n < 1 || k < 1 || k > 1 << 24 || m > 1 << 30 || n > 1 << 30)
+        return fail(ctx, LTX_ERR_SHAPE, "%s: %d x %d x %d", w, m, n, k);
     if (adapters < 0 || adapters > LTX_MAX_ADAPTERS || rank < 8 || rank > LTX_MAX_ADAPTER_RANK || rank % 8)
         return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: %d adapters of rank %d (at most %d, rank a multiple of 8 up to %d)", w,
                     adapters, rank, LTX_MAX_ADAPTERS, LTX_MAX_ADAPTER_RANK);
@@ -1179,8 +1186,8 @@ extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args) {
         (((uintptr_t)x_dev | (uintptr_t)w_dev | (uintptr_t)lora_a_dev | (uintptr_t)lora_b_dev) & 15))
         return fail(ctx, LTX_ERR_SHAPE, "%s: operand rows must be 16-byte aligned (k %d, ldx %lld, ldw %lld)", w, k,
                     (long long)ldx, (long long)ldw);
-    if (epilogue == LTX_EPI_RESID && gate_dev && ld_gate < n)
-        return fail(ctx, LTX_ERR_SHAPE, "%s: gate rows shorter than n", w);
+    if (epilogue == LTX_EPI_RESID && gate_dev && (ld_gate < n || gate_rows < 1))
+        return fail(ctx, LTX_ERR_SHAPE, "%s: %d gate rows of %lld, shorter than n or none", w, gate_rows, (long long)ld_gate);
     DeviceGuard guard(ctx);
     if ((int64_t)adapters * n > 0x7fffffff || (int64_t)((m + 15) / 16) * ((n + BM - 1) / BM) > 0x7fffffff / 8)
         return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: %d x %d with %d adapters is too large", w, m, n, adapters);
@@ -1197,6 +1204,7 @@ extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args) {
     p.coeff = coeff_dev;
     p.bias = bias_dev;
     p.gate = gate_dev;
+    p.gate_rows = gate_rows;
     p.ldo = ldo;
     p.ld_gate = ld_gate;
     p.out = out_dev;

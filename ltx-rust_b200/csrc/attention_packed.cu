@@ -74,11 +74,12 @@ struct Smem {
 
 // The pair-th pair of query tiles over all documents, found by one warp; false
 // when there are fewer.  A causal document's last tiles have the most keys and
-// go first.
-__device__ __forceinline__ bool find_item(const PackedParams &p, int pair, int lane, Item &it) {
+// go first.  `base`, `before`: where the last search ended (32 documents from
+// base, `before` pairs ahead of them); one for a later pair goes on from there.
+__device__ __forceinline__ bool find_item(const PackedParams &p, int pair, int lane, int &base, int &before, Item &it) {
     const int per = 2 * p.tile_tokens;
-    int before = 0;
-    for (int base = 0; base < p.docs; base += 32) {
+    if (pair < before) base = before = 0;
+    for (; base < p.docs; base += 32) {
         int s = 0, e = 0;
         if (base + lane < p.docs) doc_span(p.qo, base + lane, p.rows_q, p.flag, s, e);
         const int n = (e - s + per - 1) / per;
@@ -180,7 +181,7 @@ struct Share {
 // domain, with bf16 V: 2^score fits f32 and bf16 as it is, so no maximum is kept
 // and the scores are gone through once.
 enum Mode { kPlain = 0, kBias = 1, kCap = 2, kCapFixed = 3 };
-constexpr float kFixedCap = 100.f;   // 2^100 by 2^29 keys stays within f32
+constexpr float kFixedCap = 75.f;   // 2^75 by 2^29 keys by values of 2^23 stay within f32
 
 // Scores of one row in the log2 domain.  The scale goes with the log2e, and the
 // bias is linear on either side of the key the row stands beside, so a tile that
@@ -490,6 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == 0) {
         uint32_t issued = 0, n_items = 0, n_q = 0, n_asked = 0;
+        int base = 0, before = 0;
         int i = blockIdx.x / p.splits;
         // The next item, asked for when the loads of the one at hand are issued
         // (the ring holds a few microseconds of products then): earlier, a CTA
@@ -510,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             Item it{};
             bool more = false;
             while (i >= 0) {
-                if ((more = find_item(p, i % p.pairs, lane, it))) break;
+                if ((more = find_item(p, i % p.pairs, lane, base, before, it))) break;
                 i = next();
             }
             it.kvh = more ? i / p.pairs : -1;   // -1: no more
@@ -894,6 +896,9 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const ltx_packed_attention
     if (heads / kv_heads > 128) return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: more than 128 heads per key head", w);
     if (!(scale > 0.f) || !std::isfinite(scale) || !(softcap >= 0.f) || !std::isfinite(softcap))
         return fail(ctx, LTX_ERR_INVALID_ARG, "%s: scale must be finite and > 0, softcap finite and >= 0", w);
+    if (!std::isfinite(scale * kLog2e) || !std::isfinite(softcap * kLog2e) ||
+        (softcap > 0.f && (!std::isfinite(scale / softcap) || !std::isfinite(2.f * kLog2e / softcap))))
+        return fail(ctx, LTX_ERR_INVALID_ARG, "%s: scale, softcap or their quotient leaves f32", w);
     if (prefix_dev && !causal) return fail(ctx, LTX_ERR_INVALID_ARG, "%s: a prefix needs the causal mask", w);
     if (docs == 0 || rows_q == 0) return LTX_OK;
     if (!q_dev || !out_dev || !q_offsets_dev || !k_offsets_dev || (rows_k && (!k_dev || !v_dev)))

@@ -75,7 +75,11 @@ cudaError_t allow_smem(const ltx_ctx *ctx, const void *kernel, int bytes) {
     const std::lock_guard<std::mutex> hold(lock);
     if (done.count({kernel, ctx->device})) return cudaSuccess;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess) done.insert({kernel, ctx->device});
+    if (e != cudaSuccess) return e;
+    try {
+        done.insert({kernel, ctx->device});
+    } catch (const std::bad_alloc &) {   // asked again next time
+    }
     return e;
 }
 
@@ -169,6 +173,8 @@ extern "C" int ltx_ctx_synchronize(ltx_ctx *ctx) {
             return ltx::fail(ctx, LTX_ERR_INVALID_ARG, "qk_norm_rope: a position lies outside the cos/sin tables");
         if (flag == ltx::kErrBadAdapter)
             return ltx::fail(ctx, LTX_ERR_INVALID_ARG, "gemm_adapters: an adapter index lies beyond the pool");
+        if (flag == ltx::kErrBadGate)
+            return ltx::fail(ctx, LTX_ERR_INVALID_ARG, "gemm_adapters: a gate index lies outside the gate's rows");
         if (flag == ltx::kErrBadOffsets)
             return ltx::fail(ctx, LTX_ERR_INVALID_ARG,
                              "attention_packed: document offsets descend or lie outside the rows");

@@ -106,14 +106,19 @@ inline int cuda_fail(ltx_ctx *ctx, cudaError_t e, const char *what) {
 }
 
 // Makes the context's device current for the scope and puts the caller's back
-// (a launch on the default stream goes to the current device).
+// (a launch on the default stream goes to the current device).  Meanwhile calls
+// that a strict capture forbids its thread, as loading a kernel and making a
+// pool, are allowed: none of them touches the captured stream.
 struct DeviceGuard {
     int prev = -1;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
     explicit DeviceGuard(const ltx_ctx *ctx) {
         if (cudaGetDevice(&prev) != cudaSuccess || prev == ctx->device) prev = -1;
         if (prev >= 0) cudaSetDevice(ctx->device);
+        cudaThreadExchangeStreamCaptureMode(&mode);
     }
     ~DeviceGuard() {
+        cudaThreadExchangeStreamCaptureMode(&mode);
         if (prev >= 0) cudaSetDevice(prev);
     }
     DeviceGuard(const DeviceGuard &) = delete;

@@ -109,6 +109,7 @@ constexpr int kErrTooManyTimesteps = 1001;   // device error code: more distinct
 // LTX_ERR_INVALID_ARG by ltx_ctx_synchronize.
 constexpr int kErrBadPosition = 1002;   // a rotary position outside its table
 constexpr int kErrBadAdapter = 1003;    // an adapter index beyond the pool
+constexpr int kErrBadGate = 1005;       // a gate index outside the gate's rows
 constexpr int kErrBadOffsets = 1004;    // document offsets that descend or leave the buffer
 cudaError_t timestep_set(cudaStream_t st, const float *ts, int64_t rows, int umax, float *ts_u, int *idx, int *flag,
                          int code);

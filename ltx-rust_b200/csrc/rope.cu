@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_vec_kernel(NormRopeParams p)
 template <typename T, int LANES>
 void launch_vec(const NormRopeParams &p, cudaStream_t st) {
     constexpr int kHeads = 32 / LANES * kHeadsDeep;
-    const dim3 grid((unsigned)((p.rows + 7) / 8), (unsigned)((p.heads + kHeads - 1) / kHeads + (p.kv_heads + kHeads - 1) / kHeads));
+    const dim3 grid((unsigned)(((int64_t)p.rows + 7) / 8), (unsigned)((p.heads + kHeads - 1) / kHeads + (p.kv_heads + kHeads - 1) / kHeads));
     if (p.interleaved) qk_norm_rope_vec_kernel<T, LANES, true><<<grid, 256, 0, st>>>(p);
     else qk_norm_rope_vec_kernel<T, LANES, false><<<grid, 256, 0, st>>>(p);
 }
@@ -374,7 +374,7 @@ extern "C" int ltx_rope_table(ltx_ctx *ctx, const int32_t *pos_dev, int32_t rows
     if (!ctx) return LTX_ERR_INVALID_ARG;
     if (rows < 0 || rot_dim < 2 || rot_dim > kMaxRot || rot_dim % 2)
         return fail(ctx, LTX_ERR_SHAPE, "rope_table: %d rows, rot_dim %d (even, 2..%d)", rows, rot_dim, kMaxRot);
-    if (!(theta > 0) || !std::isfinite(theta) || !(factor > 0) || !std::isfinite(factor) || !std::isfinite(amplitude) ||
+    if (!(theta > 0) || !std::isfinite(theta) || !(factor > 0) || !std::isfinite(factor) || !std::isfinite((float)amplitude) ||
         original_len < 0)
         return fail(ctx, LTX_ERR_INVALID_ARG, "rope_table: theta and factor must be finite and > 0, original_len >= 0");
     if (original_len > 0 && !(turns_high > turns_low && std::isfinite(turns_high) && std::isfinite(turns_low)))
@@ -387,7 +387,7 @@ extern "C" int ltx_rope_table(ltx_ctx *ctx, const int32_t *pos_dev, int32_t rows
     for (int b = 0; b < 8; ++b) p.powers[b] = std::pow(theta, -(double)(1 << b) / p.half);
     const bool vec = p.half % 4 == 0 && !(((uintptr_t)cos_dev | (uintptr_t)sin_dev) & 15);
     const int at_once = 256 / (vec ? p.half / 4 : p.half);
-    const int grid = std::min((rows + at_once - 1) / at_once, ctx->sm_count * 6);   // all at once
+    const int grid = (int)std::min<int64_t>(((int64_t)rows + at_once - 1) / at_once, ctx->sm_count * 6);   // all at once
     if (vec) rope_table_1d_kernel<4><<<grid, 256, 0, ctx->stream>>>(p);
     else rope_table_1d_kernel<1><<<grid, 256, 0, ctx->stream>>>(p);
     const cudaError_t e = cudaGetLastError();

@@ -268,7 +268,7 @@ ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 # The arguments of the packed-batch calls as the header's structs lay them out (ltx_norm_rope, ltx_adapter_gemm,
 # ltx_packed_attention): packed in one step, a tenth of the time ctypes takes for as many single ones.
 _NORM_ROPE = struct.Struct("@9P4q9if")
-_ADAPTER_GEMM = struct.Struct("@10P4q6i")
+_ADAPTER_GEMM = struct.Struct("@10P4q7i")
 _PACKED_ATTENTION = struct.Struct("@8P4q8i2f")
 
 
@@ -344,6 +344,8 @@ def qk_norm_rope(ctx: "Context", q, k, q_out, k_out, heads, kv_heads, cos, sin, 
         gq = _dense(ctx, what, "gamma_q", gamma_q, f32, (d,))
     if gamma_k is not None:
         gk = _dense(ctx, what, "gamma_k", gamma_k, f32, (d,))
+    if (cos is None) != (sin is None):
+        raise LtxError(1, f"{what}: cos and sin go together")
     if cos is not None:
         shape = table, half = _matrix(what, "cos", cos)
         cp, sp = _dense(ctx, what, "cos", cos, f32, shape), _dense(ctx, what, "sin", sin, f32, shape)
@@ -381,7 +383,7 @@ def gemm_adapters(ctx: "Context", x, w, out, adapter_idx, lora_a, lora_b, coeff,
         raise LtxError(2, f"{what}: gate has no rows")
     gate_idx = 0 if gate_idx is None else _dense(ctx, what, "gate_idx", gate_idx, i32, (M,))
     rc = lib().ltx_gemm_adapters(ctx.h, _ADAPTER_GEMM.pack(xp, wp, op, bias, gp, gate_idx, ip, ap, bp, cp, ldx, ldw, ldo, ldg, M,
-                                                           N, K, epilogue, n, rank))
+                                                           N, K, epilogue, n, rank, 0 if gate is None else gate.shape[0]))
     if rc:
         ctx.check(rc, "ltx_gemm_adapters")
 

@@ -279,9 +279,32 @@ def test_gemm_adapters_empty_and_index_beyond_the_pool(ctx):
     assert e.value.kind == "INVALID_ARG" and "adapter" in str(e.value)
     assert out[0].tolist() == [64.0 + 64 * 8] * 8 and out[1].tolist() == [64.0] * 8
     empty = a[:0], b[:0], c[:0]
+    ltx_b200.gemm_adapters(ctx, x, w, out, ints([5, 7]), *empty, epilogue=2)   # no adapters: the indices are not looked at
+    ctx.synchronize()
+    out.zero_()
     ltx_b200.gemm_adapters(ctx, x, w, out, ints([-1, -1]), *empty, epilogue=2)
     ctx.synchronize()
     assert bool((out == 64).all())
+
+
+@pytest.mark.parametrize("m,n", [(3, 8), (300, 130), (2500, 4096)])
+def test_gemm_adapters_gate_rows_outside_the_gate(ctx, m, n):
+    """A gate index outside the gate takes its nearest row and is reported; every access stays inside."""
+    import ltx_b200
+    x, w = torch.ones(m, 64, device="cuda", dtype=BF16), torch.ones(n, 64, device="cuda", dtype=BF16)
+    a, b = torch.ones(1, 8, 64, device="cuda", dtype=BF16), torch.ones(1, n, 8, device="cuda", dtype=BF16)
+    rows = torch.arange(1, 4, device="cuda", dtype=F32)[:, None].expand(3, n).contiguous()
+    out, c = torch.zeros(m, n, device="cuda"), torch.ones(1, device="cuda")
+    idx = torch.tensor([-7, 1, 1 << 30, 2, -(1 << 31), 3], dtype=torch.int32, device="cuda").repeat(m // 6 + 1)[:m].contiguous()
+    ltx_b200.gemm_adapters(ctx, x, w, out, ints([-1] * m), a, b, c, epilogue=3, gate=rows, gate_idx=idx)
+    with pytest.raises(ltx_b200.LtxError) as e:
+        ctx.synchronize()
+    assert e.value.kind == "INVALID_ARG" and "gate" in str(e.value)
+    assert torch.equal(out, 64 * rows[idx.clamp(0, 2).long()])
+    out.zero_()
+    ltx_b200.gemm_adapters(ctx, x, w, out, ints([-1] * m), a, b, c, epilogue=3, gate=rows, gate_idx=idx.clamp(0, 2))
+    ctx.synchronize()
+    assert torch.equal(out, 64 * rows[idx.clamp(0, 2).long()])
 
 
 # ── attention_packed ─────────────────────────────────────────────────────────
@@ -411,6 +434,28 @@ def test_attention_packed_cap_and_distance(ctx, shape, cap, slope, causal, d):
 @pytest.mark.parametrize("vt", [BF16, F16])
 def test_attention_packed_few_rows_long_keys(ctx, lq, lk, h, hk, d, kw, vt):
     attention_case(ctx, lq, lk, h, hk, d, vt, **kw)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_packed_many_short_documents(ctx, causal):
+    """More documents than CTAs and than one search sees at once, some without rows or keys."""
+    attention_case(ctx, [(7 * i) % 61 for i in range(900)], [(11 * i) % 83 for i in range(900)], 4, 2, 64, causal=causal)
+
+
+@pytest.mark.parametrize("vt", [BF16, F16])
+def test_attention_packed_one_key_among_millions(ctx, vt):
+    """A row that one key rules by 2^45 keeps that key's value: the sum of millions of others is nothing beside it."""
+    import ltx_b200
+    n, d = 1 << 23, 128
+    q, k = torch.zeros(64 * 2, d, device="cuda", dtype=BF16), torch.zeros(n, d, device="cuda", dtype=BF16)
+    q[:, 0], k[n // 3, 0] = 1.0, 32.0
+    v = torch.ones(n, d, device="cuda", dtype=vt)
+    v[n // 3] = -1.0
+    out = torch.zeros(128, d, device="cuda", dtype=BF16)
+    ltx_b200.attention_packed(ctx, q, k, v, out, ints([0, 128]), ints([0, n]), 1, 1, 1.0)
+    ctx.synchronize()
+    # the others weigh e^-32 2^23 = 1.1e-7; bf16's half step is 2e-3
+    assert bool((out == -1).all())
 
 
 @pytest.mark.parametrize("lq,lk", [([700, 500], [1024, 1500]), ([2], [9000])])
@@ -608,6 +653,29 @@ def test_layer_captured_twice_and_replayed():
     ctx.close()
 
 
+def test_first_calls_of_a_context_captured():
+    """A context whose very first calls are captured, in the strictest capture mode: workspaces and pools come into being
+    under the capture."""
+    import ltx_b200
+    st = torch.cuda.Stream()
+    ctx = ltx_b200.Context(0, st.cuda_stream)
+    s = layer_state(31, [90, 3])
+    keep = s["resid"].clone()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        layer(ctx, s)
+    with torch.cuda.stream(st):
+        g.replay()
+        got = s["resid"].clone()
+        s["resid"].copy_(keep)
+    layer(ctx, s)
+    ctx.synchronize()
+    assert torch.equal(s["resid"], got) and not torch.equal(got, keep)
+    del g
+    ctx.close()
+
+
 # ── refusals of the C entry points ───────────────────────────────────────────
 
 def refused(ctx, kind, fn, *args, **kw):
@@ -636,6 +704,8 @@ def test_refusals(ctx):
     refused(ctx, "INVALID_ARG", L.attention_packed, *ok, 1, 1, float("nan"))
     refused(ctx, "INVALID_ARG", L.attention_packed, *ok, 1, 1, 1.0, softcap=-1.0)
     refused(ctx, "INVALID_ARG", L.attention_packed, *ok, 1, 1, 1.0, prefix=ints([1]))
+    refused(ctx, "INVALID_ARG", L.attention_packed, *ok, 1, 1, 3e38)
+    refused(ctx, "INVALID_ARG", L.attention_packed, *ok, 1, 1, 1.0, softcap=1e-39)
     three = torch.zeros(4, 384, device="cuda", dtype=BF16)
     two = torch.zeros(4, 256, device="cuda", dtype=BF16)
     refused(ctx, "SHAPE", L.attention_packed, three, two, two, three, o, o, 3, 2, 1.0)
@@ -652,5 +722,7 @@ def test_refusals(ctx):
     refused(ctx, "INVALID_ARG", L.gemm_adapters, x, w, y, i, *pool(8), epilogue=7)
     refused(ctx, "SHAPE", L.gemm_adapters, x[:, :60], w[:, :60], y, i, *pool(8, 60))
     gate = torch.zeros(1, 8, device="cuda")
+    refused(ctx, "SHAPE", L.gemm_adapters, x, w, torch.zeros(4, 8, device="cuda"), i, *pool(8), epilogue=3, gate=gate[:0])
+    refused(ctx, "INVALID_ARG", L.rope_table, None, t, t, amplitude=1e39)
     refused(ctx, "DTYPE", L.gemm_adapters, x, w, y, i, *pool(8), epilogue=3, gate=gate)
     ctx.synchronize()

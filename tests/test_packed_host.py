@@ -83,4 +83,5 @@ def test_wrong_shapes_are_refused():
     assert kind_of(L.gemm_adapters, x, w, fake(4, 8), fake(5, dtype=torch.int32), a, b, c) == "SHAPE"
     assert kind_of(L.qk_norm_rope, q, None, fake(4, 64), None, 1, 0, None, None) == "SHAPE"
     t = fake(4, 8, dtype=torch.float32)
+    assert kind_of(L.qk_norm_rope, q, None, q, None, 1, 0, t, None) == "INVALID_ARG"
     assert kind_of(L.rope_table, fake(3, dtype=torch.int32), t, t) == "SHAPE"
