@@ -18,7 +18,7 @@ struct PackedParams {
     int64_t ldo;
     const int *qo, *ko, *prefix;
     const float *slopes;
-    int docs, rows_q, rows_k, kv_heads, group, tile_tokens, causal, pairs, splits;
+    int docs, rows_q, rows_k, kv_heads, group, tile_tokens, causal, pairs, splits, head_group;
     float scale, softcap;
     int *flag;
 };
