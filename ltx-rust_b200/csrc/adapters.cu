@@ -320,9 +320,9 @@ __global__ void __launch_bounds__(kLowThreads)
 
 // ── the projection ───────────────────────────────────────────────────────────
 //
-// 11 warps: 0 TMA, 1 MMA, 2-9 epilogue (two accumulators: the epilogue of one
-// tile runs under the next one's products), 10 the builder: it lists each tile's
-// adapters and copies its rows of low, zeros for other adapters' tokens, into
+// 12 warps: 0 TMA, 1 MMA, 2-9 epilogue (two accumulators: the epilogue of one
+// tile runs under the next one's products), 10 and 11 the builders: they list each
+// tile's adapters and copy its rows of low, zeros for other adapters' tokens, into
 // buffers beside the ring while the main blocks are multiplied.
 // Few tiles: a cluster of `splits` CTAs shares a tile's blocks and joins its
 // f32 sums through distributed shared memory in the order of the ranks.
@@ -332,16 +332,15 @@ struct ProjCfg {
     static constexpr int A_BYTES = BM * 128, B_BYTES = TN * 128, STAGE = A_BYTES + B_BYTES;
     // up to 128 tokens: as deep as HBM's latency asks (96 KB and more), and no
     // deeper, so that low_kernel's CTAs run beside these
-    static constexpr int STAGES = TN == 256 ? 4 : TN == 128 ? 3 : TN == 64 ? 4 : TN == 32 ? 6 : 7;
-    static constexpr int BUFS = TN == 256 ? 1 : TN <= 32 ? 4 : 2;   // rows of low
+    static constexpr int STAGES = TN >= 128 ? 3 : TN == 64 ? 4 : TN == 32 ? 6 : 7;
+    static constexpr int BUFS = TN <= 32 ? 4 : 2;   // rows of low
     static constexpr int RING = STAGES * STAGE, BUF = RING, BAR = BUF + BUFS * B_BYTES;
-    static constexpr int LIST = BAR + ((2 * STAGES + 8 + 2 * BUFS) * 8 + 8 + 15) / 16 * 16;
+    static constexpr int LIST = BAR + ((2 * STAGES + 9 + 2 * BUFS) * 8 + 8 + 15) / 16 * 16;
     static constexpr int BYTES = 1024 + LIST + 2 * (int)sizeof(TileList<TN>) + (int)sizeof(ListScratch<TN>);
     static constexpr int ACC = TN < 32 ? 32 : TN, COLS = 2 * ACC;
     static_assert(TN * BM * 4 <= RING, "the f32 partials fit the ring");
     static_assert(BYTES <= 232448, "shared memory exceeds the per-CTA limit");
 };
-constexpr int kProjThreads = 352;
 
 // Tile -> (token tile, weight tile): groups of group_m token tiles, token tiles
 // fastest inside a group.
@@ -464,26 +463,107 @@ struct TileEpilogue {
     }
 };
 
+// K steps (16 ranks each) of a rank block.
+__device__ __forceinline__ int rank_steps(const AdapterParams &p, int rb) { return (min(p.rank - rb * 64, 64) + 15) >> 4; }
+
 // One block of `low` for the product with adapter a's columns of B, by a warp:
 // rows of ROWS tokens from m0 on, zeros for tokens of other adapters and behind
 // the rank.  `which`: 64 ranks and the bf16 part.  Asynchronous (one commit group).
 template <int ROWS>
 __device__ __forceinline__ void copy_low(const AdapterParams &p, int a, int which, int m0, const int16_t *tok, int lane,
                                          unsigned char *to) {
-    const int ld = p.rank_blocks * 64, rb = which / p.parts;
-    const __nv_bfloat16 *src = p.low + (which % p.parts ? (int64_t)p.m * ld : 0) + rb * 64;
-    const uint32_t dst = smem_u32(to);
+    const int ld = p.rank_blocks * 64, rb = which / p.parts, c = lane & 7;   // a lane's 16-byte piece of each row
+    const __nv_bfloat16 *src = p.low + (which % p.parts ? (int64_t)p.m * ld : 0) + (int64_t)m0 * ld + rb * 64 + c * 8;
+    const bool in_rank = rb * 64 + c * 8 < p.rank;
+    if (c < 2 * rank_steps(p, rb)) {   // what the product reads
+        const uint32_t dst = smem_u32(to);
 #pragma unroll 8
-    for (int x = lane; x < ROWS * 8; x += 32) {   // 16-byte piece c of token j sits at c ^ (j % 8)
-        const int j = x >> 3, c = x & 7;
-        const bool mine = tok[j] == a && rb * 64 + c * 8 < p.rank;
-        const __nv_bfloat16 *from = mine ? src + (int64_t)(m0 + j) * ld + c * 8 : p.low;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + j * 128 + ((c ^ (j & 7)) << 4)), "l"(from),
-                     "r"(mine ? 16 : 0)
-                     : "memory");
+        for (int j = lane >> 3; j < ROWS; j += 4) {   // piece c of token j sits at c ^ (j % 8)
+            const bool mine = in_rank && tok[j] == a;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + j * 128 + ((c ^ (j & 7)) << 4)),
+                         "l"(mine ? src + (int64_t)j * ld : p.low), "r"(mine ? 16 : 0)
+                         : "memory");
+        }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
+
+// Whether a barrier's phase has ended, without waiting for it.
+__device__ __forceinline__ bool mbar_ready(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok;
+}
+
+// The builder warps, kBuilders from warp 10 on: the first lists a tile's adapters,
+// then they take its blocks of `low` in turn.  What a block costs is the latency
+// of its copy and the way to the MMA thread and back, so several are on their way.
+// tile(i): the i-th tile's first token, -1 behind the last; copy(a, which, m0, buffer);
+// hand_over(buffer).
+constexpr int kBuilders = 2;
+template <int TN, int BUFS, typename Tile, typename Share, typename Copy, typename HandOver>
+__device__ __forceinline__ void build_blocks(const AdapterParams &p, int who, int lane, TileList<TN> *lists, ListScratch<TN> &scratch,
+                                             uint64_t *lfull, uint64_t *lempty, uint64_t *tfree, uint64_t *bempty, int code,
+                                             bool &aborted, Tile tile, Share share, Copy copy, HandOver hand_over) {
+    const int per_adapter = p.rank_blocks * p.parts;
+    bool waited = false;
+    uint32_t built = 0;   // blocks of the tiles before
+    for (uint32_t i = 0; !aborted; ++i) {
+        const int m0 = tile(i);
+        if (m0 < 0) break;
+        TileList<TN> &list = lists[i & 1];
+        if (who == 0) {
+            if (!warp_wait(&lempty[i & 1], ((i >> 1) & 1) ^ 1, p.flag, code, &aborted)) break;
+            if (!warp_wait(tfree, (i & 1) ^ 1, p.flag, code, &aborted)) break;   // the others still read the last tile's tokens
+            if (p.adapters) build_list<TN, 32>(p, m0, lane, list, scratch);
+            else if (lane == 0) list.count = 0;
+            mbar_arrive(&lfull[i & 1]);
+            __syncwarp();
+        } else if (!warp_wait(&lfull[i & 1], (i >> 1) & 1, p.flag, code, &aborted)) {
+            break;
+        }
+        int a0, na;
+        share(list.count, a0, na);
+        if (na > 0 && !waited) {
+            grid_dep_wait();
+            waited = true;
+        }
+        int pending = -1;   // a block that is on its way
+        for (int b = (who + kBuilders - built % kBuilders) % kBuilders; b < na; b += kBuilders) {
+            const uint32_t at = built + b;
+            const int buf = at % BUFS;
+            uint64_t *bar = &bempty[buf];
+            const uint32_t parity = ((at / BUFS) & 1) ^ 1;
+            if (pending >= 0 && !__all_sync(0xffffffffu, mbar_ready(bar, parity))) {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                hand_over(pending);
+                pending = -1;
+            }
+            if (!warp_wait(bar, parity, p.flag, code + 1, &aborted)) break;
+            const int e = a0 + b;
+            copy(list.ids[e / per_adapter], e % per_adapter, m0, buf);
+            if (pending >= 0) {
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                hand_over(pending);
+            }
+            pending = buf;
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (pending >= 0 && !aborted) hand_over(pending);
+        built += na;
+        __syncwarp();
+        if (who != 0 && lane == 0) mbar_arrive(tfree);
+    }
+    grid_dep_wait();   // low_kernel has ended before this kernel does: the workspace is free behind it
+}
+
+constexpr int kProjThreads = (10 + kBuilders) * 32;
 
 template <int TN, int EPI>
 __global__ void __launch_bounds__(kProjThreads, 1)
@@ -494,7 +574,8 @@ __global__ void __launch_bounds__(kProjThreads, 1)
     unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::BAR), *empty = full + C::STAGES, *tfull = empty + C::STAGES;
     uint64_t *tempty = tfull + 2, *lfull = tempty + 2, *lempty = lfull + 2, *bfull = lempty + 2, *bempty = bfull + C::BUFS;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bempty + C::BUFS);
+    uint64_t *tfree = bempty + C::BUFS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tfree + 1);
     TileList<TN> *lists = reinterpret_cast<TileList<TN> *>(smem + C::LIST);
     ListScratch<TN> &scratch = *reinterpret_cast<ListScratch<TN> *>(smem + C::LIST + 2 * sizeof(TileList<TN>));
     float *part = reinterpret_cast<float *>(smem);   // partial sums in the ring's place (splits > 1)
@@ -539,6 +620,7 @@ __global__ void __launch_bounds__(kProjThreads, 1)
             mbar_init(&bfull[i], 32);
             mbar_init(&bempty[i], 1);
         }
+        mbar_init(tfree, kBuilders - 1);
         fence_barrier_init();
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // for the loads of this very thread
         if (behind)
@@ -613,12 +695,13 @@ __global__ void __launch_bounds__(kProjThreads, 1)
                 tc_fence_after();
                 const uint32_t d = tmem + acc * C::ACC;
                 uint32_t more = 0;
-                auto multiply = [&](uint32_t b_addr) {
+                auto multiply = [&](uint32_t b_addr, int steps) {
                     const int s = it % C::STAGES;
                     const uint32_t a_addr = smem_u32(smem + s * C::STAGE);
                     if (!b_addr) b_addr = a_addr + C::A_BYTES;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
+                        if (q >= steps) break;
                         umma_f16_ss(d, sdesc_sw128(a_addr + q * 32, 16, 1024), sdesc_sw128(b_addr + q * 32, 16, 1024), idesc,
                                     more);
                         more = 1;
@@ -629,16 +712,17 @@ __global__ void __launch_bounds__(kProjThreads, 1)
                 auto main_block = [&](int) {
                     if (!mbar_wait(&full[it % C::STAGES], (it / C::STAGES) & 1, p.flag, 415, &aborted)) return false;
                     tc_fence_after();
-                    multiply(0);
+                    multiply(0, 4);
                     return true;
                 };
-                auto adapter_block = [&](int) {
+                int a0, na;
+                auto adapter_block = [&](int e) {
                     const int b = built % C::BUFS;
                     if (!mbar_wait(&full[it % C::STAGES], (it / C::STAGES) & 1, p.flag, 416, &aborted) ||
                         !mbar_wait(&bfull[b], (built / C::BUFS) & 1, p.flag, 417, &aborted))
                         return false;
                     tc_fence_after();
-                    multiply(smem_u32(smem + C::BUF + b * C::B_BYTES));
+                    multiply(smem_u32(smem + C::BUF + b * C::B_BYTES), rank_steps(p, (a0 + e) % per_adapter / p.parts));
                     umma_commit(&bempty[b]);
                     ++built;
                     return true;
@@ -647,7 +731,6 @@ __global__ void __launch_bounds__(kProjThreads, 1)
                     for (int k = 0; k < nk; ++k)
                         if (!main_block(k)) break;
                 if (aborted || !mbar_wait(&lfull[acc], (i >> 1) & 1, p.flag, 413, &aborted)) break;
-                int a0, na;
                 share(lists[acc].count, a0, na);
                 blocks_in_order(behind ? 0 : nk, na, main_block, adapter_block);
                 if (aborted) break;
@@ -655,49 +738,24 @@ __global__ void __launch_bounds__(kProjThreads, 1)
                 umma_commit(&tfull[acc]);
             }
         }
-    } else if (warp == 10) {
-        bool waited = false;
-        uint32_t i = 0, built = 0;
-        for (int t = first; t < tiles && !aborted; t += stride, ++i) {
-            int mt, nt;
-            tile_at(p, t, mt, nt);
-            const int m0 = mt * TN;
-            TileList<TN> &list = lists[i & 1];
-            if (!warp_wait(&lempty[i & 1], ((i >> 1) & 1) ^ 1, p.flag, 418, &aborted)) break;
-            if (p.adapters) {
-                build_list<TN, 32>(p, m0, lane, list, scratch);
-            } else if (lane == 0) {
-                list.count = 0;
-            }
-            mbar_arrive(&lfull[i & 1]);
-            __syncwarp();
-            int a0, na;
-            share(list.count, a0, na);
-            if (na > 0 && !waited) {
-                grid_dep_wait();
-                waited = true;
-            }
-            auto hand_over = [&](uint32_t which) {
+    } else if (warp >= 10) {
+        build_blocks<TN, C::BUFS>(
+            p, warp - 10, lane, lists, scratch, lfull, lempty, tfree, bempty, 418, aborted,
+            [&](uint32_t i) {
+                const int t = first + (int)i * stride;
+                if (t >= tiles) return -1;
+                int mt, nt;
+                tile_at(p, t, mt, nt);
+                return mt * TN;
+            },
+            share,
+            [&](int a, int which, int m0, int buf) {
+                copy_low<TN>(p, a, which, m0, scratch.tok, lane, smem + C::BUF + buf * C::B_BYTES);
+            },
+            [&](int buf) {
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&bfull[which % C::BUFS]);
-            };
-            for (int b = 0; b < na; ++b, ++built) {
-                const int buf = built % C::BUFS;
-                if (!warp_wait(&bempty[buf], ((built / C::BUFS) & 1) ^ 1, p.flag, 419, &aborted)) break;
-                const int e = a0 + b;
-                copy_low<TN>(p, list.ids[e / per_adapter], e % per_adapter, m0, scratch.tok, lane, smem + C::BUF + buf * C::B_BYTES);
-                if constexpr (C::BUFS == 1) {
-                    asm volatile("cp.async.wait_group 0;" ::: "memory");
-                    hand_over(built);
-                } else if (b > 0) {   // the one before, while this one is on its way
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    hand_over(built - 1);
-                }
-            }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            if (C::BUFS > 1 && na > 0 && !aborted) hand_over(built - 1);
-        }
-        grid_dep_wait();   // low_kernel has ended before this kernel does: the workspace is free behind it
+                mbar_arrive(&bfull[buf]);
+            });
     } else {
         // warps 2-5 and 6-9 take every other 32 tokens of a tile
         const int quad = warp & 3, side = warp >= 6 ? 32 : 0;
@@ -768,7 +826,7 @@ struct PairCfg {
     static constexpr int A_BYTES = BM * 128, B_BYTES = HALF * 128, STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = 6, BUFS = 2;
     static constexpr int RING = STAGES * STAGE, BUF = RING, BAR = BUF + BUFS * B_BYTES;
-    static constexpr int LIST = BAR + ((2 * STAGES + 8 + 2 * BUFS) * 8 + 8 + 15) / 16 * 16;
+    static constexpr int LIST = BAR + ((2 * STAGES + 9 + 2 * BUFS) * 8 + 8 + 15) / 16 * 16;
     static constexpr int BYTES = 1024 + LIST + 2 * (int)sizeof(TileList<TOKENS>) + (int)sizeof(ListScratch<TOKENS>);
     static_assert(BYTES <= 232448, "shared memory exceeds the per-CTA limit");
 };
@@ -831,7 +889,8 @@ __global__ void __launch_bounds__(kProjThreads, 1)
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::BAR), *empty = full + C::STAGES;
     uint64_t *tfull = empty + C::STAGES, *tempty = tfull + 2, *lfull = tempty + 2, *lempty = lfull + 2;
     uint64_t *bfull = lempty + 2, *bempty = bfull + C::BUFS;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bempty + C::BUFS);
+    uint64_t *tfree = bempty + C::BUFS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tfree + 1);
     TileList<C::TOKENS> *lists = reinterpret_cast<TileList<C::TOKENS> *>(smem + C::LIST);
     ListScratch<C::TOKENS> &scratch = *reinterpret_cast<ListScratch<C::TOKENS> *>(smem + C::LIST + 2 * sizeof(TileList<C::TOKENS>));
 
@@ -857,6 +916,7 @@ __global__ void __launch_bounds__(kProjThreads, 1)
             mbar_init(&bfull[i], 2);
             mbar_init(&bempty[i], 1);
         }
+        mbar_init(tfree, kBuilders - 1);
         fence_barrier_init();
     }
     if (warp == 1) {
@@ -922,7 +982,7 @@ __global__ void __launch_bounds__(kProjThreads, 1)
                 tc_fence_after();
                 const uint32_t d = tmem + acc * C::TOKENS;
                 uint32_t more = 0;
-                auto multiply = [&](uint32_t b_addr) {
+                auto multiply = [&](uint32_t b_addr, int steps) {
                     const int s = it % C::STAGES;
                     if (!mbar_wait_cluster(&full[s], (it / C::STAGES) & 1, p.flag, 436, &aborted)) return false;
                     tc_fence_after();
@@ -930,6 +990,7 @@ __global__ void __launch_bounds__(kProjThreads, 1)
                     if (!b_addr) b_addr = a_addr + C::A_BYTES;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
+                        if (q >= steps) break;
                         pair_mma(d, sdesc_sw128(a_addr + q * 32, 16, 1024), sdesc_sw128(b_addr + q * 32, 16, 1024), idesc, more);
                         more = 1;
                     }
@@ -938,11 +999,11 @@ __global__ void __launch_bounds__(kProjThreads, 1)
                     return true;
                 };
                 blocks_in_order(
-                    nk, na, [&](int) { return multiply(0); },
-                    [&](int) {
+                    nk, na, [&](int) { return multiply(0, 4); },
+                    [&](int e) {
                         const int b = built % C::BUFS;
                         if (!mbar_wait_cluster(&bfull[b], (built / C::BUFS) & 1, p.flag, 437, &aborted) ||
-                            !multiply(smem_u32(smem + C::BUF + b * C::B_BYTES)))
+                            !multiply(smem_u32(smem + C::BUF + b * C::B_BYTES), rank_steps(p, e % per_adapter / p.parts)))
                             return false;
                         pair_commit(&bempty[b]);
                         ++built;
@@ -953,43 +1014,28 @@ __global__ void __launch_bounds__(kProjThreads, 1)
                 mbar_arrive(&lempty[acc]);
             }
         }
-    } else if (warp == 10) {
-        bool waited = false;
-        uint32_t i = 0, built = 0;
-        for (int t = first; t < tiles && !aborted; t += stride, ++i) {
-            int mt, nt;
-            tile_at(p, t, mt, nt);
-            const int m0 = mt * C::TOKENS;
-            TileList<C::TOKENS> &list = lists[i & 1];
-            if (!warp_wait(&lempty[i & 1], ((i >> 1) & 1) ^ 1, p.flag, 438, &aborted)) break;
-            if (p.adapters) build_list<C::TOKENS, 32>(p, m0, lane, list, scratch);
-            else if (lane == 0) list.count = 0;
-            mbar_arrive(&lfull[i & 1]);
-            __syncwarp();
-            const int na = list.count * per_adapter;
-            if (na > 0 && !waited) {
-                grid_dep_wait();
-                waited = true;
-            }
-            auto hand_over = [&](uint32_t which) {
+    } else if (warp >= 10) {
+        build_blocks<C::TOKENS, C::BUFS>(
+            p, warp - 10, lane, lists, scratch, lfull, lempty, tfree, bempty, 438, aborted,
+            [&](uint32_t i) {
+                const int t = first + (int)i * stride;
+                if (t >= tiles) return -1;
+                int mt, nt;
+                tile_at(p, t, mt, nt);
+                return mt * C::TOKENS;
+            },
+            [&](int count, int &a0, int &na) {
+                a0 = 0;
+                na = count * per_adapter;
+            },
+            [&](int a, int which, int m0, int buf) {
+                copy_low<C::HALF>(p, a, which, m0 + rank * C::HALF, scratch.tok + rank * C::HALF, lane, smem + C::BUF + buf * C::B_BYTES);
+            },
+            [&](int buf) {
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive_at(&bfull[which % C::BUFS], 0);
-            };
-            for (int e = 0; e < na; ++e, ++built) {
-                const int buf = built % C::BUFS;
-                if (!warp_wait(&bempty[buf], ((built / C::BUFS) & 1) ^ 1, p.flag, 439, &aborted)) break;
-                copy_low<C::HALF>(p, list.ids[e / per_adapter], e % per_adapter, m0 + rank * C::HALF, scratch.tok + rank * C::HALF, lane,
-                                  smem + C::BUF + buf * C::B_BYTES);
-                if (e > 0) {   // the one before, while this one is on its way
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    hand_over(built - 1);
-                }
-            }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            if (na > 0 && !aborted) hand_over(built - 1);
-        }
-        grid_dep_wait();   // low_kernel has ended before this kernel does: the workspace is free behind it
+                if (lane == 0) mbar_arrive_at(&bfull[buf], 0);
+            });
     } else {
         // warps 2-5 and 6-9 take every other 32 tokens of a tile
         const int quad = warp & 3, side = warp >= 6 ? 32 : 0;
@@ -1156,7 +1202,7 @@ cudaError_t run_pair(const ltx_ctx *ctx, AdapterParams p, int epilogue, const CU
 // 23 / 31; 200 x 4096 x 4096 27.6 / 27.3 / 29 / 44 / 64; 512 x 4096 x 4096 37 / 39 / 47 / 76.
 int tokens_for(int m, int n, int sms) {
     if (m <= 64) return m <= 16 ? 16 : m <= 32 ? 32 : 64;
-    for (int t = 256; t > 16; t /= 2)
+    for (int t = m <= 128 ? 128 : 256; t > 16; t /= 2)
         if ((int64_t)((m + t - 1) / t) * ((n + BM - 1) / BM) * 5 >= sms * 2) return t;
     return 16;
 }
