@@ -320,8 +320,8 @@ __global__ void __launch_bounds__(kLowThreads)
 
 // ── the projection ───────────────────────────────────────────────────────────
 //
-// 12 warps: 0 TMA, 1 MMA, 2-9 epilogue (two accumulators: the epilogue of one
-// tile runs under the next one's products), 10 and 11 the builders: they list each
+// 12 to 14 warps: 0 TMA, 1 MMA, 2-9 epilogue (two accumulators: the epilogue of one
+// tile runs under the next one's products), from 10 on the builders: they list each
 // tile's adapters and copy its rows of low, zeros for other adapters' tokens, into
 // buffers beside the ring while the main blocks are multiplied.
 // Few tiles: a cluster of `splits` CTAs shares a tile's blocks and joins its
@@ -333,7 +333,8 @@ struct ProjCfg {
     // up to 128 tokens: as deep as HBM's latency asks (96 KB and more), and no
     // deeper, so that low_kernel's CTAs run beside these
     static constexpr int STAGES = TN >= 128 ? 3 : TN == 64 ? 4 : TN == 32 ? 6 : 7;
-    static constexpr int BUFS = TN <= 32 ? 4 : 2;   // rows of low
+    static constexpr int BUFS = TN <= 32 ? 4 : TN == 256 ? 2 : 3, BUILDERS = TN == 256 ? 2 : 3;   // for rows of low, and who copies them
+    static constexpr int THREADS = (10 + BUILDERS) * 32;
     static constexpr int RING = STAGES * STAGE, BUF = RING, BAR = BUF + BUFS * B_BYTES;
     static constexpr int LIST = BAR + ((2 * STAGES + 9 + 2 * BUFS) * 8 + 8 + 15) / 16 * 16;
     static constexpr int BYTES = 1024 + LIST + 2 * (int)sizeof(TileList<TN>) + (int)sizeof(ListScratch<TN>);
@@ -501,16 +502,18 @@ __device__ __forceinline__ bool mbar_ready(uint64_t *bar, uint32_t parity) {
     return ok;
 }
 
-// The builder warps, kBuilders from warp 10 on: the first lists a tile's adapters,
+// The builder warps, BUILDERS from warp 10 on: the first lists a tile's adapters,
 // then they take its blocks of `low` in turn.  What a block costs is the latency
 // of its copy and the way to the MMA thread and back, so several are on their way.
 // tile(i): the i-th tile's first token, -1 behind the last; copy(a, which, m0, buffer);
 // hand_over(buffer).
-constexpr int kBuilders = 2;
-template <int TN, int BUFS, typename Tile, typename Share, typename Copy, typename HandOver>
+// BUFS >= BUILDERS: a builder is then never two rounds of a buffer ahead of the
+// products, which the parity of a barrier could not tell from none.
+template <int TN, int BUFS, int BUILDERS, typename Tile, typename Share, typename Copy, typename HandOver>
 __device__ __forceinline__ void build_blocks(const AdapterParams &p, int who, int lane, TileList<TN> *lists, ListScratch<TN> &scratch,
                                              uint64_t *lfull, uint64_t *lempty, uint64_t *tfree, uint64_t *bempty, int code,
                                              bool &aborted, Tile tile, Share share, Copy copy, HandOver hand_over) {
+    static_assert(BUFS >= BUILDERS);
     const int per_adapter = p.rank_blocks * p.parts;
     bool waited = false;
     uint32_t built = 0;   // blocks of the tiles before
@@ -535,7 +538,7 @@ __device__ __forceinline__ void build_blocks(const AdapterParams &p, int who, in
             waited = true;
         }
         int pending = -1;   // a block that is on its way
-        for (int b = (who + kBuilders - built % kBuilders) % kBuilders; b < na; b += kBuilders) {
+        for (int b = (who + BUILDERS - built % BUILDERS) % BUILDERS; b < na; b += BUILDERS) {
             const uint32_t at = built + b;
             const int buf = at % BUFS;
             uint64_t *bar = &bempty[buf];
@@ -563,10 +566,8 @@ __device__ __forceinline__ void build_blocks(const AdapterParams &p, int who, in
     grid_dep_wait();   // low_kernel has ended before this kernel does: the workspace is free behind it
 }
 
-constexpr int kProjThreads = (10 + kBuilders) * 32;
-
 template <int TN, int EPI>
-__global__ void __launch_bounds__(kProjThreads, 1)
+__global__ void __launch_bounds__(ProjCfg<TN>::THREADS, 1)
     project_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                    const __grid_constant__ CUtensorMap tmB, AdapterParams p) {
     using C = ProjCfg<TN>;
@@ -620,7 +621,7 @@ __global__ void __launch_bounds__(kProjThreads, 1)
             mbar_init(&bfull[i], 32);
             mbar_init(&bempty[i], 1);
         }
-        mbar_init(tfree, kBuilders - 1);
+        mbar_init(tfree, C::BUILDERS - 1);
         fence_barrier_init();
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // for the loads of this very thread
         if (behind)
@@ -739,7 +740,7 @@ __global__ void __launch_bounds__(kProjThreads, 1)
             }
         }
     } else if (warp >= 10) {
-        build_blocks<TN, C::BUFS>(
+        build_blocks<TN, C::BUFS, C::BUILDERS>(
             p, warp - 10, lane, lists, scratch, lfull, lempty, tfree, bempty, 418, aborted,
             [&](uint32_t i) {
                 const int t = first + (int)i * stride;
@@ -824,7 +825,10 @@ __global__ void __launch_bounds__(kProjThreads, 1)
 struct PairCfg {
     static constexpr int TOKENS = 256, HALF = 128;
     static constexpr int A_BYTES = BM * 128, B_BYTES = HALF * 128, STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = 6, BUFS = 2;
+    // Four builders and a shorter ring instead of two and six stages: a mixed tile's
+    // blocks cost up to a third less (642 x 11552 x 960 with 12 adapters of rank 128:
+    // 142 -> 100 us), tiles of one adapter a hundredth more.
+    static constexpr int STAGES = 5, BUFS = 4, BUILDERS = 4, THREADS = (10 + BUILDERS) * 32;
     static constexpr int RING = STAGES * STAGE, BUF = RING, BAR = BUF + BUFS * B_BYTES;
     static constexpr int LIST = BAR + ((2 * STAGES + 9 + 2 * BUFS) * 8 + 8 + 15) / 16 * 16;
     static constexpr int BYTES = 1024 + LIST + 2 * (int)sizeof(TileList<TOKENS>) + (int)sizeof(ListScratch<TOKENS>);
@@ -880,7 +884,7 @@ __device__ __forceinline__ void pair_commit(uint64_t *bar) {
 }
 
 template <int EPI>
-__global__ void __launch_bounds__(kProjThreads, 1)
+__global__ void __launch_bounds__(PairCfg::THREADS, 1)
     project_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                         const __grid_constant__ CUtensorMap tmB, AdapterParams p) {
     using C = PairCfg;
@@ -916,7 +920,7 @@ __global__ void __launch_bounds__(kProjThreads, 1)
             mbar_init(&bfull[i], 2);
             mbar_init(&bempty[i], 1);
         }
-        mbar_init(tfree, kBuilders - 1);
+        mbar_init(tfree, C::BUILDERS - 1);
         fence_barrier_init();
     }
     if (warp == 1) {
@@ -1015,7 +1019,7 @@ __global__ void __launch_bounds__(kProjThreads, 1)
             }
         }
     } else if (warp >= 10) {
-        build_blocks<C::TOKENS, C::BUFS>(
+        build_blocks<C::TOKENS, C::BUFS, C::BUILDERS>(
             p, warp - 10, lane, lists, scratch, lfull, lempty, tfree, bempty, 438, aborted,
             [&](uint32_t i) {
                 const int t = first + (int)i * stride;
@@ -1166,7 +1170,7 @@ cudaError_t run_project(const ltx_ctx *ctx, AdapterParams p, int epilogue, const
     p.group_m = group_of(p, TN);
     const int grid = p.splits > 1 ? (int)tiles * p.splits : (int)std::min<int64_t>(tiles, sms);
     auto go = [&](auto kern) {
-        return launch(ctx, kern, grid, kProjThreads, ProjCfg<TN>::BYTES, ProjCfg<TN>::BYTES, p.splits, p.adapters > 0, tw, tx, tb, p);
+        return launch(ctx, kern, grid, ProjCfg<TN>::THREADS, ProjCfg<TN>::BYTES, ProjCfg<TN>::BYTES, p.splits, p.adapters > 0, tw, tx, tb, p);
     };
     switch (epilogue) {
     case LTX_EPI_BF16: return go(project_kernel<TN, LTX_EPI_BF16>);
@@ -1184,7 +1188,7 @@ cudaError_t run_pair(const ltx_ctx *ctx, AdapterParams p, int epilogue, const CU
     p.group_m = group_of(p, PairCfg::TOKENS);
     const int grid = 2 * (int)std::min<int64_t>((int64_t)p.m_tiles * p.n_tiles, ctx->sm_count / 2);
     auto go = [&](auto kern) {
-        return launch(ctx, kern, grid, kProjThreads, PairCfg::BYTES, PairCfg::BYTES, 2, p.adapters > 0, tw, tx, tb, p);
+        return launch(ctx, kern, grid, PairCfg::THREADS, PairCfg::BYTES, PairCfg::BYTES, 2, p.adapters > 0, tw, tx, tb, p);
     };
     switch (epilogue) {
     case LTX_EPI_BF16: return go(project_pair_kernel<LTX_EPI_BF16>);
