@@ -1259,9 +1259,15 @@ extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args) {
     p.ld_gate = ld_gate;
     p.out = out_dev;
     p.flag = ctx->timeout_flag;
-    const int tn = tokens_for(m, n, ctx->sm_count), tl = std::min(tn, 64);
+    int tn = tokens_for(m, n, ctx->sm_count);
     // enough 256 x 256 tiles for every pair of SMs
     const bool pair = tn == 256 && (int64_t)((m + 255) / 256) * ((n + 255) / 256) * 2 > ctx->sm_count;
+    // One SM's tile of 256 tokens has smem for two builders only: where a mixed tile
+    // may have more than a quarter of a block for the adapters per block of K, 128
+    // tokens.  us at 256 / 128: 136 x 15432 x 256 with 9 of rank 64, gated residual
+    // 59 / 42; 160 x 12000 x 640, 8 of 8 34 / 32; 256 x 16384 x 4096, 4 of 64 56 / 70.
+    if (tn == 256 && !pair && (int64_t)std::min(adapters, 256) * p.rank_blocks * p.parts * 4 > (k + 63) / 64) tn = 128;
+    const int tl = std::min(tn, 64);
     CUtensorMap tw, tx, txl, ta, tb;
     bool ok = make_map(&tw, w_dev, n, k, ldw, BM) && make_map(&tx, x_dev, m, k, ldx, pair ? 128 : tn);
     ta = tb = txl = tx;
