@@ -538,18 +538,21 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     }
 }
 
-// Joins the items that a cut of the line divides.  Block c - 1 looks at the cut
-// before CTA c: if it is the first inside its item, the partials of CTA c - 1
+// Joins the items that a cut of the line divides.  Block (c - 1, y) looks at the
+// cut before CTA c: if it is the first inside its item, the partials of CTA c - 1
 // (slot 1) and of the CTAs from c on that reach into the item (slot 0) are one
-// result.
+// result, and the block joins rows 4y to 4y + 3 of it: a warp weighs a row's
+// partials, then each warp adds up every fourth of them for all four rows, with
+// the loads of a step in flight together, and the four sums become one.
+constexpr int kJoinRows = 4, kMaxCtas = 256;
 template <int D, int N>
 __global__ void __launch_bounds__(128) few_join_kernel(PackedParams p, Partials part, int ctas) {
     __shared__ Place s_place;
     __shared__ int64_t s_per;
     __shared__ int s_go;
-    __shared__ float s_acc[4][D + 1];
-    const int c = blockIdx.x + 1, lane = threadIdx.x & 31;
-    if (threadIdx.x < 32) {
+    __shared__ float s_weight[kMaxCtas][kJoinRows], s_total[kJoinRows], s_acc[4][kJoinRows][D];
+    const int c = blockIdx.x + 1, row0 = blockIdx.y * kJoinRows, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+    if (warp == 0) {
         int64_t per, left;
         Place at{};
         cut_line(p, c, ctas, lane, per, left, at);
@@ -560,61 +563,63 @@ __global__ void __launch_bounds__(128) few_join_kernel(PackedParams p, Partials 
         }
     }
     __syncthreads();
-    if (!s_go) {
-        grid_dep_wait();   // this kernel's end stands for the attention's too
-        return;
-    }
+    grid_dep_wait();   // also where there is nothing to do: this kernel's end stands for the attention's too
+    if (!s_go) return;
     const DocWork d = s_place.d;
     const int kvh = (int)(s_place.item / d.row_tiles);
     const int token0 = (int)(s_place.item - (int64_t)kvh * d.row_tiles) * p.tile_tokens;
     // the item goes on for tiles - tile more tiles from this cut
     const int more = (int)((d.tiles - s_place.tile + s_per - 1) / s_per);
-    grid_dep_wait();
     const int rows = min(p.tile_tokens, d.lq - token0) * p.group;
-    // A warp per row, or all four on each row in turn where many CTAs share the
-    // item: then each takes every fourth partial, and warp 0 adds the four up.
-    const int warp = threadIdx.x / 32, share = more >= 4 ? 4 : 1;
-    auto slot = [&](int i) { return (int64_t)(i == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + i)); };
-    for (int r = share == 4 ? 0 : warp; r < rows; r += share == 4 ? 1 : 4) {
-        float top = -INFINITY, total = 0.f, acc[D / 32] = {};
-        for (int i = lane; i <= more; i += 32) top = fmaxf(top, part.ml[slot(i) * N + r].x);
+    if (row0 >= rows) return;
+    auto slot = [&](int i) { return (int64_t)(i == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + i)) * N + row0; };
+    float top = -INFINITY, total = 0.f;
+    const bool row_ok = row0 + warp < rows;   // a row behind the last has no partials
+    for (int i = lane; row_ok && i <= more; i += 32) top = fmaxf(top, part.ml[slot(i) + warp].x);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-#pragma unroll 4
-        for (int i = share == 4 ? warp : 0; i <= more; i += share) {
-            const float2 ml = part.ml[slot(i) * N + r];
-            const float *o = part.o + (slot(i) * N + r) * D + lane;
-            const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-            total += ml.y * f;
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int i = lane; i <= more; i += 32) {
+        const float2 ml = row_ok ? part.ml[slot(i) + warp] : make_float2(-INFINITY, 0.f);
+        const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+        s_weight[i][warp] = f;
+        total += ml.y * f;
+    }
 #pragma unroll
-            for (int x = 0; x < D / 32; ++x) {
-                const float v = o[x * 32];
-                acc[x] += f == 0.f ? 0.f : v * f;
-            }
-        }
-        if (share == 4) {
-            __syncthreads();
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (lane == 0) s_total[warp] = total;
+    __syncthreads();
+    float acc[kJoinRows][D / 32] = {};
+#pragma unroll 2
+    for (int i = warp; i <= more; i += 4) {
+        const float *o = part.o + slot(i) * D + lane;
 #pragma unroll
-            for (int x = 0; x < D / 32; ++x) s_acc[warp][x * 32 + lane] = acc[x];
-            if (lane == 0) s_acc[warp][D] = total;
-            __syncthreads();
-            if (warp != 0) continue;
-            total = s_acc[0][D] + s_acc[1][D] + s_acc[2][D] + s_acc[3][D];
+        for (int r = 0; r < kJoinRows; ++r) {
+            const float f = s_weight[i][r];
 #pragma unroll
             for (int x = 0; x < D / 32; ++x)
-                acc[x] = s_acc[0][x * 32 + lane] + s_acc[1][x * 32 + lane] + s_acc[2][x * 32 + lane] + s_acc[3][x * 32 + lane];
+                if (f != 0.f) acc[r][x] += o[r * D + x * 32] * f;
         }
-        __nv_bfloat16 *out =
-            p.out + (int64_t)(d.qs + token0 + r / p.group) * p.ldo + (kvh * p.group + r % p.group) * D + lane;
+    }
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x) out[x * 32] = __float2bfloat16_rn(total == 0.f ? 0.f : acc[x] / total);
+    for (int r = 0; r < kJoinRows; ++r)
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) s_acc[warp][r][x * 32 + lane] = acc[r][x];
+    __syncthreads();
+    if (!row_ok) return;
+    const int r = row0 + warp;
+    __nv_bfloat16 *out = p.out + (int64_t)(d.qs + token0 + r / p.group) * p.ldo + (kvh * p.group + r % p.group) * D + lane;
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) {
+        const int at = x * 32 + lane;
+        const float v = s_acc[0][warp][at] + s_acc[1][warp][at] + s_acc[2][warp][at] + s_acc[3][warp][at];
+        out[x * 32] = __float2bfloat16_rn(s_total[warp] == 0.f ? 0.f : v / s_total[warp]);
     }
 }
 
 template <int D, int N>
 int run_few(ltx_ctx *ctx, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const PackedParams &p,
             bool v_f16) {
-    const int ctas = ctx->sm_count;
+    const int ctas = std::min(ctx->sm_count, kMaxCtas);
     void *work = nullptr;
     const size_t o_bytes = (size_t)ctas * 2 * N * D * 4;
     int rc = work_alloc(ctx, o_bytes + (size_t)ctas * 2 * N * 8, &work);
@@ -628,7 +633,7 @@ int run_few(ltx_ctx *ctx, const CUtensorMap &tq, const CUtensorMap &tk, const CU
     }
     if (e == cudaSuccess && ctas > 1) {
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(ctas - 1);
+        cfg.gridDim = dim3(ctas - 1, N / kJoinRows);
         cfg.blockDim = dim3(128);
         cfg.stream = ctx->stream;
         cudaLaunchAttribute attr[1];
