@@ -174,6 +174,38 @@ __device__ __forceinline__ void load_columns(uint32_t taddr, float (&v)[N]) {
     for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i / 16][i % 16]);
 }
 
+// A row's value over the 32 lanes of a warp, for N rows that every lane holds: each
+// step halves the rows a lane goes on with, so N - 1 exchanges do for all of them.
+// A lane ends with first_row in v[0] (N 64: and the row behind it in v[1]).
+template <int N>
+__device__ __forceinline__ int first_row(int lane) { return N == 16 ? lane >> 1 : N / 32 * lane; }
+template <int N, typename F>
+__device__ __forceinline__ void over_lanes(float (&v)[N], int lane, F join) {
+    int n = N;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const bool up = lane & o;
+        if (n == 1) {
+            v[0] = join(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+        } else {
+            n /= 2;
+#pragma unroll
+            for (int i = 0; i < N / 2; ++i)
+                if (i < n) {
+                    const float keep = up ? v[i + n] : v[i], give = up ? v[i] : v[i + n];
+                    v[i] = join(keep, __shfl_xor_sync(0xffffffffu, give, o));
+                }
+        }
+    }
+}
+// The same into a warp's N words of shared memory.
+template <int N, typename F>
+__device__ __forceinline__ void over_lanes_to(float (&v)[N], int lane, float *to, F join) {
+    over_lanes<N>(v, lane, join);
+#pragma unroll
+    for (int i = 0; i < (N == 64 ? 2 : 1); ++i) to[first_row<N>(lane) + i] = v[i];
+}
+
 // Partials: slot 0 of a CTA for the item it goes on with, slot 1 for the one it begins.
 struct Partials {
     float *o;     // [ctas * 2][N][D]
@@ -196,9 +228,10 @@ __global__ void __launch_bounds__(kFewThreads, 1)
     Place *s_place = reinterpret_cast<Place *>(tmem_slot + 2);
     static_assert((2 * kSlots + 8 + 4 * kScores) * 8 + 8 + sizeof(Place) + 8 <= 512, "barriers and place exceed their block");
     int64_t *s_len = reinterpret_cast<int64_t *>(s_place + 1);
-    // per row: first keys it sees, key it stands beside, slope log2e, reference maximum; [4][N] warps' maxima or sums
+    // per row: first keys it sees, key it stands beside, slope log2e, reference maximum, what it moves by or 1 / sum;
+    // [4][N] warps' maxima or sums
     int *r_lim = reinterpret_cast<int *>(smem + L::ROWS), *r_place = r_lim + N;
-    float *r_slope = reinterpret_cast<float *>(r_place + N), *r_ref = r_slope + N, *r_warp = r_ref + N;
+    float *r_slope = reinterpret_cast<float *>(r_place + N), *r_ref = r_slope + N, *r_alpha = r_ref + N, *r_warp = r_alpha + N;
     int64_t *r_out = reinterpret_cast<int64_t *>(r_warp + 4 * N);   // where the row goes, -1 for none
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -387,14 +420,18 @@ __global__ void __launch_bounds__(kFewThreads, 1)
                 for (int r4 = 0; r4 < N; r4 += 4) {
                     const int4 lim = *reinterpret_cast<const int4 *>(r_lim + r4);
                     const float4 ref = *reinterpret_cast<const float4 *>(r_ref + r4);
+                    const float4 slope = *reinterpret_cast<const float4 *>(r_slope + r4);
+                    const int4 place = *reinterpret_cast<const int4 *>(r_place + r4);
+                    const float slopes[4] = {slope.x, slope.y, slope.z, slope.w};
+                    const int places[4] = {place.x, place.y, place.z, place.w};
                     const int lims[4] = {lim.x, lim.y, lim.z, lim.w};
                     const float refs[4] = {ref.x, ref.y, ref.z, ref.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float &v = y[r4 + e];
                         if (modified) {
-                            mod.slope2 = r_slope[r4 + e];
-                            mod.place = (float)(r_place[r4 + e] - kv);
+                            mod.slope2 = slopes[e];
+                            mod.place = (float)(places[e] - kv);
                             v = mod(v, 0);
                         } else {
                             v *= sl2;
@@ -406,27 +443,35 @@ __global__ void __launch_bounds__(kFewThreads, 1)
                 if (softmax_any(over)) {
                     // Some row's maximum outgrew its reference: each row's over the
                     // tile, by warps and then all; rows that grew move to it.
+                    float m[N];
 #pragma unroll
-                    for (int r = 0; r < N; ++r) {
-                        float m = y[r];
-#pragma unroll
-                        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-                        if (lane == 0) r_warp[quad * N + r] = m;
+                    for (int r = 0; r < N; ++r) m[r] = y[r];
+                    over_lanes_to<N>(m, lane, r_warp + quad * N, [](float a, float b) { return fmaxf(a, b); });
+                    softmax_sync();
+                    if (key < N) {
+                        const float top = fmaxf(fmaxf(r_warp[key], r_warp[N + key]), fmaxf(r_warp[2 * N + key], r_warp[3 * N + key]));
+                        const float ref = r_ref[key];
+                        const bool grew = top > ref + kRescaleLog2;
+                        r_alpha[key] = grew ? ex2(ref - top) : 1.f;
+                        if (grew) r_ref[key] = top;
                     }
                     // O^T is stable once the tile before has been added to it
                     if (j > 0) warp_wait(&p_empty[(i - 1) % kScores], ((i - 1) / kScores) & 1, p.flag, 332, &aborted);
-                    tc_fence_after();
                     softmax_sync();
-                    float o[N];
-                    if (j > 0) load_columns<N>(o_tmem, o);
-#pragma unroll
-                    for (int r = 0; r < N; ++r) {
-                        const float m = fmaxf(fmaxf(r_warp[r], r_warp[N + r]), fmaxf(r_warp[2 * N + r], r_warp[3 * N + r]));
-                        const float a = m > r_ref[r] + kRescaleLog2 ? ex2(r_ref[r] - m) : 1.f;
-                        l[r] *= a;
-                        if (j > 0) o[r] *= a;
-                    }
                     if (j > 0) {
+                        tc_fence_after();
+                        float o[N];
+                        load_columns<N>(o_tmem, o);
+#pragma unroll
+                        for (int r4 = 0; r4 < N; r4 += 4) {
+                            const float4 a = *reinterpret_cast<const float4 *>(r_alpha + r4);
+                            const float as[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                l[r4 + e] *= as[e];
+                                o[r4 + e] *= as[e];
+                            }
+                        }
 #pragma unroll
                         for (int c = 0; c < N; c += 16) {
                             uint32_t u[16];
@@ -437,12 +482,6 @@ __global__ void __launch_bounds__(kFewThreads, 1)
                         tmem_st_wait();
                         tc_fence_before();
                     }
-                    softmax_sync();   // the references have been read
-                    if (key < N) {
-                        const float m = fmaxf(fmaxf(r_warp[key], r_warp[N + key]), fmaxf(r_warp[2 * N + key], r_warp[3 * N + key]));
-                        if (m > r_ref[key] + kRescaleLog2) r_ref[key] = m;
-                    }
-                    softmax_sync();
                 }
                 // P (row r, key): 16 bytes of 8 keys at their place ^ (r % 8), 64 keys to a block of N rows
                 warp_wait(&p_empty[b], ph ^ 1, p.flag, 333, &aborted);
@@ -485,14 +524,15 @@ __global__ void __launch_bounds__(kFewThreads, 1)
                 mbar_arrive(&p_full[b]);
             }
             // the rows' sums over all keys, and O^T: lane = column d of the head
-#pragma unroll
-            for (int r = 0; r < N; ++r) {
-                float s = l[r];
-#pragma unroll
-                for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-                if (lane == 0) r_warp[quad * N + r] = s;
-            }
+            over_lanes_to<N>(l, lane, r_warp + quad * N, [](float a, float b) { return a + b; });
             softmax_sync();
+            const bool whole = w.t0 == 0 && w.t1 == d.tiles;
+            const int64_t slot = 2 * blockIdx.x + (w.t0 == 0);
+            if (key < N) {
+                const float total = r_warp[key] + r_warp[N + key] + r_warp[2 * N + key] + r_warp[3 * N + key];
+                r_alpha[key] = total == 0.f ? 0.f : 1.f / total;   // no key seen: 0; a NaN sum stays NaN
+                if (!whole) part.ml[slot * N + key] = make_float2(r_ref[key], total);
+            }
             if (n > 0) {
                 if (warp_wait(&o_full[qb], (piece >> 1) & 1, p.flag, 335, &aborted)) {
                     tc_fence_after();
@@ -505,21 +545,23 @@ __global__ void __launch_bounds__(kFewThreads, 1)
 #pragma unroll
                 for (int r = 0; r < N; ++r) l[r] = 0.f;
             }
-            const bool whole = w.t0 == 0 && w.t1 == d.tiles;
-            const int slot = 2 * blockIdx.x + (w.t0 == 0);
+            softmax_sync();
             if (key < D && !aborted) {
+                if (whole) {
 #pragma unroll
-                for (int r = 0; r < N; ++r) {
-                    const int64_t to = r_out[r];
-                    if (to < 0) continue;
-                    const float total = r_warp[r] + r_warp[N + r] + r_warp[2 * N + r] + r_warp[3 * N + r];
-                    if (whole) {
-                        const float v = total == 0.f ? 0.f : __fdividef(l[r], total);   // no key seen: 0; a NaN sum stays NaN
-                        p.out[to + key] = __float2bfloat16_rn(v);
-                    } else {
-                        part.o[((int64_t)slot * N + r) * D + key] = l[r];
-                        if (key == 0) part.ml[(int64_t)slot * N + r] = make_float2(r_ref[r], total);
+                    for (int r4 = 0; r4 < N; r4 += 4) {
+                        const float4 inv = *reinterpret_cast<const float4 *>(r_alpha + r4);
+                        const float is[4] = {inv.x, inv.y, inv.z, inv.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int64_t to = r_out[r4 + e];
+                            if (to >= 0) p.out[to + key] = __float2bfloat16_rn(is[e] == 0.f ? 0.f : l[r4 + e] * is[e]);
+                        }
                     }
+                } else {
+                    float *o = part.o + slot * N * D + key;   // rows that nothing reads included
+#pragma unroll
+                    for (int r = 0; r < N; ++r) o[r * D] = l[r];
                 }
             }
             if (n > 0) {
