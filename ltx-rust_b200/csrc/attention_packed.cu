@@ -50,6 +50,7 @@ namespace ltx {
 namespace {
 
 constexpr int kThreads = 320;
+constexpr int kMaxSplits = 8;   // CTAs that share an item, a power of two
 // The same value, unknown to the compiler: what is computed from it inside a
 // loop is not kept in registers around the loop.
 __device__ __forceinline__ int fresh(int v) {
@@ -155,13 +156,9 @@ __device__ __forceinline__ uint32_t peer_addr(const void *smem, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(smem)), "r"(rank));
     return a;
 }
-__device__ __forceinline__ float4 ld_peer4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(addr)
+__device__ __forceinline__ void st_peer4(uint32_t addr, float4 v) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                  : "memory");
-    return v;
 }
 __device__ __forceinline__ float2 ld_peer2(uint32_t addr) {
     float2 v;
@@ -764,27 +761,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (p.splits > 1 && !join) {   // no item, or a wait that gave up: meet the others all the same
             cluster_sync();
             cluster_sync();
-            cluster_sync();
         } else if (p.splits > 1) {
             // Join the cluster's partial results.  Every CTA publishes its rows'
-            // (maximum, sum) and, weighted by them, its O in the ring's place; then
-            // rank s sums columns [s D/S, (s+1) D/S) over the ranks, in their order.
+            // (maximum, sum); then it sends its O, weighted by all of them, to the
+            // owners: rank s sums columns [s D/S, (s+1) D/S) over the ranks, in their
+            // order, in the place of its ring, which no product reads any more.
+            // (Stores: nothing waits for a peer's answer.  Loads from the peers took
+            // 4 to 10 us.)
             s_ml[t * 128 + r_thread] = make_float2(m_ref, l);
             cluster_sync();
             float w_own = 0.f;
             if (row_ok) {
-                float top = -INFINITY;
-                for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ld_peer2(peer_addr(&s_ml[t * 128 + r_thread], s)).x);
-                float total = 0.f;
-                for (int s = 0; s < p.splits; ++s) {
-                    const float2 ml = ld_peer2(peer_addr(&s_ml[t * 128 + r_thread], s));
-                    total += ml.y * (ml.x == -INFINITY ? 0.f : ex2(ml.x - top));
-                }
+                float2 ml[kMaxSplits];   // every peer's answer is on its way before the first is used
+#pragma unroll
+                for (int s = 0; s < kMaxSplits; ++s)
+                    ml[s] = s < p.splits ? ld_peer2(peer_addr(&s_ml[t * 128 + r_thread], s)) : make_float2(-INFINITY, 0.f);
+                float top = -INFINITY, total = 0.f;
+#pragma unroll
+                for (int s = 0; s < kMaxSplits; ++s) top = fmaxf(top, ml[s].x);
+#pragma unroll
+                for (int s = 0; s < kMaxSplits; ++s) total += ml[s].y * (ml[s].x == -INFINITY ? 0.f : ex2(ml[s].x - top));
                 // no key seen anywhere: all weights 0; a NaN sum stays NaN
                 if (m_ref != -INFINITY) w_own = ex2(m_ref - top) / total;
                 else if (l != l) w_own = l;
             }
-            float4 *part = reinterpret_cast<float4 *>(sRing) + (t * 128 + r_thread) * (D / 4);
+            // [source][piece][256 rows]: a warp's lanes store 512 bytes in a row
+            float4 *part = reinterpret_cast<float4 *>(sRing) + t * 128 + r_thread;
+            const int per = D / 4 / p.splits, shift = __ffs(per) - 1;   // 16-byte pieces of a row for each rank
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
                 uint32_t r[32] = {};
@@ -794,36 +797,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (!row_ok) continue;
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {   // 16-byte piece i of a row sits at i ^ (row % 8)
+                for (int q = 0; q < 8; ++q) {
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (any_o && w_own != 0.f)
                         v = make_float4(__uint_as_float(r[4 * q]) * w_own, __uint_as_float(r[4 * q + 1]) * w_own,
                                         __uint_as_float(r[4 * q + 2]) * w_own, __uint_as_float(r[4 * q + 3]) * w_own);
-                    part[(c * 8 + q) ^ (r_thread & 7)] = v;
+                    const int i = c * 8 + q;
+                    st_peer4(peer_addr(part + (split * per + (i & (per - 1))) * 256, i >> shift), v);
                 }
             }
             cluster_sync();
             if (row_ok && !aborted) {
-                const int per = D / 4 / p.splits;   // 16-byte pieces of a row for each rank
-                for (int i = split * per; i < (split + 1) * per; ++i) {
-                    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int i = 0; i < per; i += 2) {
+                    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
                     for (int s = 0; s < p.splits; ++s) {
-                        const float4 v = ld_peer4(peer_addr(&part[i ^ (r_thread & 7)], s));
-                        a.x += v.x;
-                        a.y += v.y;
-                        a.z += v.z;
-                        a.w += v.w;
+                        const float4 x = part[(s * per + i) * 256], y = part[(s * per + i + 1) * 256];
+                        a = make_float4(a.x + x.x, a.y + x.y, a.z + x.z, a.w + x.w);
+                        b = make_float4(b.x + y.x, b.y + y.y, b.z + y.z, b.w + y.w);
                     }
-                    __nv_bfloat162 h0 = __floats2bfloat162_rn(a.x, a.y), h1 = __floats2bfloat162_rn(a.z, a.w);
-                    *reinterpret_cast<uint2 *>(dst + i * 4) =
-                        make_uint2(*reinterpret_cast<uint32_t *>(&h0), *reinterpret_cast<uint32_t *>(&h1));
+                    *reinterpret_cast<uint4 *>(dst + (split * per + i) * 4) =
+                        make_uint4(pack16<false>(make_float2(a.x, a.y)), pack16<false>(make_float2(a.z, a.w)),
+                                   pack16<false>(make_float2(b.x, b.y)), pack16<false>(make_float2(b.z, b.w)));
                 }
             }
-            cluster_sync();   // the peers have read this CTA's shared memory
         }
     }
-    if (p.splits > 1 && warp < 2) {   // the softmax warps' three
-        cluster_sync();
+    if (p.splits > 1 && warp < 2) {   // the softmax warps' two
         cluster_sync();
         cluster_sync();
     }
@@ -949,7 +948,7 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const ltx_packed_attention
     if (items > 0x7fffffff / 8) return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: more than 2^28 tiles", w);
     // Too few CTAs for the SMs: split the keys over a cluster, at least two K/V
     // tiles each if one document had them all.
-    while (p.splits < 8 && items * p.splits * 2 <= ctx->sm_count && (int64_t)p.splits * 4 * BKV <= rows_k) p.splits *= 2;
+    while (p.splits < kMaxSplits && items * p.splits * 2 <= ctx->sm_count && (int64_t)p.splits * 4 * BKV <= rows_k) p.splits *= 2;
     p.pairs = (int)pairs;
     // Key heads that go together, the longest pairs of all of them first: as many
     // as keep K and V within 32 MB of L2.  (A head at a time: 48.5 us for 5 x 820
