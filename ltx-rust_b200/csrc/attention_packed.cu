@@ -7,7 +7,8 @@
 // least that many), so a row needs one number and a tile of keys is either
 // whole for all rows of a warp or compared against it.
 //
-// Items are (key head, document, up to 256 query rows), one per CTA of the grid; a
+// Items are (key head, document, up to 256 query rows; 128 where there are few), one
+// per CTA of the grid; a
 // CTA that has told its roles about one takes over the next CTA not yet launched
 // (cluster launch control), so its loads and products run on under the epilogue
 // and unequal items still spread evenly.  A query row is a (token, head of the key head's group): a
@@ -79,7 +80,7 @@ struct Smem {
 // together.  `base`, `before`: where the last search ended (32 documents from
 // base, `before` pairs ahead of them); one for a later pair goes on from there.
 __device__ __forceinline__ bool find_item(const PackedParams &p, int pair, int lane, int &base, int &before, Item &it) {
-    const int per = 2 * p.tile_tokens;
+    const int per = p.item_tiles * p.tile_tokens;
     if (pair < before) base = before = 0;
     for (; base < p.docs; base += 32) {
         int s = 0, e = 0, ks = 0, ke = 0;
@@ -116,7 +117,7 @@ __device__ __forceinline__ bool find_item(const PackedParams &p, int pair, int l
         it.lq = __shfl_sync(0xffffffffu, e, src) - it.qs;
         it.ks = __shfl_sync(0xffffffffu, ks, src);
         it.lk = __shfl_sync(0xffffffffu, ke, src) - it.ks;
-        it.tile0 = 2 * __shfl_sync(0xffffffffu, which, src);
+        it.tile0 = p.item_tiles * __shfl_sync(0xffffffffu, which, src);
         it.doc = base + src;
         return true;
     }
@@ -172,7 +173,7 @@ struct Share {
     int cnt[2], j0, all, nt, prefix;
     __device__ __forceinline__ Share(const PackedParams &p, const Item &it, int split) {
         prefix = p.causal && p.prefix ? min(max(p.prefix[it.doc], 0), it.lk) : 0;
-        nt = it.lq > (it.tile0 + 1) * p.tile_tokens ? 2 : 1;   // query tiles that hold tokens
+        nt = p.item_tiles == 2 && it.lq > (it.tile0 + 1) * p.tile_tokens ? 2 : 1;   // query tiles that hold tokens
         int n[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -933,7 +934,7 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const ltx_packed_attention
              packed_map(&tv, v_dev, rows_k, kv_heads, head_dim, ldv, v_dtype == LTX_F16, 1, BKV);
     if (!ok) return fail(ctx, LTX_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed", w);
     PackedParams p{static_cast<__nv_bfloat16 *>(out_dev), ldo, q_offsets_dev, k_offsets_dev, prefix_dev, slopes_dev,
-                   docs, rows_q, rows_k, kv_heads, group, tokens, causal, 0, 1, 1, scale, softcap, ctx->timeout_flag};
+                   docs, rows_q, rows_k, kv_heads, group, tokens, causal, 0, 1, 1, 2, scale, softcap, ctx->timeout_flag};
     // Few rows per document over many keys, by their averages (the host does
     // not see the offsets): the kernel whose tiles have keys as rows and whose
     // CTAs share every document.  Under some 512 keys its join and its start
@@ -942,13 +943,26 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const ltx_packed_attention
     const int64_t rows_per_doc = (int64_t)((rows_q + some - 1) / some) * group;
     if (rows_per_doc <= kMaxFewRows && rows_k / docs >= 512)
         return attention_packed_few(ctx, tk, tv, q_dev, ldq, p, heads, head_dim, v_dtype == LTX_F16, (int)rows_per_doc);
-    // Pairs of query tiles over all documents: sum ceil(lq / per) <= (rows + docs (per - 1)) / per.
-    const int64_t per = 2 * tokens;
-    const int64_t pairs = (rows_q + (int64_t)some * (per - 1)) / per, items = pairs * kv_heads;
+    // Items over all documents: sum ceil(lq / per) <= (rows + docs (per - 1)) / per.
+    auto items_of = [&](int64_t per) { return (rows_q + (int64_t)some * (per - 1)) / per; };
+    // Too few CTAs for the SMs: split the keys over a cluster, at least one K/V tile
+    // each if one document had them all (two: 25.1 us for 546 x 913 capped causal
+    // rows x 2/1 heads, one: 20.7).
+    auto splits_of = [&](int64_t items) {
+        int s = 1;
+        while (s < kMaxSplits && items * s * 2 <= ctx->sm_count && (int64_t)s * 2 * BKV <= rows_k) s *= 2;
+        return s;
+    };
+    // Two query tiles to an item share its K and V; where that leaves half of the
+    // SMs without work even so, a tile each: half the exponentials on a CTA's way
+    // (the same rows 20.7 -> 17.0; 148 x 148 capped with slopes x 8/1 heads 21 -> 17).
+    // Where it does not, a tile each means fewer shares of the keys: 4887 capped causal
+    // rows of 7 documents x 1 head took 28.6 us instead of 19.9.
+    const int64_t twos = items_of(2 * tokens) * kv_heads;
+    if (twos * splits_of(twos) * 2 <= ctx->sm_count) p.item_tiles = 1;
+    const int64_t pairs = items_of(p.item_tiles * tokens), items = pairs * kv_heads;
     if (items > 0x7fffffff / 8) return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: more than 2^28 tiles", w);
-    // Too few CTAs for the SMs: split the keys over a cluster, at least two K/V
-    // tiles each if one document had them all.
-    while (p.splits < kMaxSplits && items * p.splits * 2 <= ctx->sm_count && (int64_t)p.splits * 4 * BKV <= rows_k) p.splits *= 2;
+    p.splits = splits_of(items);
     p.pairs = (int)pairs;
     // Key heads that go together, the longest pairs of all of them first: as many
     // as keep K and V within 32 MB of L2.  (A head at a time: 48.5 us for 5 x 820

@@ -18,7 +18,7 @@ struct PackedParams {
     int64_t ldo;
     const int *qo, *ko, *prefix;
     const float *slopes;
-    int docs, rows_q, rows_k, kv_heads, group, tile_tokens, causal, pairs, splits, head_group;
+    int docs, rows_q, rows_k, kv_heads, group, tile_tokens, causal, pairs, splits, head_group, item_tiles;
     float scale, softcap;
     int *flag;
 };
