@@ -3,8 +3,10 @@
 // with the rotation in the same pass.
 //
 // Both are bound by the bytes they move.  The table writes rot_dim * 4 bytes
-// per position; the norm reads and writes every query and key value once and
-// adds one table row per token.
+// per position: 14.4 us for 131072 x 128, 4.7 TB/s, where a fill of the same bytes
+// takes 12.4.  The norm reads and writes every query and key value once and adds
+// one table row per token: 80 us for 12288 x (32 + 32) heads x 128 in bf16, 5.1 TB/s
+// (a copy of that size runs at 6.3).
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -41,7 +43,7 @@ struct TableParams {
 // cos(pi r/2) = C(r^2) with S of degree 3 and C of degree 4, fitted here to the
 // least absolute error: with the f32 roundings 9.4e-8 at most, 2e-8 root mean
 // square.  (A value took 16 f64 and conversion cycles more with the reduction in
-// f64: 18.4 us for 131072 x 64 instead of the figure below.)
+// f64: 18.4 us for 131072 x 128 instead of 14.4.)
 struct SinCos {
     float s[4], c[5];   // the polynomials, the amplitude multiplied in
     __device__ __forceinline__ explicit SinCos(float a)
@@ -194,7 +196,8 @@ __global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(NormRopeParams p)
 // rotation once per warp: out = (x c gamma + partner s gamma') / rms, so a
 // value costs a conversion, its square, two products and its share of the
 // partner's fetch (packed: a pair of the half layout lies rot_dim/16 lanes apart,
-// one of the interleaved layout in the same word).
+// one of the interleaved layout in the same word).  Four heads deep at 63 registers:
+// two, or more blocks to an SM with spills, 3 to 26% slower, eight 2 to 40%.
 constexpr int kHeadsDeep = 4;
 
 template <typename T>
