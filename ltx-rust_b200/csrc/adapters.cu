@@ -1209,8 +1209,8 @@ cudaError_t run_pair(const ltx_ctx *ctx, AdapterParams p, int epilogue, const CU
 // stream once.  More: the widest tile (the fewest bytes per product) that still
 // makes work for two SMs in five; a cluster's joined sums and a builder's wider
 // copies cost more than they save below that.  Measured, us at 256 / 128 / 64 / 32 /
-// 16 tokens: 153 x 600 x 448 50 / 34 / 22 / 16 / 13; 512 x 1024 x 2048 41 / 21 / 18 /
-// 23 / 31; 200 x 4096 x 4096 27.6 / 27.3 / 29 / 44 / 64; 512 x 4096 x 4096 37 / 39 / 47 / 76.
+// 16 tokens: 153 x 600 x 448 - / 25 / 18 / 16 / 14; 512 x 1024 x 2048 41 / 22 / 19 /
+// 24 / 32; 200 x 4096 x 4096 29 / 27 / 32 / 44 / 65; 512 x 4096 x 4096 35 / 40 / 50 / 80.
 int tokens_for(int m, int n, int sms) {
     if (m <= 64) return m <= 16 ? 16 : m <= 32 ? 32 : 64;
     for (int t = m <= 128 ? 128 : 256; t > 16; t /= 2)

@@ -950,13 +950,13 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const ltx_packed_attention
     if (rows_per_doc <= kMaxFewRows && rows_k / docs >= 512)
         return attention_packed_few(ctx, tk, tv, q_dev, ldq, p, heads, head_dim, v_dtype == LTX_F16, (int)rows_per_doc);
     // Items over all documents: sum ceil(lq / per) <= (rows + docs (per - 1)) / per.
-    auto items_of = [&](int64_t per) { return (rows_q + (int64_t)some * (per - 1)) / per; };
+    auto items_of = [&p, some](int64_t per) { return (p.rows_q + (int64_t)some * (per - 1)) / per; };
     // Too few CTAs for the SMs: split the keys over a cluster, at least one K/V tile
     // each if one document had them all (two: 25.1 us for 546 x 913 capped causal
     // rows x 2/1 heads, one: 20.7).
-    auto splits_of = [&](int64_t items) {
+    auto splits_of = [&p, ctx](int64_t items) {
         int s = 1;
-        while (s < kMaxSplits && items * s * 2 <= ctx->sm_count && (int64_t)s * 2 * BKV <= rows_k) s *= 2;
+        while (s < kMaxSplits && items * s * 2 <= ctx->sm_count && (int64_t)s * 2 * BKV <= p.rows_k) s *= 2;
         return s;
     };
     // Two query tiles to an item share its K and V; where that leaves half of the
@@ -971,9 +971,9 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const ltx_packed_attention
     p.splits = splits_of(items);
     p.pairs = (int)pairs;
     // Key heads that go together, the longest pairs of all of them first: as many
-    // as keep K and V within 32 MB of L2.  (A head at a time: 48.5 us for 5 x 820
-    // causal rows x 16/4 heads, 44 with all four together; all 32 heads of an 8192
-    // long document together: 949 us, 899 a head at a time.)
+    // as keep K and V within 32 MB of L2.  (5 x 820 capped causal rows x 16/4 heads:
+    // 44.7 us a head at a time, 35.3 all four together.  8192 x 32 heads: 892 a head
+    // at a time, 942 all together, 900 in eights.)
     p.head_group = (int)std::clamp<int64_t>((32 << 20) / std::max<int64_t>(1, (int64_t)rows_k * head_dim * 4), 1, kv_heads);
     const bool fixed = !slopes_dev && v_dtype == LTX_BF16 && softcap * kLog2e <= kFixedCap;
     const Mode mode = softcap > 0.f ? (fixed ? kCapFixed : kCap) : slopes_dev ? kBias : kPlain;
