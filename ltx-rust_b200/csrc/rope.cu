@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_any_kernel(NormRopeParams p)
 // value costs a conversion, its square, two products and its share of the
 // partner's fetch (packed: a pair of the half layout lies rot_dim/16 lanes apart,
 // one of the interleaved layout in the same word).  Four heads deep at 63 registers:
-// two, or more blocks to an SM with spills, 3 to 26% slower, eight 2 to 40%.
+// two 6 to 35% slower, eight 2 to 45%, more blocks to an SM (spills) 3 to 80%.
 constexpr int kHeadsDeep = 4;
 
 template <typename T>
