@@ -248,6 +248,28 @@ def test_gemm_adapters_every_tile_width(ctx, m, n, k, rank, adapters, lengths, e
 
 
 @pytest.mark.parametrize("epi", [0, 3])
+@pytest.mark.parametrize("m,n,k,rank,adapters,lengths", [
+    (2500, 4096, 64, 72, 9, [1, 2]), (2100, 2601, 64, 200, 30, [5]), (256, 9000, 2048, 8, 2, [1]),
+    (500, 2100, 128, 136, 12, [3, 1]), (64, 1000, 64, 24, 60, [1])])
+def test_gemm_adapters_more_adapter_blocks_than_others(ctx, m, n, k, rank, adapters, lengths, epi):
+    """Mixed tiles whose adapters take as many blocks as K or more, in ranks that fill no whole block."""
+    adapter_case(ctx, m, n, k, rank, runs(m, lengths, adapters, start=1), epi, adapters, bias=False, gate=2)
+
+
+@pytest.mark.parametrize("m,n", [(20, 300), (300, 700), (2500, 4096)])
+def test_gemm_adapters_after_a_call_that_left_nan(ctx, m, n):
+    """What an earlier call left in the workspace, NaN here, reaches no row of a later one."""
+    import ltx_b200
+    x = torch.full((m, 128), float("nan"), device="cuda", dtype=BF16)
+    w, a, b = (torch.ones(*s, device="cuda", dtype=BF16) for s in ((n, 128), (2, 256, 128), (2, n, 256)))
+    out = torch.zeros(m, n, device="cuda")
+    ltx_b200.gemm_adapters(ctx, x, w, out, ints([i % 2 for i in range(m)]), a, b, torch.ones(2, device="cuda"), epilogue=2)
+    ctx.synchronize()
+    assert bool(out.isnan().all())
+    adapter_case(ctx, m, n, 128, 24, runs(m, [2, 1], 3), 2, 3)
+
+
+@pytest.mark.parametrize("epi", [0, 3])
 def test_gemm_adapters_strides_and_odd_rows(ctx, epi):
     adapter_case(ctx, 45, 77, 96, 16, runs(45, [4, 9], 3), epi, 3, x_pad=8, o_pad=3)
     adapter_case(ctx, 300, 200, 128, 16, runs(300, [4, 90], 3), epi, 3, x_pad=24, o_pad=4)
@@ -440,6 +462,23 @@ def test_attention_packed_few_rows_long_keys(ctx, lq, lk, h, hk, d, kw, vt):
 def test_attention_packed_many_short_documents(ctx, causal):
     """More documents than CTAs and than one search sees at once, some without rows or keys."""
     attention_case(ctx, [(7 * i) % 61 for i in range(900)], [(11 * i) % 83 for i in range(900)], 4, 2, 64, causal=causal)
+
+
+@pytest.mark.parametrize("causal,cap,slope", [(False, 0.0, False), (True, 0.0, True), (True, 25.0, False)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_packed_rows_of_one_document_among_empty_ones(ctx, d, causal, cap, slope):
+    """Few rows a document on average, nearly all of them in one: row tiles of one document behind one another on the
+    line of work, documents without rows or keys between."""
+    attention_case(ctx, [0, 300] + [0] * 28 + [1, 2], [700, 900] + [640, 0] * 14 + [5, 1200], 4, 2, d, causal=causal, cap=cap,
+                   slope=slope)
+
+
+@pytest.mark.parametrize("vt", [BF16, F16])
+@pytest.mark.parametrize("cap", [0.0, 20.0, 60.0])
+def test_attention_packed_few_items_share_keys(ctx, cap, vt):
+    """So few items that clusters of eight share their keys, one tile each or none."""
+    attention_case(ctx, [100, 30], [1100, 90], 3, 1, 128, vt, cap=cap, q_std=2.0)
+    attention_case(ctx, [100, 30], [1100, 90], 2, 1, 64, vt, cap=cap, causal=True, prefix=[40, 95], q_std=2.0)
 
 
 @pytest.mark.parametrize("vt", [BF16, F16])
