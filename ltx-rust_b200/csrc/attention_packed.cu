@@ -594,11 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (it.kvh < 0) break;
                 const Share sh(p, it, split);
                 const uint32_t used = it.load0;
-                if (sh.all == 0) {   // nothing to see: O is final as it is
-                    umma_commit(&pv_done[0]);
-                    umma_commit(&pv_done[1]);
-                    continue;
-                }
+                if (sh.all == 0) continue;   // nothing to see, and nobody waits
                 auto wait_load = [&](uint32_t s, int code) {
                     return mbar_wait(&slot_full[s % kRing], (s / kRing) & 1, p.flag, code, &aborted);
                 };
@@ -647,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                             sdesc_sw128(v_addr + kk * 2048, L::HALF, 1024), idesc_pv,
                                             (j > skip(t) || kk > 0) ? 1u : 0u);
                         }
-                        if (!next) umma_commit(&pv_done[t]);
+                        if (!next && sh.cnt[t] > 0) umma_commit(&pv_done[t]);
                         if (next && j + 1 >= skip(t)) issue_qk(t, j + 1);
                     }
                     if (!ok) break;
@@ -667,9 +663,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float sc = rs.kCapped ? p.scale / p.softcap : p.scale * kLog2e;
         rs.sc = make_float2(sc, sc);
         if constexpr (rs.kCapped) rs.cap2 = p.softcap * kLog2e;
-        uint32_t n_items = 0, n_s = 0;
+        uint32_t n_items = 0, phase = 0;   // of s_full[t] (bit 0) and pv_done[t] (bit 1)
         float m_ref = -INFINITY, l = 0.f;   // a row's maximum that P is taken against (log2 domain), its sum
-        bool row_ok = false, any_o = false, join = false;
+        bool row_ok = false, any_o = false, other_o = false, join = false;
         __nv_bfloat16 *dst = nullptr;
         while (!aborted) {
             // The item stays in shared memory (volatile: read again behind the
@@ -685,6 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int token = (i.tile0 + t) * tt + r_in / p.group;   // in the document
                 const bool ok = t < sh.nt && r_in < tt * p.group && token < i.lq;
                 n_mine = t ? sh.cnt[1] : sh.cnt[0];
+                other_o = (t ? sh.cnt[0] : sh.cnt[1]) > 0;
                 const int top = (sh.j0 + n_mine - 1) * BKV;       // first key of the tile to begin with
                 row_ok = ok;
                 left = ok ? limit_of(p, i, token, sh.prefix) - top : kNoRow;
@@ -702,8 +699,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool active = left_min != kNoRow;   // the warp holds rows
             for (; n_mine > 0; --n_mine, left += BKV, left_min += BKV, place += BKV) {
                 // warp-uniform outcome: the tcgen05.ld/st below are warp-collective
-                if (!warp_wait(&s_full[t], n_s & 1, p.flag, 311, &aborted)) break;
-                ++n_s;
+                if (!warp_wait(&s_full[t], phase & 1, p.flag, 311, &aborted)) break;
+                phase ^= 1;
                 if (active) {
                     tc_fence_after();
                     rs.set_tile(place);
@@ -728,9 +725,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[t]);
             }
-            // O_t is final once the last P.V has completed; in a cluster the ring is free once both tiles' have.
-            warp_wait(&pv_done[t], n_items & 1, p.flag, 312, &aborted);
-            if (p.splits > 1) warp_wait(&pv_done[t ^ 1], n_items & 1, p.flag, 314, &aborted);
+            // O_t is final once the last P.V has completed; in a cluster (one item) the ring
+            // is free once both tiles' have.  A tile without K/V tiles has no P.V: nothing
+            // would hold the MMA thread back from the next item's phase of pv_done, which
+            // p_full does where there are some.
+            if (any_o) {
+                warp_wait(&pv_done[t], phase >> 1, p.flag, 312, &aborted);
+                phase ^= 2;
+            }
+            if (p.splits > 1 && other_o) warp_wait(&pv_done[t ^ 1], 0, p.flag, 314, &aborted);
             tc_fence_after();
             const int r_now = fresh(r_thread);
             dst = p.out + ((int64_t)it.qs + (it.tile0 + t) * tt + r_now / p.group) * p.ldo +

@@ -458,6 +458,21 @@ def test_attention_packed_few_rows_long_keys(ctx, lq, lk, h, hk, d, kw, vt):
     attention_case(ctx, lq, lk, h, hk, d, vt, **kw)
 
 
+@pytest.mark.parametrize("d,cap,slope", [(64, 0.0, False), (128, 0.0, True), (128, 20.0, False)])
+def test_attention_packed_queries_far_ahead_of_their_keys(ctx, d, cap, slope):
+    """Many more tiles than SMs, most of which see no key: a CTA takes several of them behind one that sees some."""
+    attention_case(ctx, [4096], [520], 32, 32, d, causal=True, cap=cap, slope=slope)
+    attention_case(ctx, [2000, 700, 1], [300, 1, 300], 16, 4, d, causal=True, prefix=[0, 1, 2], cap=cap, slope=slope)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [130, 300])
+def test_attention_packed_runs_of_documents_without_keys(ctx, rows, d):
+    """Runs of documents without keys behind documents of several K/V tiles, of one query tile and of two."""
+    attention_case(ctx, [rows] * 400, [700 if i % 40 == 0 else 0 for i in range(400)], 2, 2, d)
+    attention_case(ctx, [rows] * 400, [700 if i % 40 < 3 else 0 for i in range(400)], 2, 1, d, F16)
+
+
 @pytest.mark.parametrize("causal", [False, True])
 def test_attention_packed_many_short_documents(ctx, causal):
     """More documents than CTAs and than one search sees at once, some without rows or keys."""
