@@ -207,10 +207,11 @@ constexpr float kFixedCap = 75.f;   // 2^75 by 2^29 keys by values of 2^23 stay 
 template <int MODE>
 struct RowScores {
     static constexpr bool kCapped = MODE == kCap || MODE == kCapFixed;
-    float2 sc;              // kPlain, kBias: scale log2e; capped: scale / cap
+    float2 sc;              // kPlain, kBias: scale log2e; capped: scale / cap, 0 in a thread without a row
     float cap2;             // capped: cap log2e
     float slope;            // slope log2e, 0 without
     float place;            // the row's key less the tile's first
+    int ends;               // capped: the document's keys in the tile, BKV where it goes on
     int side;               // 1: the tile's keys lie before it for every row, -1: behind, 0: both
     __device__ __forceinline__ void set_tile(int pl) {
         if constexpr (MODE == kBias || MODE == kCap) {
@@ -218,7 +219,10 @@ struct RowScores {
             side = __all_sync(0xffffffffu, pl >= BKV - 1) ? 1 : __all_sync(0xffffffffu, pl <= 0) ? -1 : 0;
         }
     }
-    // 32 scores, keys e0 + 0..31: raw products to the log2 domain (kPlain: as they are)
+    // 32 scores, keys e0 + 0..31: raw products to the log2 domain (kPlain: as they are).
+    // The warp's rows agree on the form of tanh, which moves bits.  What lies outside
+    // the document has no say in it: threads without a row have scores of 0, and the
+    // keys around the document's end take the form that is right at every size.
     __device__ __forceinline__ void apply(uint32_t (&r)[32], int e0) const {
         if constexpr (MODE == kPlain) return;
         float2 v[16];
@@ -229,6 +233,7 @@ struct RowScores {
             float big = 0.f;
 #pragma unroll
             for (int u = 0; u < 16; ++u) big = fmaxf(big, fmaxf(fabsf(v[u].x), fabsf(v[u].y)));
+            if (e0 + 32 > ends) big = 2.f;
             if (!__any_sync(0xffffffffu, big > 0.5f)) {
 #pragma unroll
                 for (int u = 0; u < 16; ++u) v[u] = __fmul2_rn(tanh_small2(v[u]), make_float2(cap2, cap2));
@@ -684,6 +689,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 other_o = (t ? sh.cnt[0] : sh.cnt[1]) > 0;
                 const int top = (sh.j0 + n_mine - 1) * BKV;       // first key of the tile to begin with
                 row_ok = ok;
+                if constexpr (rs.kCapped) {
+                    rs.sc = ok ? make_float2(sc, sc) : make_float2(0.f, 0.f);
+                    rs.ends = min(BKV, i.lk - top);
+                }
                 left = ok ? limit_of(p, i, token, sh.prefix) - top : kNoRow;
                 left_min = __reduce_min_sync(0xffffffffu, left);
                 place = token + i.lk - i.lq - top;
@@ -722,6 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     aborted = __any_sync(0xffffffffu, aborted);
                     clean = BKV;
                 }
+                if constexpr (rs.kCapped) rs.ends = BKV;   // the last tile went first
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[t]);
             }

@@ -546,6 +546,31 @@ def test_attention_packed_keeps_other_documents_values_out(ctx):
     assert torch.equal(a[70:270], b[70:270]) and bool(torch.isfinite(a).all())
 
 
+@pytest.mark.parametrize("vt,cap,causal", [(BF16, 20.0, False), (BF16, 20.0, True), (F16, 20.0, False), (BF16, 60.0, True)])
+@pytest.mark.parametrize("h,hk,d", [(2, 2, 128), (3, 1, 64)])
+def test_attention_packed_capped_bits_are_the_documents_own(ctx, h, hk, d, vt, cap, causal):
+    """Capped scores, which have forms of tanh for small, middle and large ones: a document's rows are the same bits
+    whatever its neighbours' queries, keys and values hold and whatever ran before."""
+    import ltx_b200
+    g = gen(h, d, int(cap))
+    lens, own, n = [70, 200, 90], slice(70, 270), 360
+    q, k, v = normal(g, n, h * d), normal(g, n, hk * d), normal(g, n, hk * d, dtype=vt)
+    o = offsets(lens)
+
+    def attend(q, k, v):
+        out = torch.zeros(n, h * d, device="cuda", dtype=BF16)
+        ltx_b200.attention_packed(ctx, q, k, v, out, o, o, h, hk, 0.2, head_dim=d, softcap=cap, causal=causal)
+        return out[own]
+
+    want = attend(q, k, v)
+    for size in (30.0, 1e4, float("nan")):
+        q2, k2, v2 = q * size, k * size, v * size
+        attend(q2, k2, v2)          # what it leaves in shared memory
+        for t, t2 in ((q, q2), (k, k2), (v, v2)):
+            t2[own] = t[own]
+        assert torch.equal(attend(q2, k2, v2), want)
+
+
 def test_attention_packed_nothing_to_do(ctx):
     import ltx_b200
     q = torch.ones(4, 128, device="cuda", dtype=BF16)
