@@ -277,6 +277,13 @@ struct RowScores {
 // its runs do).
 constexpr uint32_t kPolyPairs = 0x1111u;
 
+// The larger of two, NaN if either is (the polynomial exponential does not keep a NaN).
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+
 // One row's 128 scores of a K/V tile: S from TMEM, the row's maximum, P back
 // into TMEM, the row's sum.  `left` keys are the row's to see (`masked`: some row
 // of the warp does not see all); O is moved along when the reference grows.
@@ -298,7 +305,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_tmem, uint32_t o_tmem, c
     for (int u = 0; u < 8; ++u) m8[u] = -INFINITY;
     auto look = [&](const uint32_t (&r)[32]) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) m8[e & 7] = fmaxf(m8[e & 7], __uint_as_float(r[e]));
+        for (int e = 0; e < 32; ++e) m8[e & 7] = max_nan(m8[e & 7], __uint_as_float(r[e]));
     };
     if constexpr (MODE != kPlain) {
         tmem_ld_32x32b_x32(s_tmem + 64, rh[0]);
@@ -340,13 +347,14 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_tmem, uint32_t o_tmem, c
         look(rh[0]);
         look(rh[1]);
     }
-    float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])), fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
+    float mx = max_nan(max_nan(max_nan(m8[0], m8[1]), max_nan(m8[2], m8[3])),
+                       max_nan(max_nan(m8[4], m8[5]), max_nan(m8[6], m8[7])));
     if constexpr (MODE == kPlain) mx *= rs.sc.x;   // scale > 0: max(s * scale) = scale * max(s)
     // The rows of one warp decide together: tcgen05.ld/st are
     // warp-collective (.sync.aligned), so the O rescale runs for the
     // whole warp when any of its rows needs it; a row that does not
     // keeps its reference (alpha = 1).
-    const bool grow = mx > m_ref + kRescaleLog2;
+    const bool grow = !(mx <= m_ref + kRescaleLog2);   // a NaN becomes the reference, and with it all of the row
     if (__any_sync(0xffffffffu, grow)) {
         // O_t and l are relative to m_ref; move them to mx (the P.V before
         // was issued before this tile's QK, whose completion was waited for).

@@ -60,12 +60,12 @@ struct ScoreMod {
 
 // 2^x on the FMA pipe, two at a time, as exp2_fma2 of attention.cu: x = n + f with
 // n = rint(x), 2^f by a cubic (7.7e-5 relative, under f16's half step), 2^n added
-// to the exponent; below 2^-120 it stays there.  A NaN stays one.
+// to the exponent; below 2^-120 it stays there.  Not for a NaN (whose exponent the
+// addition would change): the caller's other values have to carry it.
 __device__ __forceinline__ float2 exp2_poly2(float2 x) {
     constexpr float kRound = 12582912.0f;   // 1.5 * 2^23
     constexpr float c0 = 0x1.fff682p-1f, c1 = 0x1.62f1e0p-1f, c2 = 0x1.f0e03ap-3f, c3 = 0x1.c46242p-5f;
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-120.f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-120.f));
+    x = make_float2(fmaxf(x.x, -120.f), fmaxf(x.y, -120.f));
     const float2 t = __fadd2_rn(x, make_float2(kRound, kRound));
     const float2 n = __fadd2_rn(t, make_float2(-kRound, -kRound));
     const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);

@@ -571,6 +571,31 @@ def test_attention_packed_capped_bits_are_the_documents_own(ctx, h, hk, d, vt, c
         assert torch.equal(attend(q2, k2, v2), want)
 
 
+@pytest.mark.parametrize("kw", [{}, dict(slope=True), dict(softcap=60.0), dict(softcap=20.0)])
+@pytest.mark.parametrize("lq,lk", [(256, 256), (130, 512), (1, 3000)])
+def test_attention_packed_a_nan_that_a_row_sees_stays_one(ctx, lq, lk, kw):
+    """A NaN key makes the rows that see it NaN, wherever it stands, and no other row; a NaN query its own row."""
+    import ltx_b200
+    g = gen(lq, lk)
+    q, k, v = normal(g, lq, 128), normal(g, lk, 128), normal(g, lk, 128).abs()
+    kw = dict(kw)
+    slopes = torch.full((1,), 0.01, device="cuda") if kw.pop("slope", False) else None
+    place = torch.arange(lq, device="cuda") + lk - lq
+    for j in (0, 1, 3, 8, 40, 64, 120, 127, 128, 201, lk - 1):
+        k2 = k.clone()
+        k2[j] = float("nan")
+        out = torch.zeros(lq, 128, device="cuda", dtype=BF16)
+        ltx_b200.attention_packed(ctx, q, k2, v, out, ints([0, lq]), ints([0, lk]), 1, 1, 0.09, causal=True, slopes=slopes, **kw)
+        ctx.synchronize()
+        assert torch.equal(out.isnan(), (place >= j)[:, None].expand_as(out)), j
+        assert bool(out.isfinite()[place < j].all())
+    q[lq // 2] = float("nan")
+    out = torch.zeros(lq, 128, device="cuda", dtype=BF16)
+    ltx_b200.attention_packed(ctx, q, k, v, out, ints([0, lq]), ints([0, lk]), 1, 1, 0.09, slopes=slopes, **kw)
+    ctx.synchronize()
+    assert torch.equal(out.isnan().all(1), torch.arange(lq, device="cuda") == lq // 2)
+
+
 def test_attention_packed_nothing_to_do(ctx):
     import ltx_b200
     q = torch.ones(4, 128, device="cuda", dtype=BF16)
