@@ -703,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 left = ok ? limit_of(p, i, token, sh.prefix) - top : kNoRow;
                 left_min = __reduce_min_sync(0xffffffffu, left);
-                place = token + i.lk - i.lq - top;
+                place = key_beside(i.lq, i.lk, token) - top;
                 if constexpr (MODE == kBias || MODE == kCap)
                     rs.slope = p.slopes && ok ? p.slopes[i.kvh * p.group + r_in % p.group] * kLog2e : 0.f;
                 // V rows behind the document's end, in the first tile loaded: tile

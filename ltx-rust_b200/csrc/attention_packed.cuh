@@ -46,6 +46,11 @@ __device__ __forceinline__ int limit_of(const PackedParams &p, const Item &it, i
     return max(prefix, (int)min((int64_t)it.lk, max((int64_t)0, upto)));
 }
 
+// The key from which token `t`'s distances count.  A token that stands before the
+// first key takes that one: all its distances are then less by the same number, which
+// the softmax does not see and f32 scores would lose bits to.
+__device__ __forceinline__ int key_beside(int lq, int lk, int t) { return max(t + lk - lq, 0); }
+
 // How a raw score becomes one in the log2 domain when it is capped or biased.
 struct ScoreMod {
     float scale, twice_over_cap, cap2;   // scale; 2 log2e / cap (0 = no cap); cap log2e

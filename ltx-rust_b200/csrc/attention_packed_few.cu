@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(kFewThreads, 1)
                 const int prefix = p.causal && p.prefix ? min(max(p.prefix[doc], 0), d.lk) : 0;
                 const Item it{d.qs, d.lq, d.ks, d.lk, 0, doc, w.kvh, 0};
                 r_lim[key] = ok ? limit_of(p, it, token, prefix) : 0;
-                r_place[key] = token + d.lk - d.lq;
+                r_place[key] = key_beside(d.lq, d.lk, token);
                 r_slope[key] = ok && p.slopes ? p.slopes[w.kvh * p.group + key % p.group] * kLog2e : 0.f;
                 r_ref[key] = -INFINITY;
                 r_out[key] = ok ? (int64_t)(d.qs + token) * p.ldo + (w.kvh * p.group + key % p.group) * D : -1;

@@ -571,6 +571,43 @@ def test_attention_packed_capped_bits_are_the_documents_own(ctx, h, hk, d, vt, c
         assert torch.equal(attend(q2, k2, v2), want)
 
 
+def far_rows(q, k, v, lq, lk, rows, slope, scale):
+    """Rows `rows` of one document and head in 64 bits, and a bound: the distance counts for a key's weight, from the
+    nearest key on, not for the row as a whole."""
+    Q, K, V = q[rows].to(F64), k[:lk].to(F64), v[:lk].to(F64)
+    raw, j = Q @ K.t() * scale, torch.arange(lk, device="cuda")
+    away = slope * (rows[:, None] + lk - lq - j[None]).abs().to(F64)
+    p = torch.softmax(raw - away, -1)
+    # a score's error: its product's sums, and the 2^-23 of its own size in the log2 domain, four roundings
+    e = (Q.abs() @ K.abs().t() * scale).amax(-1, keepdim=True) * 68 * 2.0 ** -24 + \
+        4 * (raw.abs() + away - away.amin(-1, keepdim=True)) * 2.0 ** -23
+    o, mass = p @ V, p @ V.abs()
+    # P's rounding and the exponential's polynomial as in attention64; an error of a score moves its weight and the sum
+    t = mass * (HALF[BF16] + 1e-4 + (lk + 8) * 2.0 ** -24 + 2 * (p * e).sum(-1, keepdim=True)) + 2 * (p * e) @ V.abs()
+    return o, t + (o.abs() + t) * HALF[BF16]
+
+
+@pytest.mark.parametrize("lk,others", [(64, 0), (200, 0), (64, 16000)])
+def test_attention_packed_distance_of_rows_far_from_all_keys(ctx, lk, others):
+    """A million queries over a few keys: the first stand 2^20 keys before the nearest, and the weights of the keys among
+    each other are those of the distances between them all the same.  Once in the kernel for few rows, which takes the
+    batch where its other documents hold the most keys."""
+    import ltx_b200
+    lq, slope, scale = 1 << 20, 2.0 ** -0.25, 0.125
+    g = gen(lk, others)
+    nk = lk + 600 * others
+    q, k, v = normal(g, lq + 1, 64), torch.zeros(nk, 64, device="cuda", dtype=BF16), torch.zeros(nk, 64, device="cuda", dtype=BF16)
+    k[:lk], v[:lk] = normal(g, lk, 64), normal(g, lk, 64)
+    out = torch.zeros_like(q)
+    qo, ko = ([0, lq], [0, lk]) if not others else ([0, lq] + [lq + 1] * others, [0, lk] + [nk] * others)
+    ltx_b200.attention_packed(ctx, q, k, v, out, ints(qo), ints(ko), 1, 1, scale, head_dim=64,
+                              slopes=torch.tensor([slope], device="cuda"))
+    ctx.synchronize()
+    rows = torch.cat([torch.arange(0, 300), torch.arange(lq // 2, lq // 2 + 100), torch.arange(lq - 300, lq)]).cuda()
+    want, tol = far_rows(q, k, v, lq, lk, rows, slope, scale)
+    within(out[rows], want, tol)
+
+
 @pytest.mark.parametrize("kw", [{}, dict(slope=True), dict(softcap=60.0), dict(softcap=20.0)])
 @pytest.mark.parametrize("lq,lk", [(256, 256), (130, 512), (1, 3000)])
 def test_attention_packed_a_nan_that_a_row_sees_stays_one(ctx, lq, lk, kw):
