@@ -197,8 +197,11 @@ struct Share {
 // What changes a row's scores: nothing but the scale, a bias by distance, or a cap
 // (and perhaps a bias).  kCapFixed: a cap alone, of at most kFixedCap in the log2
 // domain, with bf16 V: 2^score fits f32 and bf16 as it is, so no maximum is kept
-// and the scores are gone through once.
-enum Mode { kPlain = 0, kBias = 1, kCap = 2, kCapFixed = 3 };
+// and the scores are gone through once.  kCapFar: a cap above kExpCap (log2 domain),
+// where tanh_exp would move small scores by more than half a step of f16's P (2e-4 at
+// kExpCap); tanh_any2 for every cap took 1920 us instead of 1775 (8192 x 32 x 128, f16).
+enum Mode { kPlain = 0, kBias = 1, kCap = 2, kCapFixed = 3, kCapFar = 4 };
+constexpr float kExpCap = 512.f;
 constexpr float kFixedCap = 75.f;   // 2^75 by 2^29 keys by values of 2^23 stay within f32
 
 // Scores of one row in the log2 domain.  The scale goes with the log2e, and the
@@ -206,7 +209,8 @@ constexpr float kFixedCap = 75.f;   // 2^75 by 2^29 keys by values of 2^23 stay 
 // lies on one side for every row of the warp needs one multiply-add more.
 template <int MODE>
 struct RowScores {
-    static constexpr bool kCapped = MODE == kCap || MODE == kCapFixed;
+    static constexpr bool kCapped = MODE == kCap || MODE == kCapFixed || MODE == kCapFar;
+    static constexpr bool kCappedOnline = MODE == kCap || MODE == kCapFar;
     float2 sc;              // kPlain, kBias: scale log2e; capped: scale / cap, 0 in a thread without a row
     float cap2;             // capped: cap log2e
     float slope;            // slope log2e, 0 without
@@ -214,7 +218,7 @@ struct RowScores {
     int ends;               // capped: the document's keys in the tile, BKV where it goes on
     int side;               // 1: the tile's keys lie before it for every row, -1: behind, 0: both
     __device__ __forceinline__ void set_tile(int pl) {
-        if constexpr (MODE == kBias || MODE == kCap) {
+        if constexpr (MODE == kBias || kCappedOnline) {
             place = (float)pl;
             side = __all_sync(0xffffffffu, pl >= BKV - 1) ? 1 : __all_sync(0xffffffffu, pl <= 0) ? -1 : 0;
         }
@@ -229,7 +233,10 @@ struct RowScores {
 #pragma unroll
         for (int u = 0; u < 16; ++u)
             v[u] = __fmul2_rn(make_float2(__uint_as_float(r[2 * u]), __uint_as_float(r[2 * u + 1])), sc);
-        if constexpr (kCapped) {
+        if constexpr (MODE == kCapFar) {
+#pragma unroll
+            for (int u = 0; u < 16; ++u) v[u] = __fmul2_rn(tanh_any2(v[u]), make_float2(cap2, cap2));
+        } else if constexpr (kCapped) {
             float big = 0.f;
 #pragma unroll
             for (int u = 0; u < 16; ++u) big = fmaxf(big, fmaxf(fabsf(v[u].x), fabsf(v[u].y)));
@@ -240,15 +247,12 @@ struct RowScores {
             } else if (!__any_sync(0xffffffffu, big > 1.f)) {
 #pragma unroll
                 for (int u = 0; u < 16; ++u) v[u] = __fmul2_rn(tanh_poly2(v[u]), make_float2(cap2, cap2));
-            } else {   // tanh(u) = 1 - 2 / (2^(2u log2e) + 1): right at both ends
+            } else {
 #pragma unroll
-                for (int u = 0; u < 16; ++u) {
-                    v[u].x = cap2 * (1.f - __fdividef(2.f, ex2(v[u].x * (2.f * kLog2e)) + 1.f));
-                    v[u].y = cap2 * (1.f - __fdividef(2.f, ex2(v[u].y * (2.f * kLog2e)) + 1.f));
-                }
+                for (int u = 0; u < 16; ++u) v[u] = make_float2(cap2 * tanh_exp(v[u].x), cap2 * tanh_exp(v[u].y));
             }
         }
-        if (MODE == kBias || (MODE == kCap && slope != 0.f)) {
+        if (MODE == kBias || (kCappedOnline && slope != 0.f)) {
             if (side != 0) {
                 const float s = side > 0 ? slope : -slope, base = s * ((float)e0 - place);
 #pragma unroll
@@ -298,7 +302,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_tmem, uint32_t o_tmem, c
         }
     };
     // pass 1: the row max over the 128 scores.  Keys 64..127 stay in registers
-    // (rh) for pass 2; keys 0..63 are read again (kCap: they are put back changed).
+    // (rh) for pass 2; keys 0..63 are read again (kCap, kCapFar: they are put back changed).
     uint32_t rh[2][32];
     float m8[8];
 #pragma unroll
@@ -326,7 +330,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_tmem, uint32_t o_tmem, c
             rs.apply(r, c);
             mask(r, c);
             look(r);
-            if constexpr (MODE == kCap) tmem_st_32x32b_x32(s_tmem + c, r);
+            if constexpr (rs.kCappedOnline) tmem_st_32x32b_x32(s_tmem + c, r);
         }
     } else {
         uint32_t r01[2][32];
@@ -380,7 +384,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_tmem, uint32_t o_tmem, c
         l *= alpha;
         if (grow) m_ref = mx;
     }
-    if constexpr (MODE == kCap) tmem_st_wait();
+    if constexpr (rs.kCappedOnline) tmem_st_wait();
     // pass 2: P = 2^(s - m_ref), at most 2^kRescaleLog2, in f32, stored as
     // packed 16-bit pairs (key 2c in the low half of column c) into columns
     // 64..127 of S_t, which pass 1 has read.  A row that has seen no key yet has
@@ -413,7 +417,7 @@ __device__ __forceinline__ void softmax_tile(uint32_t s_tmem, uint32_t o_tmem, c
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if constexpr (MODE == kBias) rs.apply(r0[h], 32 * h);
-            if constexpr (MODE != kCap) mask(r0[h], 32 * h);
+            if constexpr (!rs.kCappedOnline) mask(r0[h], 32 * h);
             p_store(r0[h], 64 + 16 * h, with_poly);
         }
     };
@@ -704,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 left = ok ? limit_of(p, i, token, sh.prefix) - top : kNoRow;
                 left_min = __reduce_min_sync(0xffffffffu, left);
                 place = key_beside(i.lq, i.lk, token) - top;
-                if constexpr (MODE == kBias || MODE == kCap)
+                if constexpr (MODE == kBias || rs.kCappedOnline)
                     rs.slope = p.slopes && ok ? p.slopes[i.kvh * p.group + r_in % p.group] * kLog2e : 0.f;
                 // V rows behind the document's end, in the first tile loaded: tile
                 // A's threads zero theirs, B's where A skips that tile
@@ -866,11 +870,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <int D>
 cudaError_t launch_packed(const ltx_ctx *ctx, bool f16, Mode mode, const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv,
                           const PackedParams &p) {
-    auto kern = f16 ? (mode == kCap    ? packed_kernel<D, true, kCap>
+    auto kern = f16 ? (mode == kCap      ? packed_kernel<D, true, kCap>
+                       : mode == kCapFar ? packed_kernel<D, true, kCapFar>
                        : mode == kBias ? packed_kernel<D, true, kBias>
                                        : packed_kernel<D, true, kPlain>)
                     : (mode == kCap        ? packed_kernel<D, false, kCap>
                        : mode == kCapFixed ? packed_kernel<D, false, kCapFixed>
+                       : mode == kCapFar   ? packed_kernel<D, false, kCapFar>
                        : mode == kBias     ? packed_kernel<D, false, kBias>
                                            : packed_kernel<D, false, kPlain>);
     cudaError_t e = allow_smem(ctx, reinterpret_cast<const void *>(kern), Smem<D>::BYTES);
@@ -941,7 +947,7 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const ltx_packed_attention
     if (!(scale > 0.f) || !std::isfinite(scale) || !(softcap >= 0.f) || !std::isfinite(softcap))
         return fail(ctx, LTX_ERR_INVALID_ARG, "%s: scale must be finite and > 0, softcap finite and >= 0", w);
     if (!std::isfinite(scale * kLog2e) || !std::isfinite(softcap * kLog2e) ||
-        (softcap > 0.f && (!std::isfinite(scale / softcap) || !std::isfinite(2.f * kLog2e / softcap))))
+        (softcap > 0.f && (!std::isnormal(scale / softcap) || !std::isnormal(softcap))))
         return fail(ctx, LTX_ERR_INVALID_ARG, "%s: scale, softcap or their quotient leaves f32", w);
     if (prefix_dev && !causal) return fail(ctx, LTX_ERR_INVALID_ARG, "%s: a prefix needs the causal mask", w);
     if (docs == 0 || rows_q == 0) return LTX_OK;
@@ -997,7 +1003,8 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const ltx_packed_attention
     // at a time, 942 all together, 900 in eights.)
     p.head_group = (int)std::clamp<int64_t>((32 << 20) / std::max<int64_t>(1, (int64_t)rows_k * head_dim * 4), 1, kv_heads);
     const bool fixed = !slopes_dev && v_dtype == LTX_BF16 && softcap * kLog2e <= kFixedCap;
-    const Mode mode = softcap > 0.f ? (fixed ? kCapFixed : kCap) : slopes_dev ? kBias : kPlain;
+    const bool far = softcap * kLog2e > kExpCap;
+    const Mode mode = softcap > 0.f ? (fixed ? kCapFixed : far ? kCapFar : kCap) : slopes_dev ? kBias : kPlain;
     const cudaError_t e = head_dim == 64 ? launch_packed<64>(ctx, v_dtype == LTX_F16, mode, tq, tk, tv, p)
                                          : launch_packed<128>(ctx, v_dtype == LTX_F16, mode, tq, tk, tv, p);
     return e == cudaSuccess ? LTX_OK : cuda_fail(ctx, e, w);

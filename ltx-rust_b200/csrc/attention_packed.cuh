@@ -51,18 +51,6 @@ __device__ __forceinline__ int limit_of(const PackedParams &p, const Item &it, i
 // the softmax does not see and f32 scores would lose bits to.
 __device__ __forceinline__ int key_beside(int lq, int lk, int t) { return max(t + lk - lq, 0); }
 
-// How a raw score becomes one in the log2 domain when it is capped or biased.
-struct ScoreMod {
-    float scale, twice_over_cap, cap2;   // scale; 2 log2e / cap (0 = no cap); cap log2e
-    float slope2, place;                 // slope log2e (0 = no bias), the row's key less the tile's first
-    __device__ __forceinline__ float operator()(float s, int e) const {
-        s *= scale;
-        // tanh(u) = 1 - 2 / (2^(2u log2e) + 1): absolute error of some 1e-7, right at both ends
-        s = twice_over_cap > 0.f ? cap2 * (1.f - __fdividef(2.f, ex2(s * twice_over_cap) + 1.f)) : s * kLog2e;
-        return s - slope2 * fabsf(place - (float)e);
-    }
-};
-
 // 2^x on the FMA pipe, two at a time, as exp2_fma2 of attention.cu: x = n + f with
 // n = rint(x), 2^f by a cubic (7.7e-5 relative, under f16's half step), 2^n added
 // to the exponent; below 2^-120 it stays there.  Not for a NaN (whose exponent the
@@ -102,6 +90,27 @@ __device__ __forceinline__ float2 tanh_small2(float2 u) {
     q = __ffma2_rn(q, z, make_float2(h0, h0));
     return __fmul2_rn(q, u);
 }
+
+// tanh(u) = 1 - 2 / (2^(2u log2e) + 1): right at both ends, absolute error at most 4e-7
+__device__ __forceinline__ float tanh_exp(float u) { return 1.f - __fdividef(2.f, ex2(u * (2.f * kLog2e)) + 1.f); }
+// With the polynomial where that would be many times a small u's last bits, which a
+// large cap turns into a score's: relative error 3e-6 of any u.
+__device__ __forceinline__ float2 tanh_any2(float2 u) {
+    const float2 s = tanh_small2(u);
+    return make_float2(fabsf(u.x) <= 0.5f ? s.x : tanh_exp(u.x), fabsf(u.y) <= 0.5f ? s.y : tanh_exp(u.y));
+}
+
+// How two raw scores of a key, of neighbouring rows, become scores in the log2
+// domain when they are capped or biased.
+struct ScoreMod {
+    float2 scale;      // scale / cap, or scale log2e without a cap
+    float cap2;        // cap log2e, 0 without
+    __device__ __forceinline__ float2 operator()(float2 s, float2 slope2, float2 away) const {   // slope log2e, distance
+        s = __fmul2_rn(s, scale);
+        if (cap2 > 0.f) s = __fmul2_rn(tanh_any2(s), make_float2(cap2, cap2));
+        return make_float2(s.x - slope2.x * fabsf(away.x), s.y - slope2.y * fabsf(away.y));
+    }
+};
 
 // Two f32 to a pair of f16 or bf16, the first in the low half.
 template <bool F16>

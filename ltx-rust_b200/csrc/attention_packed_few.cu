@@ -380,10 +380,9 @@ __global__ void __launch_bounds__(kFewThreads, 1)
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const bool modified = p.softcap > 0.f || p.slopes;
         ScoreMod mod{};
-        mod.scale = p.scale;
-        mod.twice_over_cap = p.softcap > 0.f ? 2.f * kLog2e / p.softcap : 0.f;
+        const float sl2 = p.scale * kLog2e, over = p.softcap > 0.f ? p.scale / p.softcap : sl2;
+        mod.scale = make_float2(over, over);
         mod.cap2 = p.softcap * kLog2e;
-        const float sl2 = p.scale * kLog2e;
         uint32_t used = 0, tile = 0, piece = 0;
         for_pieces(p, start, length, [&](const DocWork &d, int doc, const Piece &w) {
             softmax_sync();   // the row words of the piece before have been read
@@ -430,16 +429,19 @@ __global__ void __launch_bounds__(kFewThreads, 1)
                     const int places[4] = {place.x, place.y, place.z, place.w};
                     const int lims[4] = {lim.x, lim.y, lim.z, lim.w};
                     const float refs[4] = {ref.x, ref.y, ref.z, ref.w};
+                    if (modified) {
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            const float2 v = mod(make_float2(y[r4 + e], y[r4 + e + 1]), make_float2(slopes[e], slopes[e + 1]),
+                                                 make_float2((float)(places[e] - kv), (float)(places[e + 1] - kv)));
+                            y[r4 + e] = v.x;
+                            y[r4 + e + 1] = v.y;
+                        }
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float &v = y[r4 + e];
-                        if (modified) {
-                            mod.slope2 = slopes[e];
-                            mod.place = (float)(places[e] - kv);
-                            v = mod(v, 0);
-                        } else {
-                            v *= sl2;
-                        }
+                        if (!modified) v *= sl2;
                         if (kv >= lims[e]) v = -INFINITY;
                         over |= v > refs[e] + kRescaleLog2;
                     }

@@ -608,6 +608,29 @@ def test_attention_packed_distance_of_rows_far_from_all_keys(ctx, lk, others):
     within(out[rows], want, tol)
 
 
+@pytest.mark.parametrize("cap", [300.0, 3e3, 1e5, 1e8, 1e30])
+@pytest.mark.parametrize("vt", [BF16, F16])
+@pytest.mark.parametrize("lq,lk", [([300], [333]), ([2, 1], [3000, 777])])
+def test_attention_packed_cap_far_above_the_scores(ctx, lq, lk, vt, cap):
+    """A cap far above the scores hardly changes them, whatever f32 makes of 1 beside scores over the cap."""
+    import ltx_b200
+    h, d = 2, 128
+    g = gen(sum(lq), int(math.log2(cap)))
+    q, k, v = normal(g, sum(lq), h * d, std=3.0), normal(g, sum(lk), h * d), normal(g, sum(lk), h * d, dtype=vt)
+    out = torch.zeros_like(q)
+    ltx_b200.attention_packed(ctx, q, k, v, out, offsets(lq), offsets(lk), h, h, 1 / math.sqrt(d), softcap=cap)
+    ctx.synchronize()
+    # attention64's bound for uncapped scores; the capped ones differ by s^3 / 3 cap^2, which is in `want`, and the tanh
+    # moves them by at most 2^-17 of themselves, or with caps up to 355 by 4e-7 of the cap (in both directions of the
+    # weight and its sum)
+    want, _ = attention64(q, k, v, lq, lk, h, h, d, 1 / math.sqrt(d), cap, None, False, None)
+    _, tol = attention64(q, k, v, lq, lk, h, h, d, 1 / math.sqrt(d), 0.0, None, False, None)
+    big = max(float((q[a:b].to(F64).view(-1, h, d).transpose(0, 1) @ k[c:e].to(F64).view(-1, h, d).permute(1, 2, 0)).abs().max())
+              for a, b, c, e in zip([0, lq[0]], [lq[0], sum(lq)], [0, lk[0]], [lk[0], sum(lk)]) if b > a) / math.sqrt(d)
+    vmax = float(v.abs().max())
+    within(out, want, tol + 2 * vmax * (big * 2.0 ** -17 + (cap * 4e-7 if cap <= 355 else 0)))
+
+
 @pytest.mark.parametrize("kw", [{}, dict(slope=True), dict(softcap=60.0), dict(softcap=20.0)])
 @pytest.mark.parametrize("lq,lk", [(256, 256), (130, 512), (1, 3000)])
 def test_attention_packed_a_nan_that_a_row_sees_stays_one(ctx, lq, lk, kw):
