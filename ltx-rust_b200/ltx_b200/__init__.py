@@ -292,11 +292,12 @@ def _dense(ctx, what, name, t, dtype, shape):
 
 def _rows(ctx, what, name, t, dtypes, rows, cols):
     """(address, leading dimension) of a CUDA matrix [rows, cols] of the context's device with contiguous rows that do
-    not overlap; LtxError for any other.  A single row's stride says nothing, so its length stands for it."""
+    not overlap; LtxError for any other.  A single row's stride says nothing, so its length stands for it, and neither
+    does the step inside rows of one value."""
     if t.get_device() != ctx.device or t.dtype not in dtypes or t.shape != (rows, cols):
         _refuse(ctx, what, name, t, dtypes, (rows, cols))
     ld, step = t.stride()
-    if step == 1 and ld >= cols:
+    if (step == 1 or cols == 1) and ld >= cols:
         return t.data_ptr(), ld
     if rows and cols and ((step != 1 and cols > 1) or (ld < cols and rows > 1)):
         _refuse(ctx, what, name, t, dtypes, (rows, cols))

@@ -275,6 +275,26 @@ def test_gemm_adapters_strides_and_odd_rows(ctx, epi):
     adapter_case(ctx, 300, 200, 128, 16, runs(300, [4, 90], 3), epi, 3, x_pad=24, o_pad=4)
 
 
+def test_one_column_of_a_larger_matrix(ctx):
+    """One output, or one head of one value, that is a column of a larger matrix, its inner stride not 1."""
+    import ltx_b200
+    g = gen(61)
+    x, w = normal(g, 5, 64), normal(g, 1, 64)
+    full = torch.full((5, 6), 7.0, device="cuda")
+    out = full[:, ::3][:, 1:]
+    assert out.stride() == (6, 3)
+    none = torch.zeros(0, 8, 64, device="cuda", dtype=BF16), torch.zeros(0, 1, 8, device="cuda", dtype=BF16)
+    ltx_b200.gemm_adapters(ctx, x, w, out, ints([-1] * 5), *none, torch.zeros(0, device="cuda"), epilogue=2)
+    q = torch.full((5, 6), 4.0, device="cuda")
+    ltx_b200.qk_norm_rope(ctx, q[:, ::3][:, 1:], None, q[:, ::3][:, 1:], None, 1, 0, None, None, eps=0.0)
+    ctx.synchronize()
+    want, size = x.to(F64) @ w.to(F64).t(), x.to(F64).abs() @ w.to(F64).abs().t()
+    within(out, want, size * 68 * 2.0 ** -24)
+    within(q[:, 3:4], torch.ones_like(q[:, 3:4], dtype=F64), 8 * 2.0 ** -24)
+    full[:, 3], q[:, 3] = 7, 4
+    assert bool((full == 7).all()) and bool((q == 4).all())
+
+
 @pytest.mark.parametrize("epi", [0, 2])
 def test_gemm_adapters_without_any(ctx, epi):
     """Every row without an adapter is the plain projection; an empty pool too."""

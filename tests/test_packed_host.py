@@ -85,3 +85,15 @@ def test_wrong_shapes_are_refused():
     t = fake(4, 8, dtype=torch.float32)
     assert kind_of(L.qk_norm_rope, q, None, q, None, 1, 0, t, None) == "INVALID_ARG"
     assert kind_of(L.rope_table, fake(3, dtype=torch.int32), t, t) == "SHAPE"
+
+
+def test_rows_of_one_value_keep_their_stride():
+    """A column of a larger matrix, whatever its inner stride, is read at its rows' distance."""
+    column = Fake(torch.zeros(5, 6, dtype=BF16)[:, ::3][:, 1:])
+    assert column.stride() == (6, 3) and tuple(column.shape) == (5, 1)
+    assert L._rows(CTX, "t", "x", column, (BF16,), 5, 1)[1] == 6
+    assert L._rows(CTX, "t", "x", Fake(torch.zeros(5, 1, dtype=BF16)), (BF16,), 5, 1)[1] == 1
+    assert L._rows(CTX, "t", "x", Fake(torch.zeros(5, 8, dtype=BF16)[:1, :6]), (BF16,), 1, 6)[1] >= 6
+    with pytest.raises(L.LtxError) as e:
+        L._rows(CTX, "t", "x", Fake(torch.zeros(1, 1, dtype=BF16).expand(5, 1)), (BF16,), 5, 1)
+    assert e.value.kind == "SHAPE"
