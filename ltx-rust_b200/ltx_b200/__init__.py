@@ -298,7 +298,7 @@ def _rows(ctx, what, name, t, dtypes, rows, cols):
         _refuse(ctx, what, name, t, dtypes, (rows, cols))
     ld, step = t.stride()
     if (step == 1 or cols == 1) and ld >= cols:
-        return t.data_ptr(), ld
+        return t.data_ptr(), ld if rows > 1 else cols
     if rows and cols and ((step != 1 and cols > 1) or (ld < cols and rows > 1)):
         _refuse(ctx, what, name, t, dtypes, (rows, cols))
     return t.data_ptr(), cols

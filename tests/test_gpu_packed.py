@@ -275,6 +275,24 @@ def test_gemm_adapters_strides_and_odd_rows(ctx, epi):
     adapter_case(ctx, 300, 200, 128, 16, runs(300, [4, 90], 3), epi, 3, x_pad=24, o_pad=4)
 
 
+def test_one_row_of_a_matrix_of_unaligned_rows(ctx):
+    """A single aligned row whose matrix has a leading dimension that 16-byte loads could not take."""
+    import ltx_b200
+    g = gen(62)
+    buf, w = normal(g, 4, 68), normal(g, 24, 64)
+    none = torch.zeros(0, 8, 64, device="cuda", dtype=BF16), torch.zeros(0, 24, 8, device="cuda", dtype=BF16)
+    out = torch.zeros(1, 24, device="cuda")
+    x = buf[2:3, :64]
+    ltx_b200.gemm_adapters(ctx, x, w, out, ints([-1]), *none, torch.zeros(0, device="cuda"), epilogue=2)
+    qkv = normal(g, 4, 3 * 64 + 4)[2:3]
+    q, k, v = qkv[:, :64], qkv[:, 64:128], qkv[:, 128:192]
+    o = torch.zeros(1, 64, device="cuda", dtype=BF16)
+    ltx_b200.attention_packed(ctx, q, k, v, o, ints([0, 1]), ints([0, 1]), 1, 1, 1.0, head_dim=64)
+    ctx.synchronize()
+    within(out, x.to(F64) @ w.to(F64).t(), x.to(F64).abs() @ w.to(F64).abs().t() * 68 * 2.0 ** -24)
+    assert torch.equal(o, v)
+
+
 def test_one_column_of_a_larger_matrix(ctx):
     """One output, or one head of one value, that is a column of a larger matrix, its inner stride not 1."""
     import ltx_b200

@@ -97,3 +97,11 @@ def test_rows_of_one_value_keep_their_stride():
     with pytest.raises(L.LtxError) as e:
         L._rows(CTX, "t", "x", Fake(torch.zeros(1, 1, dtype=BF16).expand(5, 1)), (BF16,), 5, 1)
     assert e.value.kind == "SHAPE"
+
+
+def test_a_single_rows_stride_does_not_count():
+    """One row of a matrix whose rows are not 16-byte aligned is as good as any other that is."""
+    row = Fake(torch.zeros(3, 68, dtype=BF16)[2:, :64])
+    assert row.stride() == (68, 1)
+    assert L._rows(CTX, "t", "x", row, (BF16,), 1, 64)[1] == 64
+    assert L._rows(CTX, "t", "x", Fake(torch.zeros(3, 68, dtype=BF16)[:, :64]), (BF16,), 3, 64)[1] == 68
