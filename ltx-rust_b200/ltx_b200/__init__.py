@@ -339,6 +339,8 @@ def qk_norm_rope(ctx: "Context", q, k, q_out, k_out, heads, kv_heads, cos, sin, 
     qop, ldqo = _rows(ctx, what, "q_out", q_out, (dt,), rows, heads * d)
     kp = kop = gq = gk = cp = sp = pp = ldk = ldko = table = half = 0
     if kv_heads:
+        if k is None or k_out is None:
+            raise LtxError(1, f"{what}: {kv_heads} key heads without k or k_out")
         kp, ldk = _rows(ctx, what, "k", k, (dt,), rows, kv_heads * d)
         kop, ldko = _rows(ctx, what, "k_out", k_out, (dt,), rows, kv_heads * d)
     if gamma_q is not None:

@@ -105,3 +105,9 @@ def test_a_single_rows_stride_does_not_count():
     assert row.stride() == (68, 1)
     assert L._rows(CTX, "t", "x", row, (BF16,), 1, 64)[1] == 64
     assert L._rows(CTX, "t", "x", Fake(torch.zeros(3, 68, dtype=BF16)[:, :64]), (BF16,), 3, 64)[1] == 68
+
+
+def test_key_heads_without_keys_are_refused():
+    q = fake(4, 128)
+    assert kind_of(L.qk_norm_rope, q, None, q, None, 1, 1, None, None) == "INVALID_ARG"
+    assert kind_of(L.qk_norm_rope, q, q, q, None, 1, 1, None, None) == "INVALID_ARG"
