@@ -42,7 +42,7 @@ int work_alloc(ltx_ctx *ctx, size_t bytes, void **out) {
         props.location.type = cudaMemLocationTypeDevice;
         props.location.id = ctx->device;
         LTX_CUDA_TRY(ctx, cudaMemPoolCreate(&ctx->pool, &props));
-        uint64_t hold = ~0ull;   // freed blocks stay in the pool for the next call
+        uint64_t hold = kKeptWorkBytes;   // what lies free beyond that goes back to the device at the next synchronisation
         LTX_CUDA_TRY(ctx, cudaMemPoolSetAttribute(ctx->pool, cudaMemPoolAttrReleaseThreshold, &hold));
     }
     if (keep && ctx->kept) {   // behind the calls that use it

@@ -878,6 +878,26 @@ def test_first_calls_of_a_context_captured():
     ctx.close()
 
 
+def test_large_workspaces_go_back_to_the_device():
+    """What one call needs beyond 64 MB is free for other allocators after the next synchronisation."""
+    import ltx_b200
+    ctx = ltx_b200.Context(0)
+    m, rank = 1 << 18, 256          # 2 parts x m x rank x 2 bytes: 256 MB
+    x, w = torch.ones(m, 8, device="cuda", dtype=BF16), torch.ones(8, 8, device="cuda", dtype=BF16)
+    a, b = torch.ones(1, rank, 8, device="cuda", dtype=BF16), torch.ones(1, 8, rank, device="cuda", dtype=BF16)
+    c, out, idx = torch.ones(1, device="cuda"), torch.zeros(m, 8, device="cuda"), torch.zeros(m, device="cuda", dtype=torch.int32)
+    ltx_b200.gemm_adapters(ctx, x[:256], w, out[:256], idx[:256], a, b, c, epilogue=2)
+    ctx.synchronize()
+    before = torch.cuda.mem_get_info(0)[0]
+    for _ in range(2):
+        ltx_b200.gemm_adapters(ctx, x, w, out, idx, a, b, c, epilogue=2)
+        ctx.synchronize()
+    torch.cuda.synchronize()
+    assert before - torch.cuda.mem_get_info(0)[0] <= 96 << 20
+    assert bool((out == 8 + 8 * rank).all())
+    ctx.close()
+
+
 # ── refusals of the C entry points ───────────────────────────────────────────
 
 def refused(ctx, kind, fn, *args, **kw):
