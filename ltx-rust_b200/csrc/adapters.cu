@@ -35,6 +35,7 @@ constexpr int kMaxWords = LTX_MAX_ADAPTERS / 32;
 struct AdapterParams {
     int m, n, k, rank, adapters, rank_blocks, parts, splits, m_tiles, n_tiles, group_m;
     int gate_rows;
+    int early;                          // the projection starts while low is formed
     int tile_lanes, unit, low_stages;   // low_kernel: clusters per tile, adapters in one product, depth of its ring
     const int *idx, *gate_idx;
     const float *coeff, *bias, *gate;
@@ -1177,7 +1178,7 @@ cudaError_t run_project(const ltx_ctx *ctx, AdapterParams p, int epilogue, const
     p.group_m = group_of(p, TN);
     const int grid = p.splits > 1 ? (int)tiles * p.splits : (int)std::min<int64_t>(tiles, sms);
     auto go = [&](auto kern) {
-        return launch(ctx, kern, grid, ProjCfg<TN>::THREADS, ProjCfg<TN>::BYTES, ProjCfg<TN>::BYTES, p.splits, p.adapters > 0, tw, tx, tb, p);
+        return launch(ctx, kern, grid, ProjCfg<TN>::THREADS, ProjCfg<TN>::BYTES, ProjCfg<TN>::BYTES, p.splits, p.early, tw, tx, tb, p);
     };
     switch (epilogue) {
     case LTX_EPI_BF16: return go(project_kernel<TN, LTX_EPI_BF16>);
@@ -1195,7 +1196,7 @@ cudaError_t run_pair(const ltx_ctx *ctx, AdapterParams p, int epilogue, const CU
     p.group_m = group_of(p, PairCfg::TOKENS);
     const int grid = 2 * (int)std::min<int64_t>((int64_t)p.m_tiles * p.n_tiles, ctx->sm_count / 2);
     auto go = [&](auto kern) {
-        return launch(ctx, kern, grid, PairCfg::THREADS, PairCfg::BYTES, PairCfg::BYTES, 2, p.adapters > 0, tw, tx, tb, p);
+        return launch(ctx, kern, grid, PairCfg::THREADS, PairCfg::BYTES, PairCfg::BYTES, 2, p.early, tw, tx, tb, p);
     };
     switch (epilogue) {
     case LTX_EPI_BF16: return go(project_pair_kernel<LTX_EPI_BF16>);
@@ -1275,6 +1276,10 @@ extern "C" int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args) {
     // 59 / 42; 160 x 12000 x 640, 8 of 8 34 / 32; 256 x 16384 x 4096, 4 of 64 56 / 70.
     if (tn == 256 && !pair && (int64_t)std::min(adapters, 256) * p.rank_blocks * p.parts * 4 > (k + 63) / 64) tn = 128;
     const int tl = std::min(tn, 64);
+    // The waits of a projection that starts early count low_kernel's time in their 2 s.
+    // That takes 6e-13 s per value of x and product (tiles of all different adapters of
+    // rank 256, A from HBM), so beyond a tenth of the limit the projection comes after it.
+    p.early = adapters && (int64_t)m * k * std::min(adapters, tl) * ((rank + BM - 1) / BM) <= (int64_t)1 << 38;
     CUtensorMap tw, tx, txl, ta, tb;
     bool ok = make_map(&tw, w_dev, n, k, ldw, BM) && make_map(&tx, x_dev, m, k, ldx, pair ? 128 : tn);
     ta = tb = txl = tx;

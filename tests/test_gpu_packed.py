@@ -256,6 +256,26 @@ def test_gemm_adapters_more_adapter_blocks_than_others(ctx, m, n, k, rank, adapt
     adapter_case(ctx, m, n, k, rank, runs(m, lengths, adapters, start=1), epi, adapters, bias=False, gate=2)
 
 
+def test_gemm_adapters_long_low_rank_products(ctx):
+    """So many rows, each with one of 64 adapters of the largest rank, that the low-rank product alone takes a good part
+    of the time that a kernel's waits may last."""
+    import ltx_b200
+    m, n, k, rank, adapters = (1 << 17) + 77, 72, 16384, 256, 64
+    g = gen(m, k)
+    x = torch.empty(m, k, device="cuda", dtype=BF16)
+    for i in range(0, m, 4096):
+        x[i:i + 4096] = normal(g, min(4096, m - i), k)
+    w, a, b = normal(g, n, k, std=0.05), normal(g, adapters, rank, k, std=0.05), normal(g, adapters, n, rank, std=0.2)
+    coeff = torch.rand(adapters, device="cuda", generator=g) + 0.5
+    idx = (torch.arange(m, device="cuda") * 37 % (adapters + 1) - 1).to(torch.int32)
+    out = torch.zeros(m, n, device="cuda")
+    ltx_b200.gemm_adapters(ctx, x, w, out, idx, a, b, coeff, epilogue=2)
+    ctx.synchronize()
+    for rows in (slice(0, 300), slice(m // 2, m // 2 + 300), slice(m - 300, m)):
+        y, tol = adapters64(x[rows], w, idx[rows], a, b, coeff, 2, None, None, None, None)
+        within(out[rows], y, tol)
+
+
 @pytest.mark.parametrize("m,n", [(20, 300), (300, 700), (2500, 4096)])
 def test_gemm_adapters_after_a_call_that_left_nan(ctx, m, n):
     """What an earlier call left in the workspace, NaN here, reaches no row of a later one."""
