@@ -402,7 +402,7 @@ int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args);
  * or 128; out overlaps no input.  What k and v hold outside the documents, or
  * in other documents, never reaches a row, NaN and infinities included; a
  * non-finite v row inside a document may reach every row of the document.
- * At most 2^29 rows.  Under a cap without slopes (bf16 v, softcap up to 51)
+ * At most 2^29 rows and 2^24 documents.  Under a cap without slopes (bf16 v, softcap up to 51)
  * probabilities are kept unnormalised up to e^softcap, so sums over a row of
  * |v| have to stay under 2^52. */
 typedef struct {

@@ -947,6 +947,8 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const ltx_packed_attention
         return fail(ctx, LTX_ERR_SHAPE, "%s: %d documents, %d x %d rows, %d heads over %d key heads", w, docs, rows_q,
                     rows_k, heads, kv_heads);
     if (rows_q > 1 << 29 || rows_k > 1 << 29) return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: more than 2^29 rows", w);
+    // a search through the offsets, 32 documents at a time, has to stay well under the 2 s that the others wait for it
+    if (docs > 1 << 24) return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: more than 2^24 documents", w);
     if (heads / kv_heads > 128) return fail(ctx, LTX_ERR_UNSUPPORTED, "%s: more than 128 heads per key head", w);
     if (!(scale > 0.f) || !std::isfinite(scale) || !(softcap >= 0.f) || !std::isfinite(softcap))
         return fail(ctx, LTX_ERR_INVALID_ARG, "%s: scale must be finite and > 0, softcap finite and >= 0", w);

@@ -714,6 +714,21 @@ def test_attention_packed_a_nan_that_a_row_sees_stays_one(ctx, lq, lk, kw):
     assert torch.equal(out.isnan().all(1), torch.arange(lq, device="cuda") == lq // 2)
 
 
+def test_attention_packed_the_most_documents(ctx):
+    """2^24 documents, all but the last without rows: found in time; one more is refused."""
+    import ltx_b200
+    docs, g = 1 << 24, gen(24)
+    q, k, v = normal(g, 300, 128), normal(g, 400, 128), normal(g, 400, 128)
+    out = torch.zeros_like(q)
+    o = torch.zeros(2, docs + 2, device="cuda", dtype=torch.int32)
+    o[0, docs:], o[1, docs:] = 300, 400
+    ltx_b200.attention_packed(ctx, q, k, v, out, o[0, :docs + 1], o[1, :docs + 1], 1, 1, 0.1)
+    ctx.synchronize()
+    want, tol = attention64(q, k, v, [300], [400], 1, 1, 128, 0.1, 0.0, None, False, None)
+    within(out, want, tol)
+    refused(ctx, "UNSUPPORTED", ltx_b200.attention_packed, q, k, v, out, o[0], o[1], 1, 1, 0.1)
+
+
 def test_attention_packed_nothing_to_do(ctx):
     import ltx_b200
     q = torch.ones(4, 128, device="cuda", dtype=BF16)
