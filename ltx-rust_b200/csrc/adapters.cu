@@ -124,7 +124,7 @@ __device__ __forceinline__ void build_list(const AdapterParams &p, int m0, int t
     for (int i = tid; i < TN; i += NT) {
         int a = m0 + i < p.m ? p.idx[m0 + i] : -1;
         if (a >= p.adapters) {
-            atomicExch(p.flag, kErrBadAdapter);
+            report_index(p.flag, kErrBadAdapter);
             a = -1;
         }
         s.tok[i] = (int16_t)max(a, -1);
@@ -402,7 +402,7 @@ struct Ahead {
 __device__ __forceinline__ int gate_row(const AdapterParams &p, int m, int lane) {
     int g = p.gate && p.gate_idx && m + lane < p.m ? __ldg(p.gate_idx + m + lane) : 0;
     if ((unsigned)g >= (unsigned)p.gate_rows && p.gate) {
-        atomicExch(p.flag, kErrBadGate);
+        report_index(p.flag, kErrBadGate);
         g = g < 0 ? 0 : p.gate_rows - 1;
     }
     return g;

@@ -34,7 +34,7 @@ struct Item {
 // the array holds; an entry that descends or lies outside raises the flag.
 __device__ __forceinline__ void doc_span(const int *off, int i, int rows, int *flag, int &s, int &e) {
     const int a = off[i], b = off[i + 1];
-    if (a < 0 || b < a || b > rows) atomicExch(flag, kErrBadOffsets);
+    if (a < 0 || b < a || b > rows) report_index(flag, kErrBadOffsets);
     s = min(max(a, 0), rows);
     e = min(max(b, s), rows);
 }

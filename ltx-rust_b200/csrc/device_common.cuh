@@ -66,6 +66,10 @@ __device__ __forceinline__ uint64_t global_ns() {
     return t;
 }
 
+// Reports a bad index value, unless something is reported already: a wait that
+// gave up says more, and puts its code in any other's place.
+__device__ __forceinline__ void report_index(int *flag, int code) { atomicCAS(flag, 0, code); }
+
 // System-scope acquire load / release store of a 32-bit stamp (a word another
 // GPU writes or reads over NVLink).
 __device__ __forceinline__ uint32_t ld_acquire_sys(const uint32_t *p) {

@@ -140,7 +140,7 @@ __device__ __forceinline__ int64_t table_row(const NormRopeParams &p, int row) {
     if (!p.pos) return row % p.table_rows;
     const int r = p.pos[row];
     if ((unsigned)r >= (unsigned)p.table_rows) {
-        atomicExch(p.flag, kErrBadPosition);
+        report_index(p.flag, kErrBadPosition);
         return r < 0 ? 0 : p.table_rows - 1;
     }
     return r;

@@ -756,6 +756,39 @@ def test_attention_packed_reports_bad_offsets(ctx):
     ctx.synchronize()
 
 
+def test_a_bad_index_does_not_hide_a_wait_that_gave_up():
+    """Whichever comes first, a wait that gave up is what the next synchronisation reports."""
+    import ltx_b200
+    ctx = ltx_b200.Context(0)
+    q, t = torch.ones(3, 64, device="cuda", dtype=BF16), torch.ones(4, 32, device="cuda")
+    flag = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def bad_calls():
+        ltx_b200.qk_norm_rope(ctx, q, None, q, None, 1, 0, t, t, pos=ints([1, 4, -2]))
+        ltx_b200.attention_packed(ctx, q, q, q, torch.zeros_like(q), ints([0, 9]), ints([0, 3]), 1, 1, 1.0, head_dim=64)
+        x, w = torch.ones(2, 64, device="cuda", dtype=BF16), torch.ones(8, 64, device="cuda", dtype=BF16)
+        a, b = torch.ones(1, 8, 64, device="cuda", dtype=BF16), torch.ones(1, 8, 8, device="cuda", dtype=BF16)
+        out, gate = torch.zeros(2, 8, device="cuda"), torch.ones(1, 8, device="cuda")
+        ltx_b200.gemm_adapters(ctx, x, w, out, ints([0, 1]), a, b, torch.ones(1, device="cuda"), epilogue=3, gate=gate,
+                               gate_idx=ints([0, 1]))
+
+    for first in (True, False):
+        if not first:
+            bad_calls()
+        ctx.wait_flag(flag, 1, timeout_ms=20)
+        if first:
+            bad_calls()
+        with pytest.raises(ltx_b200.LtxError) as e:
+            ctx.synchronize()
+        assert e.value.kind == "TIMEOUT"
+    ctx.synchronize()
+    bad_calls()
+    with pytest.raises(ltx_b200.LtxError) as e:
+        ctx.synchronize()
+    assert e.value.kind == "INVALID_ARG"
+    ctx.close()
+
+
 # ── together, on other streams, captured ─────────────────────────────────────
 
 def layer(ctx, s):
