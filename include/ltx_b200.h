@@ -293,7 +293,9 @@ int ltx_attention_fwd(ltx_ctx *ctx, const void *q_dev, int64_t ldq, const void *
  * mask = None (crates/ltx-dit/src/attention.rs:228-285).  All of them are
  * inference operators, take caller-owned buffers on the context's device,
  * set the context's device for the call and restore the caller's, and may be
- * captured into a CUDA graph.  Outputs overlap no input unless said otherwise.
+ * captured into a CUDA graph (ltx_gemm_adapters with adapters, and attention of
+ * few rows, put allocation and free nodes into it: such a graph has one
+ * executable at a time and is no child of another).  Outputs overlap no input unless said otherwise.
  * Index arrays on the device are read as they are: every access they lead to
  * stays inside the buffers whatever they hold, and a bad value is reported by
  * the next ltx_ctx_synchronize. */
@@ -402,7 +404,9 @@ int ltx_gemm_adapters(ltx_ctx *ctx, const ltx_adapter_gemm *args);
  * or 128; out overlaps no input.  What k and v hold outside the documents, or
  * in other documents, never reaches a row, NaN and infinities included; a
  * non-finite v row inside a document may reach every row of the document.
- * At most 2^29 rows and 2^24 documents.  Under a cap without slopes (bf16 v, softcap up to 51)
+ * At most 2^29 rows and 2^24 documents.  How the work is cut goes by the batch's
+ * average rows and keys per document: long and single-token documents go faster
+ * in calls of their own.  Under a cap without slopes (bf16 v, softcap up to 51)
  * probabilities are kept unnormalised up to e^softcap, so sums over a row of
  * |v| have to stay under 2^52. */
 typedef struct {

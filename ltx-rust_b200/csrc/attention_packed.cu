@@ -35,10 +35,10 @@
 // Bound by the exponentials and their way from S to P: a row's tile passes max,
 // exponential and conversion in one thread while the other tile's products run (three
 // clips: tensor pipe 51% busy, special functions 41%).  One document of 8192 rows x 32
-// heads x 128: 905 us, 1215 TFLOP/s; with slopes 1410; capped, bf16 V 1480, f16 1775;
-// x 64: 778.  Three clips of 8192 rows together: 411, 907 TFLOP/s (their last tiles,
-// and what is left at the end).  4099 capped causal rows of 5 documents x 16/4 heads:
-// 47.
+// heads x 128: 900 us, 1220 TFLOP/s; with slopes 1430; capped, bf16 V 1280, f16 1775;
+// x 64: 792.  Three clips of 8192 rows together: 411, 907 TFLOP/s (1.9 us a K/V tile
+// and 8 for each of 1056 items, seven to an SM and twenty more).  4099 capped causal
+// rows of 5 documents x 16/4 heads: 47.
 // All waits are bounded (2 s) and report LTX_ERR_TIMEOUT through the flag.
 #include <cuda.h>
 #include <cuda_fp16.h>
@@ -977,7 +977,9 @@ extern "C" int ltx_attention_packed_fwd(ltx_ctx *ctx, const ltx_packed_attention
     // Few rows per document over many keys, by their averages (the host does
     // not see the offsets): the kernel whose tiles have keys as rows and whose
     // CTAs share every document.  Under some 512 keys its join and its start
-    // cost more than it saves.
+    // cost more than it saves.  Averages do badly by a batch of both kinds: 512
+    // rows and 64 single ones over 4000 keys x 32/8 heads take 636 us together, in
+    // tiles of 64 rows, 20 + 174 in two calls.
     const int some = std::min(docs, rows_q);
     const int64_t rows_per_doc = (int64_t)((rows_q + some - 1) / some) * group;
     if (rows_per_doc <= kMaxFewRows && rows_k / docs >= 512)

@@ -503,7 +503,8 @@ __global__ void __launch_bounds__(kFewThreads, 1)
                         // a row that has seen no key has reference -inf and all of its scores too
                         const float v = ex2(y[r] - (refs[e] == -INFINITY ? 0.f : refs[e]));
                         unsigned char *to = pw + r * 128 + ((chunk ^ (r & 7)) << 4);
-                        // the sum takes what the product takes: a row that one key rules is exact
+                        // bf16: the sum takes what the product takes, so a row that one key rules is exact;
+                        // f16's half step is an eighth of the output's
                         if constexpr (VF16) {
                             l[r] += v;
                             *reinterpret_cast<__half *>(to) = __float2half_rn(v);
