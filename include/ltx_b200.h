@@ -295,10 +295,11 @@ int ltx_attention_fwd(ltx_ctx *ctx, const void *q_dev, int64_t ldq, const void *
  * set the context's device for the call and restore the caller's, and may be
  * captured into a CUDA graph (ltx_gemm_adapters with adapters, and attention of
  * few rows, put allocation and free nodes into it: such a graph has one
- * executable at a time and is no child of another).  Outputs overlap no input unless said otherwise.
- * Index arrays on the device are read as they are: every access they lead to
- * stays inside the buffers whatever they hold, and a bad value is reported by
- * the next ltx_ctx_synchronize. */
+ * executable at a time and is no child of another).  Outputs overlap no input
+ * unless said otherwise.  Index arrays on the device are read as they are: every
+ * access they lead to stays inside the buffers whatever they hold, and a bad
+ * value is reported by the next ltx_ctx_synchronize (a wait that gave up before
+ * or after it is reported instead). */
 
 /* Which two values of a head's rotated part form a pair. */
 typedef enum {
